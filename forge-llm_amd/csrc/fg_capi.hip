@@ -11,6 +11,8 @@
 #include <string>
 
 #include "../../include/forge_mi355x.h"
+#include "fg_attn.h"
+#include "fg_decoder.h"
 #include "fg_device.h"
 
 namespace fg {
@@ -1135,6 +1137,165 @@ int fg_quant_fp8_row_blocks(const void* x, int64_t ldx, int x_dtype, uint8_t* q,
   return hip_status(fg::launch_quant_fp8_row_blocks(x, ldx, x_dtype, q, ldq, s, s_row, s_block, (int)M, (int)K, block,
                                                     static_cast<hipStream_t>(stream)),
                     "fg_quant_fp8_row_blocks launch");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------- between the linears
+namespace {
+
+int item_bytes(int dt) { return dt == FG_F32 ? 4 : (dt == FG_E4M3 ? 1 : 2); }
+
+// Whether `cache` can hold 16-bit values of `dtype`, or e4m3 codes, as the kernels read them.
+int check_cache(const fg_kv_cache* c, int dtype, const char* op) {
+  if (!c || !c->k || !c->v) return fail(FG_EINVAL, "%s: null cache", op);
+  if (c->num_pages <= 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->head_dim <= 0 || c->num_pages >= kMaxDim)
+    return fail(FG_EINVAL, "%s: bad cache sizes", op);
+  if (c->dtype != dtype && c->dtype != FG_E4M3)
+    return fail(FG_EINVAL, "%s: the cache holds another type than the queries' and not e4m3", op);
+  const bool fp8 = c->dtype == FG_E4M3;
+  if (fp8 && (!c->k_scale || !c->v_scale)) return fail(FG_EINVAL, "%s: an e4m3 cache needs k_scale and v_scale", op);
+  if (c->head_dim > 256 || c->head_dim % (fp8 ? 16 : 8))
+    return fail(FG_EUNSUPPORTED, "%s: head_dim %d is not a multiple of %d up to 256", op, c->head_dim, fp8 ? 16 : 8);
+  const int64_t item = item_bytes(c->dtype), strides[3] = {c->page_stride, c->head_stride, c->token_stride};
+  for (int64_t s : strides)
+    if (s < 0 || s * item % 16) return fail(FG_EINVAL, "%s: cache strides are no whole 16-byte units", op);
+  if (c->token_stride < c->head_dim && c->page_size > 1) return fail(FG_EINVAL, "%s: cache tokens overlap", op);
+  if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
+    return fail(FG_EINVAL, "%s: the cache is not 16-byte aligned", op);
+  // rows are 32-bit numbers of 16-byte units
+  const double span = ((double)(c->num_pages - 1) * c->page_stride + (double)(c->page_size - 1) * c->token_stride) * item / 16;
+  if (span >= 4294967295.0) return fail(FG_EUNSUPPORTED, "%s: the pages of one head span 64 GiB or more", op);
+  return FG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual, int64_t ldr, void* residual_out,
+                   int64_t ldro, int residual_dtype, const void* weight, int weight_dtype, float eps, void* y,
+                   int64_t ldy, int y_dtype, float* s, int64_t s_row, int64_t s_block, int32_t block, int64_t M,
+                   int64_t K, fg_stream_t stream) {
+  if (M < 0 || K <= 0 || M >= kMaxDim) return fail(FG_EINVAL, "fg_add_rmsnorm: bad sizes");
+  if (K > fg::kNormMaxK) return fail(FG_EUNSUPPORTED, "fg_add_rmsnorm: rows of more than %d columns", fg::kNormMaxK);
+  if (M == 0) return FG_OK;
+  const bool codes = y_dtype == FG_I8 || y_dtype == FG_E4M3;
+  if (!x || !y || (codes && !s) || (residual && !residual_out)) return fail(FG_EINVAL, "fg_add_rmsnorm: null tensor");
+  if (!is_float_dt(x_dtype) || (weight && !is_float_dt(weight_dtype))) return fail(FG_EINVAL, "fg_add_rmsnorm: bad dtype");
+  if (residual && residual_dtype != x_dtype && residual_dtype != FG_F32)
+    return fail(FG_EINVAL, "fg_add_rmsnorm: the residual is of x's type or fp32");
+  if (!codes && y_dtype != x_dtype) return fail(FG_EINVAL, "fg_add_rmsnorm: y is of x's type, int8 or e4m3");
+  if (block != 0 && (!codes || block < 8 || block > 512 || (block & (block - 1))))
+    return fail(FG_EINVAL, "fg_add_rmsnorm: a block of scales is a power of two from 8 to 512 columns of codes");
+  if (ldx < K || ldy < K || (residual && (ldr < K || ldro < K)))
+    return fail(FG_EINVAL, "fg_add_rmsnorm: leading dimensions too small");
+  if (codes && (s_row < 0 || s_block < 0)) return fail(FG_EINVAL, "fg_add_rmsnorm: bad scale strides");
+  fg::NormArgs a;
+  a.x = x; a.ldx = ldx; a.r = residual; a.ldr = ldr; a.ro = residual_out; a.ldro = ldro;
+  a.w = weight; a.wdt = weight_dtype; a.eps = eps; a.y = y; a.ldy = ldy; a.ydt = y_dtype;
+  a.s = s; a.s_row = s_row; a.s_block = s_block; a.log_l = block ? __builtin_ctz((unsigned)block) - 3 : -1;
+  a.K = (int)K;
+  return hip_status(fg::launch_add_rmsnorm(a, x_dtype, residual_dtype, M, static_cast<hipStream_t>(stream)),
+                    "fg_add_rmsnorm launch");
+}
+
+int fg_rope_append(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                   const void* v, int64_t v_token, int64_t v_head, void* q_out, int64_t qo_token, int64_t qo_head,
+                   int dtype, const void* positions, int32_t positions_int64, const float* table, int64_t ld_table,
+                   int64_t max_pos, int32_t rot, int32_t interleaved, const void* slots, int32_t slots_int64,
+                   const fg_kv_cache* cache, int64_t T, int32_t q_heads, fg_stream_t stream) {
+  if (T < 0 || T >= kMaxDim || q_heads <= 0 || max_pos < 0) return fail(FG_EINVAL, "fg_rope_append: bad sizes");
+  if (T == 0) return FG_OK;
+  if (dtype != FG_F16 && dtype != FG_BF16) return fail(FG_EINVAL, "fg_rope_append: q, k and v are fp16 or bf16");
+  const int bad = check_cache(cache, dtype, "fg_rope_append");
+  if (bad) return bad;
+  if (!q || !k || !v || !q_out || !positions || !table || !slots) return fail(FG_EINVAL, "fg_rope_append: null tensor");
+  if (rot < 2 || rot % 2 || rot > cache->head_dim || ld_table < rot)
+    return fail(FG_EINVAL, "fg_rope_append: rot is even, at most head_dim and at most the table's columns");
+  fg::RopeAppendArgs a;
+  a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k); a.v = static_cast<const uint16_t*>(v);
+  a.q_t = q_token; a.q_h = q_head; a.k_t = k_token; a.k_h = k_head; a.v_t = v_token; a.v_h = v_head;
+  a.qo = static_cast<uint16_t*>(q_out); a.qo_t = qo_token; a.qo_h = qo_head;
+  a.pos = positions; a.pos64 = positions_int64; a.table = table; a.ld_table = ld_table; a.max_pos = max_pos;
+  a.slots = slots; a.slots64 = slots_int64;
+  const int64_t item = item_bytes(cache->dtype);
+  a.kc = static_cast<uint8_t*>(cache->k); a.vc = static_cast<uint8_t*>(cache->v);
+  a.c_page = cache->page_stride * item; a.c_head = cache->head_stride * item; a.c_token = cache->token_stride * item;
+  a.n_slots = cache->num_pages * cache->page_size; a.page = cache->page_size;
+  a.ks = cache->k_scale; a.vs = cache->v_scale;
+  a.Hq = q_heads; a.Hk = cache->kv_heads; a.D = cache->head_dim; a.rot = rot;
+  return hip_status(fg::launch_rope_append(a, T, dtype == FG_BF16, cache->dtype == FG_E4M3, interleaved != 0,
+                                           static_cast<hipStream_t>(stream)),
+                    "fg_rope_append launch");
+}
+
+}  // extern "C"
+
+namespace {
+
+// The sizes of an attention call into `a`; a message for sizes that no plan is made for.
+const char* attn_sizes(fg::AttnArgs& a, int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                       int64_t prefix_len, int64_t max_seq_len, int64_t max_query_len, bool ragged) {
+  if (T < 0 || B < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || prefix_len < 0 || max_seq_len < 0 ||
+      max_query_len <= 0)
+    return "bad sizes";
+  if (q_heads % kv_heads) return "q_heads is no multiple of kv_heads";
+  if (!ragged && (T != B || max_query_len != 1)) return "without query_start each sequence has one query token";
+  if (T * q_heads >= kMaxDim || prefix_len >= kMaxDim - 4096 || max_seq_len >= kMaxDim - 4096 ||
+      max_query_len * q_heads >= kMaxDim || B * max_query_len * q_heads >= kMaxDim)
+    return "sizes past 32 bits";
+  a.T = (int)T; a.B = (int)B; a.Hq = q_heads; a.Hk = kv_heads; a.G = q_heads / kv_heads; a.D = head_dim;
+  a.prefix_len = (int)prefix_len; a.max_len = (int)max_seq_len; a.max_q = (int)max_query_len;
+  a.starts = ragged ? reinterpret_cast<const int32_t*>(1) : nullptr;  // the plan asks only whether there are any
+  return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fg_prefix_attention_workspace_bytes(int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                           int64_t prefix_len, int64_t max_seq_len, int64_t max_query_len,
+                                           int32_t ragged) {
+  fg::AttnArgs a = {};
+  if (attn_sizes(a, T, B, q_heads, kv_heads, head_dim, prefix_len, max_seq_len, max_query_len, ragged != 0)) return 0;
+  return T == 0 ? 0 : fg::attn_plan(a);
+}
+
+int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const fg_kv_cache* cache,
+                        const int32_t* prefix_pages, int64_t prefix_len, const int32_t* page_table, int64_t ld_pages,
+                        const int32_t* seq_lens, const int32_t* query_start, int64_t T, int64_t B, int32_t q_heads,
+                        int64_t max_seq_len, int64_t max_query_len, float scale, void* out, int64_t o_token,
+                        int64_t o_head, float* lse, void* workspace, size_t workspace_bytes, fg_stream_t stream) {
+  const int bad = check_cache(cache, dtype, "fg_prefix_attention");
+  if (bad) return bad;
+  fg::AttnArgs a = {};
+  if (const char* why = attn_sizes(a, T, B, q_heads, cache->kv_heads, cache->head_dim, prefix_len, max_seq_len,
+                                   max_query_len, query_start != nullptr))
+    return fail(FG_EINVAL, "fg_prefix_attention: %s", why);
+  if (T == 0) return FG_OK;
+  if (dtype != FG_F16 && dtype != FG_BF16) return fail(FG_EINVAL, "fg_prefix_attention: q is fp16 or bf16");
+  if (!q || !out || (B > 0 && !seq_lens) || (max_seq_len > 0 && B > 0 && !page_table) || (prefix_len > 0 && !prefix_pages))
+    return fail(FG_EINVAL, "fg_prefix_attention: null tensor");
+  if (B > 0 && ld_pages * cache->page_size < max_seq_len)
+    return fail(FG_EINVAL, "fg_prefix_attention: max_seq_len is past the page table's columns");
+  const size_t need = fg::attn_plan(a);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return fail(FG_EINVAL, "fg_prefix_attention: the workspace needs %zu bytes, 16-byte aligned", need);
+  const int64_t item = item_bytes(cache->dtype);
+  a.q = static_cast<const uint16_t*>(q); a.q_t = q_token; a.q_h = q_head;
+  a.out = static_cast<uint16_t*>(out); a.o_t = o_token; a.o_h = o_head; a.lse = lse;
+  a.k = static_cast<const uint8_t*>(cache->k); a.v = static_cast<const uint8_t*>(cache->v);
+  a.c_head = cache->head_stride * item;
+  a.c_page = (uint32_t)(cache->page_stride * item / 16); a.c_token = (uint32_t)(cache->token_stride * item / 16);
+  a.ks = cache->k_scale; a.vs = cache->v_scale;
+  a.prefix_pages = prefix_pages; a.pages = page_table; a.ld_pages = ld_pages; a.lens = seq_lens; a.starts = query_start;
+  a.page = cache->page_size; a.n_pages = (int)cache->num_pages;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return hip_status(fg::launch_attn(a, dtype == FG_BF16, cache->dtype == FG_E4M3, workspace,
+                                    static_cast<hipStream_t>(stream)),
+                    "fg_prefix_attention launch");
 }
 
 }  // extern "C"

@@ -6,9 +6,9 @@ hand-written HIP kernels in ``libforge_mi355x.so`` (C ABI: ``include/forge_mi355
 """
 from __future__ import annotations
 
-from . import errors, layouts, ops_gemm
+from . import errors, layouts, ops_decoder, ops_gemm
 from .errors import ConfigError, HardwareUnsupported, NotFound
 
 __version__ = "0.1.0"
 
-__all__ = ["ConfigError", "HardwareUnsupported", "NotFound", "errors", "layouts", "ops_gemm"]
+__all__ = ["ConfigError", "HardwareUnsupported", "NotFound", "errors", "layouts", "ops_decoder", "ops_gemm"]

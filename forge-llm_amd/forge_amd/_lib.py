@@ -55,6 +55,13 @@ class MMConfig(ctypes.Structure):
     _fields_ = [("tile_m", ctypes.c_int32), ("tile_n", ctypes.c_int32), ("reserved", ctypes.c_int32 * 6)]
 
 
+class KVCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64), ("num_pages", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
 P, I64, I32_, INT, SZ, F32_ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 
 SIGNATURES = {
@@ -80,6 +87,14 @@ SIGNATURES = {
     "fg_quant_fp8_rowwise": ([P, I64, INT, P, I64, P, I64, I64, P, P, INT, F32_, I32_, P], INT),
     "fg_quant_fp8_block": ([P, I64, INT, P, I64, P, I64, I64, I64, I32_, I32_, P, P], INT),
     "fg_quant_fp8_row_blocks": ([P, I64, INT, P, I64, P, I64, I64, I64, I64, I32_, P], INT),
+    # a cache goes as the address of a KVCache
+    "fg_add_rmsnorm": ([P, I64, INT, P, I64, P, I64, INT, P, INT, F32_, P, I64, INT, P, I64, I64, I32_, I64, I64, P],
+                       INT),
+    "fg_rope_append": ([P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, INT, P, I32_, P, I64, I64, I32_, I32_, P,
+                        I32_, P, I64, I32_, P], INT),
+    "fg_prefix_attention_workspace_bytes": ([I64, I64, I32_, I32_, I32_, I64, I64, I64, I32_], SZ),
+    "fg_prefix_attention": ([P, I64, I64, INT, P, P, I64, P, I64, P, P, I64, I64, I32_, I64, I64, F32_, P, I64, I64, P,
+                             P, SZ, P], INT),
     "fg_version": ([], ctypes.c_char_p),
     "fg_last_error": ([], ctypes.c_char_p),
     "fg_last_kernel": ([], ctypes.c_char_p),

@@ -1,0 +1,297 @@
+"""The operators of a serving decoder layer between its quantised linears, computed by libforge_mi355x.so only.
+
+* :func:`add_rmsnorm`: the residual's addition, the RMSNorm and, if asked for, the 8-bit codes and scales that
+  ``ops_gemm.int8_linear`` / ``fp8_linear`` take;
+* :func:`rope_append`: the rotation of a projection's queries and keys by their positions, and the keys' and values' way
+  into a :class:`PagedKVCache`;
+* :func:`prefix_attention`: the attention that reads this cache, for a batch whose sequences share a prefix.
+
+The reference runs these steps around its linears (``forge/models/attention.py:245-256``, ``forge/models/layers.py:167-173``).
+As in ``ops_gemm`` every op is one call into the C ABI (``include/forge_mi355x.h``) on the current stream, raises where it
+cannot run, neither synchronises nor reads lengths on the host, and takes outputs and workspaces from torch's caching
+allocator, so a layer can be captured in a HIP graph.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .errors import ConfigError
+from .ops_gemm import _as_rows, _check, _code_or_zero, _done, _ld, _on_gpu
+
+_16BIT = (torch.float16, torch.bfloat16)
+_QUANT = {None: None, "int8": torch.int8, "fp8": torch.float8_e4m3fn, "fp8_block": torch.float8_e4m3fn}
+
+
+def _same_device(op: str, x: torch.Tensor, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != x.device:
+            raise ConfigError(f"{op}: {name} is on {t.device}, the call is on {x.device}")
+
+
+# ================================================================================================ norm
+class NormOutput(NamedTuple):
+    y: torch.Tensor
+    scale: torch.Tensor | None
+    residual: torch.Tensor
+
+
+def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None = None, *,
+                eps: float = 1e-5, quant: str | None = None, block: int = 128,
+                residual_out: torch.Tensor | None = None) -> NormOutput:
+    """``h = x + residual`` and ``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, in one pass.
+
+    ``h`` is rounded to the residual's type (``x``'s or fp32), is the new residual stream and is what is normed; it goes to
+    ``residual_out`` (may be ``residual`` itself: in place) or a new tensor.  Without a residual ``h`` is ``x``.
+    ``quant``: ``None`` gives ``y`` in ``x``'s type and no scale, ``"int8"`` / ``"fp8"`` codes with one fp32 scale per row
+    (``[M]``), ``"fp8_block"`` e4m3 codes with one per 1 x ``block`` columns (``[M, ceil(K / block)]``, the scales of a
+    block of columns next to each other, as ``fp8_linear`` reads them fastest): what ``int8_linear`` does to its input,
+    and what ``fp8_linear`` takes as ``x`` and ``x_scale``.
+    """
+    _on_gpu(x, "add_rmsnorm")
+    if quant not in _QUANT:
+        raise ConfigError(f"add_rmsnorm: unknown quant {quant!r}: use None, int8, fp8 or fp8_block")
+    if not x.is_floating_point() or x.dtype not in (torch.float32, *_16BIT):
+        raise ConfigError("add_rmsnorm: x must be an fp32, fp16 or bf16 tensor")
+    if x.dim() == 0:
+        raise ConfigError("add_rmsnorm: x needs a last dimension to norm")
+    k = x.shape[-1]
+    _same_device("add_rmsnorm", x, weight=weight, residual=residual, residual_out=residual_out)
+    if weight is not None:
+        if weight.shape != (k,) or weight.dtype not in (torch.float32, *_16BIT):
+            raise ConfigError(f"add_rmsnorm: weight must be an fp32, fp16 or bf16 tensor of [{k}]")
+        weight = weight.contiguous()
+    x2 = _as_rows(x)
+    m = x2.shape[0]
+    r2 = ro2 = None
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype not in (x.dtype, torch.float32):
+            raise ConfigError("add_rmsnorm: residual must have x's shape and x's type or fp32")
+        r2 = _as_rows(residual)
+        if residual_out is None:
+            residual_out = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        elif residual_out.shape != x.shape or residual_out.dtype != residual.dtype:
+            raise ConfigError("add_rmsnorm: residual_out must be like residual")
+        ro2 = _as_rows(residual_out)
+        if m and ro2.data_ptr() != residual_out.data_ptr():
+            raise ConfigError("add_rmsnorm: residual_out must be rows of adjacent columns that do not overlap")
+    elif residual_out is not None:
+        raise ConfigError("add_rmsnorm: residual_out without a residual")
+    ydt = _QUANT[quant] or x.dtype
+    y = torch.empty((m, k), dtype=ydt, device=x.device)
+    scale, s_row, s_block = None, 0, 0
+    if quant == "fp8_block":
+        if block < 8 or block > 512 or block & (block - 1):
+            raise ConfigError("add_rmsnorm: block is a power of two from 8 to 512")
+        scale = torch.empty((-(-k // block), m), dtype=torch.float32, device=x.device).t()
+        s_row, s_block = 1, max(m, 1)
+    elif quant is not None:
+        scale, s_row = torch.empty(m, dtype=torch.float32, device=x.device), 1
+    if m and k:
+        _check(_lib.lib().fg_add_rmsnorm(
+            _lib.ptr(x2), _ld(x2), _lib.dtype_code(x2.dtype), _lib.ptr(r2), 0 if r2 is None else _ld(r2), _lib.ptr(ro2),
+            0 if ro2 is None else _ld(ro2), _code_or_zero(r2), _lib.ptr(weight), _code_or_zero(weight), eps, _lib.ptr(y),
+            k, _lib.dtype_code(ydt), _lib.ptr(scale), s_row, s_block, block if quant == "fp8_block" else 0, m, k,
+            _lib.stream_of(x2)), "fg_add_rmsnorm")
+    _done("add_rmsnorm")
+    return NormOutput(y if x.dim() == 2 else y.reshape(x.shape), scale, x if residual is None else residual_out)
+
+
+# ================================================================================================ paged cache
+@dataclass
+class PagedKVCache:
+    """Keys and values of many sequences in pages: ``k`` and ``v`` are ``[pages, kv_heads, page_size, head_dim]`` (any
+    strides of whole 16-byte units, the same for both, columns adjacent) in fp16, bf16 or float8_e4m3fn; an e4m3 value
+    stands for ``code * k_scale[head]`` (``v_scale``), fp32 ``[kv_heads]``.  A page holds each key head's tokens next to
+    each other (:meth:`allocate`), the order in which attention reads them."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor | None = None
+    v_scale: torch.Tensor | None = None
+
+    def __post_init__(self) -> None:
+        k, v = self.k, self.v
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ConfigError("PagedKVCache: k and v are [pages, kv_heads, page_size, head_dim] of one type on one device")
+        if k.dtype not in (*_16BIT, torch.float8_e4m3fn):
+            raise ConfigError("PagedKVCache: fp16, bf16 or float8_e4m3fn")
+        if k.stride() != v.stride() or k.stride(3) != 1:
+            raise ConfigError("PagedKVCache: k and v need the same strides and adjacent columns")
+        for name in ("k_scale", "v_scale"):
+            s = getattr(self, name)
+            if (s is not None) != (k.dtype == torch.float8_e4m3fn):
+                raise ConfigError("PagedKVCache: k_scale and v_scale belong to a float8_e4m3fn cache, and to no other")
+            if s is not None and (s.shape != (k.shape[1],) or s.dtype != torch.float32 or not s.is_contiguous()
+                                  or s.device != k.device):
+                raise ConfigError(f"PagedKVCache: {name} must be contiguous fp32 of [{k.shape[1]}] on the cache's device")
+
+    @classmethod
+    def allocate(cls, num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
+                 device: str | torch.device = "cuda", k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None) -> PagedKVCache:
+        """An empty cache; scales of an e4m3 cache default to 1."""
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        if dtype == torch.float8_e4m3fn:
+            k_scale, v_scale = (torch.ones(kv_heads, device=device) if s is None else s for s in (k_scale, v_scale))
+        return cls(torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) if dtype == torch.float8_e4m3fn
+                   else torch.zeros(shape, dtype=dtype, device=device),
+                   torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) if dtype == torch.float8_e4m3fn
+                   else torch.zeros(shape, dtype=dtype, device=device), k_scale, v_scale)
+
+    @property
+    def page_size(self) -> int:
+        return self.k.shape[2]
+
+    def _handle(self) -> _lib.KVCache:
+        pages, heads, page, dim = self.k.shape
+        sp, sh, st, _ = self.k.stride()
+        return _lib.KVCache(_lib.ptr(self.k), _lib.ptr(self.v), _lib.ptr(self.k_scale), _lib.ptr(self.v_scale), sp, sh, st,
+                            pages, _lib.dtype_code(self.k.dtype), heads, page, dim)
+
+
+def _heads(op: str, name: str, t: torch.Tensor, dim: int) -> None:
+    if t.dim() != 3 or t.shape[2] != dim:
+        raise ConfigError(f"{op}: {name} must be [tokens, heads, {dim}]")
+    if t.dtype not in _16BIT:
+        raise ConfigError(f"{op}: {name} must be fp16 or bf16")
+
+
+def _columns(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _fits_cache(op: str, q: torch.Tensor, cache: PagedKVCache) -> None:
+    _same_device(op, q, cache=cache.k)
+    if cache.k.dtype != q.dtype and cache.k.dtype != torch.float8_e4m3fn:
+        raise ConfigError(f"{op}: a {cache.k.dtype} cache does not take {q.dtype} queries")
+
+
+def _index(op: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
+    if t.dim() != 1 or t.shape[0] != n or t.dtype not in (torch.int32, torch.int64):
+        raise ConfigError(f"{op}: {name} must be an int32 or int64 tensor of [{n}]")
+    return t.contiguous()
+
+
+# ================================================================================================ rotation and append
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                cache: PagedKVCache, slots: torch.Tensor, *, interleaved: bool = False,
+                q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate ``q [T, heads, dim]`` and ``k [T, kv_heads, dim]`` by ``positions [T]``, write ``k`` and ``v`` to the cache's
+    ``slots [T]`` (``page * page_size + token``; one outside the cache, as -1, is padding) and return the rotated ``q``
+    (in ``q_out``, which may be ``q``, or a new tensor).
+
+    ``cos_sin``: fp32 ``[max_position, rot]``, the cosines of the ``rot / 2`` pairs, then their sines; the first ``rot``
+    columns of a head turn, in pairs ``(i, i + rot / 2)`` or, ``interleaved``, ``(2 i, 2 i + 1)``; the others pass through.
+    The rotation is fp32, rounded once to the result's type; an e4m3 cache takes ``value / scale`` of its key head, clamped
+    to +-448.  ``q``, ``k``, ``v`` may be views of one projection's output.  A position outside the table gives NaN.  Two
+    tokens of one slot: either may stay.
+    """
+    op = "rope_append"
+    _on_gpu(q, op)
+    _fits_cache(op, q, cache)
+    dim, hk = cache.k.shape[3], cache.k.shape[1]
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _heads(op, name, t, dim)
+    t = q.shape[0]
+    if k.shape[:2] != (t, hk) or v.shape[:2] != (t, hk) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ConfigError(f"{op}: k and v must be [{t}, {hk}, {dim}] of q's type")
+    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.shape[1] % 2 or not 2 <= cos_sin.shape[1] <= dim:
+        raise ConfigError(f"{op}: cos_sin must be fp32 [positions, rot] with an even rot up to {dim}")
+    _same_device(op, q, k=k, v=v, positions=positions, cos_sin=cos_sin, slots=slots, q_out=q_out)
+    positions, slots = _index(op, "positions", positions, t), _index(op, "slots", slots, t)
+    q, k, v, cos_sin = _columns(q), _columns(k), _columns(v), _columns(cos_sin)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif q_out.shape != q.shape or q_out.dtype != q.dtype or (q_out.stride(-1) != 1 and q_out.shape[-1] > 1):
+        raise ConfigError(f"{op}: q_out must be like q, with adjacent columns")
+    if t:
+        handle = cache._handle()
+        _check(_lib.lib().fg_rope_append(
+            _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0),
+            v.stride(1), _lib.ptr(q_out), q_out.stride(0), q_out.stride(1), _lib.dtype_code(q.dtype), _lib.ptr(positions),
+            positions.dtype == torch.int64, _lib.ptr(cos_sin), _ld(cos_sin), cos_sin.shape[0], cos_sin.shape[1],
+            interleaved, _lib.ptr(slots), slots.dtype == torch.int64, _lib.ctypes.addressof(handle), t, q.shape[1],
+            _lib.stream_of(q)), "fg_rope_append")
+    _done(op)
+    return q_out
+
+
+# ================================================================================================ attention
+def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                     prefix_pages: torch.Tensor | None = None, prefix_len: int = 0,
+                     query_start: torch.Tensor | None = None, max_query_len: int = 1, max_seq_len: int | None = None,
+                     scale: float | None = None, return_lse: bool = False,
+                     out: torch.Tensor | None = None) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Attention of ``q [T, heads, dim]`` over the cache, for B sequences that share a prefix (which is read once for all):
+    each query token sees the prefix and its own sequence's tokens up to itself.  Returns ``[T, heads, dim]`` in ``q``'s
+    type, with ``return_lse`` also the logarithm of each row's softmax sum, fp32 ``[T, heads]``.
+
+    * ``prefix_pages`` int32 ``[n]``, ``prefix_len``: the pages of the shared prefix, and its tokens (a host integer; 0: none);
+    * ``page_table`` int32 ``[B, pages]``, ``seq_lens`` int32 ``[B]``: each sequence's own pages after the prefix, and how many
+      tokens they hold, those of the queries included (appended before, with :func:`rope_append`).  Entries past the length,
+      and what stands in their slots, are not read;
+    * ``query_start`` int32 ``[B + 1]``: sequence b's queries are tokens ``query_start[b] .. query_start[b + 1]`` of ``q``, and the
+      last of its tokens; ``max_query_len`` bounds their number.  ``None``: one query token per sequence (decoding);
+    * ``max_seq_len``: a host bound of ``seq_lens`` (default: what the page table can hold), by which the work is split;
+    * ``heads`` is a multiple of the cache's ``kv_heads``; ``scale`` defaults to ``1 / sqrt(dim)``.
+
+    Lengths are read on the GPU only.  Scores, softmax and sums are fp32; the probabilities are rounded to ``q``'s type for
+    the product with the values.  A row that sees no token gives zeros (lse -inf), as do query tokens of no sequence.  A
+    query token past ``max_query_len`` gives NaN.  A NaN or infinity in a value that some query token of a sequence sees can
+    show in that sequence's earlier query tokens too.
+    """
+    op = "prefix_attention"
+    _on_gpu(q, op)
+    _fits_cache(op, q, cache)
+    _, hk, page, dim = cache.k.shape
+    _heads(op, "q", q, dim)
+    t, h, _ = q.shape
+    if h % hk or h == 0:
+        raise ConfigError(f"{op}: {h} query heads are no multiple of {hk} key heads")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32:
+        raise ConfigError(f"{op}: page_table must be int32 [sequences, pages]")
+    b, width = page_table.shape
+    if seq_lens.shape != (b,) or seq_lens.dtype != torch.int32:
+        raise ConfigError(f"{op}: seq_lens must be int32 [{b}]")
+    ragged = query_start is not None
+    if ragged and (query_start.shape != (b + 1,) or query_start.dtype != torch.int32):
+        raise ConfigError(f"{op}: query_start must be int32 [{b + 1}]")
+    if not ragged and (t != b or max_query_len != 1):
+        raise ConfigError(f"{op}: without query_start each of the {b} sequences has one query token, got {t}")
+    if max_query_len < 1 or prefix_len < 0:
+        raise ConfigError(f"{op}: max_query_len must be positive and prefix_len not negative")
+    if max_seq_len is None:
+        max_seq_len = width * page
+    elif not 0 <= max_seq_len <= width * page:
+        raise ConfigError(f"{op}: max_seq_len {max_seq_len} is past the page table's {width} pages of {page}")
+    if prefix_len and (prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.dtype != torch.int32
+                       or prefix_pages.shape[0] * page < prefix_len):
+        raise ConfigError(f"{op}: a prefix of {prefix_len} tokens needs int32 prefix_pages that hold them")
+    _same_device(op, q, page_table=page_table, seq_lens=seq_lens, prefix_pages=prefix_pages, query_start=query_start, out=out)
+    if out is None:
+        out = torch.empty((t, h, dim), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or (out.stride(-1) != 1 and dim > 1):
+        raise ConfigError(f"{op}: out must be like q, with adjacent columns")
+    lse = torch.empty((t, h), dtype=torch.float32, device=q.device) if return_lse else None
+    if t:
+        q = _columns(q)
+        page_table = page_table if page_table.stride(1) == 1 or width <= 1 else page_table.contiguous()
+        seq_lens = seq_lens.contiguous()
+        prefix_pages = prefix_pages.contiguous() if prefix_len else None
+        query_start = query_start.contiguous() if ragged else None
+        lib = _lib.lib()
+        need = lib.fg_prefix_attention_workspace_bytes(t, b, h, hk, dim, prefix_len, max_seq_len, max_query_len, ragged)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        handle = cache._handle()
+        _check(lib.fg_prefix_attention(
+            _lib.ptr(q), q.stride(0), q.stride(1), _lib.dtype_code(q.dtype), _lib.ctypes.addressof(handle),
+            _lib.ptr(prefix_pages), prefix_len, _lib.ptr(page_table), _ld(page_table), _lib.ptr(seq_lens),
+            _lib.ptr(query_start), t, b, h, max_seq_len, max_query_len, dim ** -0.5 if scale is None else scale,
+            _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(lse), _lib.ptr(ws), need, _lib.stream_of(q)),
+            "fg_prefix_attention")
+    _done(op)
+    return (out, lse) if return_lse else out

@@ -261,6 +261,68 @@ int fg_quant_fp8_row_blocks(const void* x, int64_t ldx, int x_dtype, uint8_t* q,
                             int64_t s_block, int64_t M, int64_t K, int32_t block, fg_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
+ * The operators of a decoder layer between its linears.  The reference keeps them beside this path
+ * (forge/models/attention.py:245-256, forge/models/layers.py:167-173, forge/serve/runner.py:586); these are this
+ * library's own forms of them.
+ *
+ * A paged cache: pages of page_size tokens for each key head, element (page, head, token, column) of k and of v at
+ * page * page_stride + head * head_stride + token * token_stride + column (elements).  dtype FG_F16 | FG_BF16 |
+ * FG_E4M3; e4m3 values stand for code * k_scale[head] (v_scale[head]), device float[kv_heads].  k, v and every stride
+ * are whole 16-byte units, head_dim is a multiple of 8 (of 16 for FG_E4M3) up to 256.
+ * ------------------------------------------------------------------------------------------------------------- */
+typedef struct fg_kv_cache {
+  void* k;
+  void* v;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t page_stride, head_stride, token_stride;
+  int64_t num_pages;
+  int32_t dtype, kv_heads, page_size, head_dim;
+} fg_kv_cache;
+
+/* h = x + residual, rounded to residual_dtype and written to residual_out (residual NULL: h = x, nothing written);
+ * y = h * weight / sqrt(mean(h^2) + eps) in fp32, stored as y_dtype: x_dtype, or FG_I8 / FG_E4M3 codes by the largest
+ * |y| of a row (block = 0) or of each 1 x block columns (a power of two, 8..512): s = amax / 127 or amax / 448 (1 if
+ * amax is not > 0), code = y /_IEEE s rounded half to even; the scale of (row, block) at s[row * s_row + b * s_block].
+ * residual_dtype: x_dtype or FG_F32.  weight may be NULL.  residual_out may be residual itself, and y x.  K <= 32768. */
+int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual, int64_t ldr, void* residual_out,
+                   int64_t ldro, int residual_dtype, const void* weight, int weight_dtype, float eps, void* y,
+                   int64_t ldy, int y_dtype, float* s, int64_t s_row, int64_t s_block, int32_t block, int64_t M,
+                   int64_t K, fg_stream_t stream);
+
+/* Rotary embedding and cache append of T tokens: q [T][q_heads][head_dim], k and v [T][kv_heads][head_dim] (dtype
+ * FG_F16 | FG_BF16, element strides of tokens and heads, columns adjacent).  Columns (i, i + rot / 2), or (2 i, 2 i + 1)
+ * with interleaved, i < rot / 2, turn by the angle whose cosine is table[pos * ld_table + i] and sine
+ * table[pos * ld_table + rot / 2 + i] (fp32); the other columns pass through.  Rotated q goes to q_out (may be q),
+ * rotated k and v to the cache's slot page * page_size + token; a slot outside the cache (negative: padding) is not
+ * written.  A position outside [0, max_pos) gives NaN in the rotated columns.  positions and slots are int32 or, with
+ * the flag, int64. */
+int fg_rope_append(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                   const void* v, int64_t v_token, int64_t v_head, void* q_out, int64_t qo_token, int64_t qo_head,
+                   int dtype, const void* positions, int32_t positions_int64, const float* table, int64_t ld_table,
+                   int64_t max_pos, int32_t rot, int32_t interleaved, const void* slots, int32_t slots_int64,
+                   const fg_kv_cache* cache, int64_t T, int32_t q_heads, fg_stream_t stream);
+
+/* Attention of T query tokens over the cache, for B sequences that share a prefix: o = softmax(scale q K^T) V over the
+ * first prefix_len tokens of prefix_pages (which every sequence sees) and the sequence's own seq_lens[b] tokens in
+ * page_table[b].  Query tokens query_start[b] .. query_start[b + 1] are the last tokens of sequence b, each of which
+ * sees the own tokens up to itself; query_start NULL: one query token per sequence (T = B).  Query heads h of key head
+ * h / (q_heads / kv_heads).
+ *   seq_lens int32 [B] and query_start int32 [B + 1] are device memory; max_seq_len and max_query_len bound them
+ *   (longer sequences are cut, later query tokens give NaN); page ids outside the cache stand for no tokens.
+ *   A row that sees no token gives zeros and -inf; so do query tokens of no sequence.
+ *   lse (may be NULL): float [T][q_heads], the natural logarithm of the softmax's sum.
+ *   workspace: fg_prefix_attention_workspace_bytes bytes, 16-byte aligned. */
+size_t fg_prefix_attention_workspace_bytes(int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                           int64_t prefix_len, int64_t max_seq_len, int64_t max_query_len,
+                                           int32_t ragged);
+int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const fg_kv_cache* cache,
+                        const int32_t* prefix_pages, int64_t prefix_len, const int32_t* page_table, int64_t ld_pages,
+                        const int32_t* seq_lens, const int32_t* query_start, int64_t T, int64_t B, int32_t q_heads,
+                        int64_t max_seq_len, int64_t max_query_len, float scale, void* out, int64_t o_token,
+                        int64_t o_head, float* lse, void* workspace, size_t workspace_bytes, fg_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
  * Library information.  fg_device_ok replaces the capability gate triton_usable (forge/kernels/ops_gemm.py:159-175):
  * returns 1 when `device` is a gfx950 GPU this build can run on, else 0 (message in fg_last_error).
  * ------------------------------------------------------------------------------------------------------------- */

@@ -1,0 +1,128 @@
+"""Host side of the operators between a decoder layer's linears, on the CPU: the C entry points refuse bad calls before any
+launch (the pointers are placeholders that no kernel sees), and the workspace query follows the plan."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from forge_amd import _lib
+from forge_amd import ops_decoder as ops
+from forge_amd.errors import ConfigError, HardwareUnsupported
+
+P = ctypes.c_void_p(256)
+ODD = ctypes.c_void_p(264)
+
+
+def _cache(**kw):
+    c = dict(k=256, v=256, k_scale=None, v_scale=None, page_stride=8192, head_stride=1024, token_stride=64, num_pages=4,
+             dtype=_lib.BF16, kv_heads=2, page_size=16, head_dim=64)
+    c.update(kw)
+    return _lib.KVCache(**c)
+
+
+def _norm(**kw):
+    a = dict(x=P, ldx=64, xdt=_lib.BF16, r=P, ldr=64, ro=P, ldro=64, rdt=_lib.BF16, w=P, wdt=_lib.BF16, eps=1e-5, y=P, ldy=64,
+             ydt=_lib.I8, s=P, s_row=1, s_block=0, block=0, m=2, k=64, stream=None)
+    a.update(kw)
+    return _lib.lib().fg_add_rmsnorm(*a.values())
+
+
+@pytest.mark.parametrize("bad,status", [(dict(m=-1), 1), (dict(k=0), 1), (dict(k=32769), 2), (dict(x=None), 1), (dict(ro=None), 1),
+                                        (dict(s=None), 1), (dict(xdt=_lib.I8), 1), (dict(rdt=_lib.F16), 1), (dict(ydt=_lib.F16), 1),
+                                        (dict(block=24), 1), (dict(block=1024), 1), (dict(ydt=_lib.BF16, block=64), 1),
+                                        (dict(ldx=63), 1), (dict(ldro=5), 1), (dict(wdt=_lib.E4M3), 1), (dict(s_row=-1), 1)])
+def test_norm_refusals(bad, status):
+    assert _norm(**bad) == status and "fg_add_rmsnorm" in _lib.last_error()
+
+
+def test_no_work_is_no_error():
+    assert _norm(m=0, x=None, y=None) == _lib.OK
+
+
+CACHES = [(dict(k=None), 1), (dict(k=264), 1), (dict(page_stride=8190), 1), (dict(token_stride=56), 1), (dict(head_stride=-64), 1),
+          (dict(num_pages=0), 1), (dict(page_size=0), 1), (dict(dtype=_lib.F16), 1), (dict(dtype=_lib.E4M3), 1),
+          (dict(dtype=_lib.F32), 1), (dict(head_dim=264, token_stride=264), 2), (dict(head_dim=60), 2),
+          (dict(num_pages=2 ** 23, page_stride=2 ** 13), 2), (dict(num_pages=2 ** 31, page_stride=8), 1)]
+
+
+def _append(cache=None, **kw):
+    a = dict(q=P, qt=256, qh=64, k=P, kt=128, kh=64, v=P, vt=128, vh=64, qo=P, qot=256, qoh=64, dt=_lib.BF16, pos=P, p64=1,
+             table=P, ld=64, max_pos=100, rot=64, inter=0, slots=P, s64=1,
+             cache=ctypes.byref(_cache() if cache is None else cache), t=3, heads=4, stream=None)
+    a.update(kw)
+    return _lib.lib().fg_rope_append(*a.values())
+
+
+@pytest.mark.parametrize("bad", [dict(t=-1), dict(heads=0), dict(dt=_lib.F32), dict(q=None), dict(table=None), dict(rot=0),
+                                 dict(rot=63), dict(rot=66), dict(ld=62), dict(max_pos=-1), dict(cache=None), dict(k=None)])
+def test_append_refusals(bad):
+    assert _append(**bad) == _lib.EINVAL and "fg_rope_append" in _lib.last_error()
+
+
+@pytest.mark.parametrize("bad,status", CACHES)
+def test_cache_refusals(bad, status):
+    c = _cache(**bad)
+    assert _append(c) == status and _attention(c) == status
+
+
+def _attention(cache=None, **kw):
+    a = dict(q=P, qt=256, qh=64, dt=_lib.BF16, cache=ctypes.byref(_cache() if cache is None else cache), pp=P, prefix=40,
+             table=P, ld=2, lens=P, starts=None, t=3, b=3, heads=4, seq=32, maxq=1, scale=0.1, out=P, ot=256, oh=64, lse=None,
+             ws=None, bytes=0, stream=None)
+    a.update(kw)
+    return _lib.lib().fg_prefix_attention(*a.values())
+
+
+@pytest.mark.parametrize("bad,why", [(dict(t=2), "query token"), (dict(maxq=2), "query token"), (dict(heads=3), "kv_heads"),
+                                     (dict(heads=0), "sizes"), (dict(maxq=0), "sizes"), (dict(prefix=-1), "sizes"),
+                                     (dict(seq=33), "page table"), (dict(pp=None), "null"), (dict(lens=None), "null"),
+                                     (dict(out=None), "null"), (dict(), "workspace"), (dict(ws=ODD, bytes=1 << 30), "workspace"),
+                                     (dict(ws=P, bytes=64), "workspace"), (dict(t=2 ** 30, b=2 ** 30), "32 bits")])
+def test_attention_refusals(bad, why):
+    assert _attention(**bad) == _lib.EINVAL and why in _lib.last_error()
+
+
+def test_attention_without_queries_is_no_error():
+    assert _attention(t=0, b=0, q=None, out=None) == _lib.OK
+
+
+def test_workspace_follows_the_plan():
+    ws = _lib.lib().fg_prefix_attention_workspace_bytes
+    assert ws(0, 4, 8, 2, 64, 100, 100, 1, 1) == 0 and ws(4, 4, 7, 2, 64, 0, 100, 1, 0) == 0
+    assert ws(64, 64, 32, 8, 128, 0, 100, 1, 0) == 0  # one part for each sequence: nothing to join
+    row = 32 * (128 * 4 + 8)
+    short = ws(1, 1, 32, 8, 128, 100, 100, 1, 0)
+    assert short % row == 0 and short // row >= 2  # a prefix makes two parts at least
+    assert ws(1, 1, 32, 8, 128, 0, 8192, 1, 0) > short
+    assert ws(3, 0, 8, 2, 64, 0, 0, 1, 1) > 0  # tokens of no sequence
+
+
+def test_cache_descriptions():
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    ops.PagedKVCache(k, k.clone())
+    one = torch.ones(2)
+    e4 = torch.zeros(4, 2, 16, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    cache = ops.PagedKVCache(e4, e4, one, one)
+    assert cache.page_size == 16 and cache._handle().k == e4.data_ptr() and cache._handle().page_stride == 2048
+    for args in ((k, k[:3]), (k, k.half()), (k.float(), k.float()), (k[0], k[0]), (k, k.transpose(1, 2).contiguous().transpose(1, 2)),
+                 (k.transpose(2, 3), k.transpose(2, 3)), (k, k, one, one), (e4, e4), (e4, e4, one), (e4, e4, one, torch.ones(3)),
+                 (e4, e4, one, one.double())):
+        with pytest.raises(ConfigError):
+            ops.PagedKVCache(*args)
+
+
+def test_allocate():
+    c = ops.PagedKVCache.allocate(3, 2, 16, 64, torch.float8_e4m3fn, "cpu")
+    assert c.k.shape == (3, 2, 16, 64) and c.k_scale.tolist() == [1, 1] and c.k.float().abs().max() == 0
+    assert ops.PagedKVCache.allocate(3, 2, 16, 64, device="cpu").k.dtype == torch.bfloat16
+
+
+def test_no_cpu_path(monkeypatch):
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    with pytest.raises(HardwareUnsupported):
+        ops.add_rmsnorm(x, None)
+    monkeypatch.setenv("FORGE_FORCE_REF", "1")
+    with pytest.raises(HardwareUnsupported, match="FORGE_FORCE_REF"):
+        ops.add_rmsnorm(x, None)
