@@ -26,7 +26,7 @@ struct AttnArgs {
   float scale_log2;  // softmax scale * log2(e)
   // keys are split into parts of whole tiles, one workgroup each; parts_p of the prefix, parts_s of each sequence's own tokens
   int parts_p, parts_s, part_p, part_s;  // counts and tokens per part
-  int tiles_p, tiles_s;                  // row tiles
+  int tile_p, tile_s, tiles_p, tiles_s;  // rows per tile, row tiles
   int items_p, items;                    // work items of the prefix, and in all
   float* acc;  // partial sums [parts_p + parts_s][T * Hq][D], null: one part, written to out
   float2* ml;  // their maxima (in log2) and sums [parts_p + parts_s][T * Hq]
@@ -34,6 +34,7 @@ struct AttnArgs {
 
 size_t attn_plan(AttnArgs& a);
 hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, hipStream_t st);
+hipError_t launch_attn_tile(const AttnArgs& a, bool bf16, bool fp8, int first, int count, hipStream_t st);
 
 constexpr uint32_t kNoRow = 0xffffffffu;  // an entry of the row table that stands for no key
 constexpr int kMaxPart = 2048;            // tokens per part: entries of the row table
@@ -100,23 +101,33 @@ __device__ __forceinline__ bool attn_item(const AttnArgs& a, int id, AttnItem& i
   return it.row0 < it.rows && (part == 0 || it.begin < len);
 }
 
+// Key t's row in 16-byte units from the first page; kNoRow for a page outside the cache.
+__device__ __forceinline__ uint32_t attn_row(const AttnArgs& a, const AttnItem& it, int t) {
+  const int page = t / a.page, off = t - page * a.page, id = it.table[page];
+  return id >= 0 && id < a.n_pages ? (uint32_t)id * a.c_page + (uint32_t)off * a.c_token : kNoRow;
+}
+
 // Table of the item's keys in LDS: each key's row in 16-byte units from the first page, up to a whole number of tiles of
 // `tile` keys; kNoRow past the end and for pages outside the cache.
 __device__ __forceinline__ void attn_row_table(const AttnArgs& a, const AttnItem& it, uint32_t* tab, int tile) {
   const int n = max(it.end - it.begin, 0), padded = (n + tile - 1) / tile * tile;
-  for (int i = threadIdx.x; i < padded; i += blockDim.x) {
-    uint32_t row = kNoRow;
-    if (i < n) {
-      const int t = it.begin + i, page = t / a.page, off = t - page * a.page;
-      const int id = it.table[page];
-      if (id >= 0 && id < a.n_pages) row = (uint32_t)id * a.c_page + (uint32_t)off * a.c_token;
-    }
-    tab[i] = row;
-  }
+  for (int i = threadIdx.x; i < padded; i += blockDim.x) tab[i] = i < n ? attn_row(a, it, it.begin + i) : kNoRow;
 }
 
 __device__ __forceinline__ uint4 attn_ld16(const uint8_t* base, uint32_t row, int unit) {
   return *reinterpret_cast<const uint4*>(base + ((uint64_t)row + (uint32_t)unit) * 16);
+}
+
+// The transposing LDS reads: 16 lanes read 4 keys x 16 columns of 16 bits (8 keys of 8 bits), lanes 4 j .. 4 j + 3 (2 j, 2 j + 1)
+// 8 bytes each of key j, and get one column each.
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ s16x4 lds_tr16(const uint8_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      reinterpret_cast<__attribute__((address_space(3))) s16x4*>((__attribute__((address_space(3))) uint8_t*)(p)));
+}
+__device__ __forceinline__ i32x2 lds_tr8(const uint8_t* p) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+      reinterpret_cast<__attribute__((address_space(3))) i32x2*>((__attribute__((address_space(3))) uint8_t*)(p)));
 }
 
 template <bool BF16>

@@ -20,17 +20,6 @@ namespace fg {
 
 namespace {
 
-typedef int i32x2 __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ s16x4 lds_tr16(const uint8_t* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      reinterpret_cast<__attribute__((address_space(3))) s16x4*>((__attribute__((address_space(3))) uint8_t*)(p)));
-}
-__device__ __forceinline__ i32x2 lds_tr8(const uint8_t* p) {
-  return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-      reinterpret_cast<__attribute__((address_space(3))) i32x2*>((__attribute__((address_space(3))) uint8_t*)(p)));
-}
-
 // 16-byte unit u of key t in a V tile whose rows hold U units: an exchange of units that depends on the key, so that both
 // the writes (16 keys, one unit) and the transposing reads (8 keys, 32 bytes) spread over all banks.
 template <int U>
@@ -47,7 +36,7 @@ constexpr int kRowsTile = 32;  // keys per wavefront and step
 
 // DP: head columns in registers (D of them are there), R: row blocks of 16.
 template <bool BF16, bool FP8, int DP, int R>
-__global__ void __launch_bounds__(64 * kRowsWaves) attn_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(64 * kRowsWaves) attn_rows_kernel(const AttnArgs a, int first) {
   constexpr int IT = FP8 ? 1 : 2, U = DP * IT / 16, C = DP / 32, DB = DP / 16;
   constexpr int KU = U / 4;  // 16-byte loads of a lane per key
   constexpr int kVBytes = kRowsTile * DP * IT, kOBytes = 2 * 16 * R * DP * 4;
@@ -57,12 +46,13 @@ __global__ void __launch_bounds__(64 * kRowsWaves) attn_rows_kernel(const AttnAr
   __shared__ float red[2][kRowsWaves][16 * R];
 
   AttnItem it;
-  if (!attn_item<16 * R>(a, blockIdx.x, it)) return;
+  if (!attn_item<16 * R>(a, first + blockIdx.x, it)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, grp = lane >> 4;
   const int units = a.D * IT / 16;
   attn_row_table(a, it, tab, kRowsTile);
 
   // this lane's row of each row block: the fragment of Q, and the keys it sees
+  const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale turns the rows instead
   s16x8 qf[R][C];
   int seen[R];
 #pragma unroll
@@ -77,11 +67,12 @@ __global__ void __launch_bounds__(64 * kRowsWaves) attn_rows_kernel(const AttnAr
       const int d = FP8 ? 64 * (c / 2) + 16 * grp + 8 * (c % 2) : 32 * c + 8 * grp;
       uint4 u = make_uint4(0, 0, 0, 0);
       if (in && d < a.D) __builtin_memcpy(&u, __builtin_assume_aligned(qp + d, 2), 16);
+      u.x ^= sign; u.y ^= sign; u.z ^= sign; u.w ^= sign;
       qf[r][c] = __builtin_bit_cast(s16x8, u);
     }
   }
   const int min_seen = it.causal ? it.seen0 + it.row0 / a.G : it.end;  // what the tile's first row sees
-  const float sc = a.scale_log2 * (FP8 ? a.ks[it.head] : 1.f);
+  const float sc = fabsf(a.scale_log2) * (FP8 ? a.ks[it.head] : 1.f);
   const uint8_t *kb = a.k + it.head * a.c_head, *vb = a.v + it.head * a.c_head;
 
   f32x4 o[R][DB];
@@ -152,7 +143,7 @@ __global__ void __launch_bounds__(64 * kRowsWaves) attn_rows_kernel(const AttnAr
     for (int r = 0; r < R; ++r) {
       float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = s[r][j / 4][j % 4] * sc;
+      for (int j = 0; j < 8; ++j) x[j] = s[r][j / 4][j % 4];
       if (ok != 0xffffffffu || it.begin + t0 + kRowsTile > min_seen) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -163,6 +154,7 @@ __global__ void __launch_bounds__(64 * kRowsWaves) attn_rows_kernel(const AttnAr
       float top = x[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+      top *= sc;
       if (__any(top > m[r] + kSlack)) {
         top = fmaxf(top, __shfl_xor(top, 16, kWave));
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
@@ -175,7 +167,7 @@ __global__ void __launch_bounds__(64 * kRowsWaves) attn_rows_kernel(const AttnAr
       const float base = attn_base(m[r]);
       uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - base);
+      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], sc, -base));
       l[r] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = pack2<BF16>(x[2 * j], x[2 * j + 1]);
@@ -324,33 +316,58 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
 }
 
 
-// Cuts the keys into parts, the rows into tiles.  Host lengths only: a sequence shorter than max_len leaves parts that end
-// at once.
-static int split_keys(int64_t len, int64_t items, int* part) {
-  items = std::max<int64_t>(items, 1);  // no sequences
-  // parts of at least one tile per wavefront, at most the row table, and about four workgroups per CU in all
-  const int64_t unit = kRowsTile * kRowsWaves, want = std::max<int64_t>(1, (4 * device_cus() + items - 1) / items);
-  int64_t p = (len + want - 1) / want;
-  p = std::min<int64_t>(kMaxPart, std::max<int64_t>(unit, (p + unit - 1) / unit * unit));
+// Cuts the keys of `items` row tiles into parts, a workgroup each: about `want` of them in all, whole multiples of `unit` keys
+// and at most `most`.  Host lengths only: a sequence shorter than max_len leaves parts that end at once.
+static int split_keys(int64_t len, int64_t items, int64_t want, int64_t unit, int64_t most, int* part) {
+  const int64_t parts = std::max<int64_t>(1, want / std::max<int64_t>(items, 1));
+  const int64_t p = std::min(most, std::max<int64_t>(unit, ((len + parts - 1) / parts + unit - 1) / unit * unit));
   *part = (int)p;
   return (int)std::max<int64_t>(1, (len + p - 1) / p);
 }
 
-// Row blocks of 16 per item; two of them with 256 columns would not fit the registers.
-static int rows_r(int64_t rows, int D) { return rows <= 16 || D > 128 ? 1 : 2; }
+// Rows per work item: 16 or 32 for attn_rows_kernel (32 with 256 columns would not fit its registers), 128 for attn_tile_kernel.
+static int rows_tile(int64_t rows, int D) {
+  if (rows <= 16) return 16;
+  return rows <= 32 && D <= 128 ? 32 : 128;
+}
+
+static void plan_segment(int64_t len, int64_t rows, int64_t heads, int D, int* tile, int* tiles, int* parts, int* part) {
+  *tile = rows_tile(rows, D);
+  *tiles = (int)((rows + *tile - 1) / *tile);
+  const int64_t items = *tiles * heads, cus = device_cus();
+  *parts = *tile == 128 ? split_keys(len, items, 2 * cus, 64, 1 << 30, part)
+                        : split_keys(len, items, 4 * cus, kRowsTile * kRowsWaves, kMaxPart, part);
+}
 
 // Fills in the plan; returns the partial sums' bytes.  items is -1 where the work items would pass 32 bits.
 size_t attn_plan(AttnArgs& a) {
-  const int64_t rows_p = (int64_t)a.T * a.G, rows_s = (int64_t)a.max_q * a.G, tile = 16 * rows_r(std::max(rows_p, rows_s), a.D);
-  a.tiles_p = (int)((rows_p + tile - 1) / tile);
-  a.tiles_s = (int)((rows_s + tile - 1) / tile);
-  a.parts_p = a.prefix_len ? split_keys(a.prefix_len, (int64_t)a.tiles_p * a.Hk, &a.part_p) : 0;
-  a.parts_s = split_keys(a.max_len, (int64_t)a.tiles_s * a.Hk * a.B, &a.part_s);
+  a.parts_p = a.tiles_p = a.part_p = 0;
+  a.tile_p = 16;
+  if (a.prefix_len) plan_segment(a.prefix_len, (int64_t)a.T * a.G, a.Hk, a.D, &a.tile_p, &a.tiles_p, &a.parts_p, &a.part_p);
+  plan_segment(a.max_len, (int64_t)a.max_q * a.G, (int64_t)a.Hk * a.B, a.D, &a.tile_s, &a.tiles_s, &a.parts_s, &a.part_s);
   const int64_t items_p = (int64_t)a.parts_p * a.tiles_p * a.Hk, items = items_p + (int64_t)a.parts_s * a.tiles_s * a.Hk * a.B;
   a.items_p = (int)items_p;
   a.items = items < (1LL << 31) ? (int)items : -1;
   if (a.parts_p + a.parts_s == 1 && !a.starts) return 0;
   return (size_t)(a.parts_p + a.parts_s) * a.T * a.Hq * ((size_t)a.D * 4 + sizeof(float2));
+}
+
+template <int R>
+static hipError_t launch_attn_rows(const AttnArgs& a, bool bf16, bool fp8, int first, int count, hipStream_t st) {
+  auto go = [&](auto b_tag, auto f_tag, auto d_tag) {
+    hipLaunchKernelGGL((attn_rows_kernel<decltype(b_tag)::value, decltype(f_tag)::value, decltype(d_tag)::value, R>),
+                       dim3((unsigned)count), dim3(64 * kRowsWaves), 0, st, a, first);
+    return hipGetLastError();
+  };
+  auto by_d = [&](auto b_tag, auto f_tag) {
+    if (a.D <= 64) return go(b_tag, f_tag, std::integral_constant<int, 64>{});
+    if constexpr (R == 1) {
+      if (a.D > 128) return go(b_tag, f_tag, std::integral_constant<int, 256>{});
+    }
+    return go(b_tag, f_tag, std::integral_constant<int, 128>{});
+  };
+  auto by_f = [&](auto b_tag) { return fp8 ? by_d(b_tag, std::true_type{}) : by_d(b_tag, std::false_type{}); };
+  return bf16 ? by_f(std::true_type{}) : by_f(std::false_type{});
 }
 
 hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, hipStream_t st) {
@@ -362,27 +379,17 @@ hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, hipStream_t s
     a.acc = static_cast<float*>(ws);
     a.ml = reinterpret_cast<float2*>(a.acc + (size_t)(a.parts_p + a.parts_s) * a.T * a.Hq * a.D);
   }
-  const int R = rows_r(std::max((int64_t)a.T * a.G, (int64_t)a.max_q * a.G), a.D);
-  auto go = [&](auto b_tag, auto f_tag, auto d_tag, auto r_tag) {
-    hipLaunchKernelGGL((attn_rows_kernel<decltype(b_tag)::value, decltype(f_tag)::value, decltype(d_tag)::value,
-                                         decltype(r_tag)::value>),
-                       dim3((unsigned)a.items), dim3(64 * kRowsWaves), 0, st, a);
-    return hipGetLastError();
+  auto items = [&](int tile, int first, int count) {
+    if (count == 0) return hipSuccess;
+    if (tile == 128) return launch_attn_tile(a, bf16, fp8, first, count, st);
+    return tile == 16 ? launch_attn_rows<1>(a, bf16, fp8, first, count, st) : launch_attn_rows<2>(a, bf16, fp8, first, count, st);
   };
-  auto by_r = [&](auto b_tag, auto f_tag, auto d_tag) {
-    if constexpr (decltype(d_tag)::value <= 128) {
-      if (R == 2) return go(b_tag, f_tag, d_tag, std::integral_constant<int, 2>{});
-    }
-    return go(b_tag, f_tag, d_tag, std::integral_constant<int, 1>{});
-  };
-  auto by_d = [&](auto b_tag, auto f_tag) {
-    if (a.D <= 64) return by_r(b_tag, f_tag, std::integral_constant<int, 64>{});
-    if (a.D <= 128) return by_r(b_tag, f_tag, std::integral_constant<int, 128>{});
-    return by_r(b_tag, f_tag, std::integral_constant<int, 256>{});
-  };
-  auto by_f = [&](auto b_tag) { return fp8 ? by_d(b_tag, std::true_type{}) : by_d(b_tag, std::false_type{}); };
-  hipError_t e = a.items == 0 ? hipSuccess : (bf16 ? by_f(std::true_type{}) : by_f(std::false_type{}));
-  note_kernel("attn_rows_kernel R=%d parts=%d+%d%s", R, a.parts_p, a.parts_s, bytes ? " + attn_join_kernel" : "");
+  // one launch for the prefix and the sequences where one kernel takes both
+  const bool one = a.tile_p == a.tile_s || a.items_p == 0;
+  hipError_t e = one ? hipSuccess : items(a.tile_p, 0, a.items_p);
+  if (e == hipSuccess) e = one ? items(a.tile_s, 0, a.items) : items(a.tile_s, a.items_p, a.items - a.items_p);
+  note_kernel("attn rows %d x %d parts + rows %d x %d parts%s", a.items_p ? a.tile_p : 0, a.parts_p, a.tile_s, a.parts_s,
+              bytes ? " + attn_join_kernel" : "");
   if (e != hipSuccess || !bytes) return e;
   const unsigned grid = (unsigned)(((int64_t)a.T * a.Hq + 3) / 4);
   if (bf16) hipLaunchKernelGGL(attn_join_kernel<true>, dim3(grid), dim3(256), 0, st, a);

@@ -56,7 +56,7 @@ def _append(cache=None, **kw):
 
 
 @pytest.mark.parametrize("bad", [dict(t=-1), dict(heads=0), dict(dt=_lib.F32), dict(q=None), dict(table=None), dict(rot=0),
-                                 dict(rot=63), dict(rot=66), dict(ld=62), dict(max_pos=-1), dict(cache=None), dict(k=None)])
+                                 dict(rot=63), dict(rot=66), dict(ld=62), dict(max_pos=-1), dict(k=None)])
 def test_append_refusals(bad):
     assert _append(**bad) == _lib.EINVAL and "fg_rope_append" in _lib.last_error()
 
