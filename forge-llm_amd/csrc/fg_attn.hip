@@ -145,11 +145,12 @@ __global__ void __launch_bounds__(64 * kRowsWaves) attn_rows_kernel(const AttnAr
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = s[r][j / 4][j % 4];
       if (ok != 0xffffffffu || it.begin + t0 + kRowsTile > min_seen) {
+        asm volatile("");  // a branch, so that whole tiles skip it
+        const int left = seen[r] - (it.begin + t0);  // keys of the tile that this lane's row sees
+        const uint32_t mask = (left >= 32 ? ok : (left > 0 ? ok & ((1u << left) - 1) : 0u)) >> (4 * grp);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int t = 16 * (j / 4) + 4 * grp + j % 4;
-          if (!(ok >> t & 1) || it.begin + t0 + t >= seen[r]) x[j] = -__builtin_inff();
-        }
+        for (int j = 0; j < 8; ++j)
+          if (!(mask >> (16 * (j / 4) + j % 4) & 1)) x[j] = -__builtin_inff();
       }
       float top = x[0];
 #pragma unroll
