@@ -22,22 +22,28 @@ struct AttnArgs {
   int64_t ld_pages;
   const int32_t *lens, *starts;  // starts: [B + 1] or null (one query token per sequence)
   int T, B, Hq, Hk, G, D, page, n_pages;
+  int item;  // bytes of a cached value
   int prefix_len, max_len, max_q;
   float scale_log2;  // softmax scale * log2(e)
   // keys are split into parts of whole tiles, one workgroup each; parts_p of the prefix, parts_s of each sequence's own tokens
   int parts_p, parts_s, part_p, part_s;  // counts and tokens per part
-  int tile_p, tile_s, tiles_p, tiles_s;  // rows per tile, row tiles
-  int items_p, items;                    // work items of the prefix, and in all
+  bool tile_p, tile_s;                   // whether attn_tile takes the segment, or attn_rows
+  bool joined;                           // a sequence's items take the prefix's keys too
+  bool lead;                             // the prefix's items go first, not spread among the sequences'
+  int tiles_p, tiles_s;                  // row tiles
+  int items_p, items;                    // workgroups for the prefix, and in all
   float* acc;  // partial sums [parts_p + parts_s][T * Hq][D], null: one part, written to out
   float2* ml;  // their maxima (in log2) and sums [parts_p + parts_s][T * Hq]
 };
 
 size_t attn_plan(AttnArgs& a);
 hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, hipStream_t st);
-hipError_t launch_attn_tile(const AttnArgs& a, bool bf16, bool fp8, int first, int count, hipStream_t st);
 
 constexpr uint32_t kNoRow = 0xffffffffu;  // an entry of the row table that stands for no key
-constexpr int kMaxPart = 2048;            // tokens per part: entries of the row table
+constexpr int kMaxPart = 2048;            // attn_rows: tokens per part, entries of its row table
+constexpr int kRowsWaves = 4, kRowsTile = 32;  // wavefronts, keys per wavefront and step
+constexpr int kTileRows = 128;            // attn_tile: rows per item
+enum { kAttnRows = 0, kAttnTile = 1, kAttnMixed = 2 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -50,51 +56,70 @@ struct AttnItem {
   int row0, rows;   // first row of the tile among the segment's rows, and the segment's rows
   int token0;       // first query token of the segment
   int begin, end;   // its keys
-  int len;          // keys of the segment
+  int front;        // keys in front that are the prefix's (an item of a sequence that takes both)
   int seen0;        // keys that the segment's first query token sees; each further one sees one more (prefix: all see all)
   bool causal;
   const int32_t* table;
   int slot;  // part index
 };
 
+// Work item `id` of `pairs` sets of keys (key head, part, sequence) times `tiles` row tiles: consecutive workgroups go to the
+// eight XCDs in turn, so every eighth one takes the next row tile of the same keys and finds them in its L2.  Needs sets
+// enough for all XCDs: else row tiles go round in turn.
+__host__ __device__ __forceinline__ bool attn_by_xcd(int pairs) { return pairs % 8 == 0 || pairs >= 64; }
+__host__ __device__ __forceinline__ int64_t attn_count(int64_t pairs, int64_t tiles) {
+  return (pairs < (1 << 30) && attn_by_xcd((int)pairs) ? (pairs + 7) / 8 * 8 : pairs) * tiles;
+}
+
 // Item `id` of the grid; false: nothing to do.  TILE rows per item.
 template <int TILE>
 __device__ __forceinline__ bool attn_item(const AttnArgs& a, int id, AttnItem& it) {
-  if (id < a.items_p) {
-    // neighbours share keys: row tiles innermost
-    const int tile = id % a.tiles_p, rest = id / a.tiles_p, part = rest % a.parts_p;
-    it.head = rest / a.parts_p;
+  const bool prefix = id < a.items_p;
+  if (!prefix) id -= a.items_p;
+  const int tiles = prefix ? a.tiles_p : a.tiles_s, pairs = prefix ? a.parts_p * a.Hk : a.parts_s * a.Hk * a.B;
+  int pair, tile;
+  if (attn_by_xcd(pairs)) {
+    pair = (id / 8) / tiles * 8 + id % 8;
+    tile = (id / 8) % tiles;
+    if (pair >= pairs) return false;
+  } else {
+    pair = id / tiles;
+    tile = id % tiles;
+  }
+  it.front = 0;
+  if (prefix) {
+    const int part = pair / a.Hk;  // neighbours read the heads of one page, which lie next to each other
+    it.head = pair - part * a.Hk;
     it.row0 = tile * TILE;
     it.rows = a.T * a.G;
     it.token0 = 0;
     it.begin = part * a.part_p;
     it.end = min(it.begin + a.part_p, a.prefix_len);
-    it.len = it.seen0 = a.prefix_len;
+    it.seen0 = a.prefix_len;
     it.causal = false;
     it.table = a.prefix_pages;
     it.slot = part;
     return it.row0 < it.rows;
   }
-  id -= a.items_p;
-  const int tile = id % a.tiles_s, rest = id / a.tiles_s, head = rest % a.Hk, rest2 = rest / a.Hk;
-  const int part = rest2 % a.parts_s, seq = rest2 / a.parts_s;
+  const int rest = pair / a.Hk, seq = rest / a.parts_s, part = rest - seq * a.parts_s;
+  tile = a.tiles_s - 1 - tile;  // the tiles that see the most first
   int t0 = seq, n = 1;  // the sequence's query tokens
   if (a.starts) {
     t0 = max(a.starts[seq], 0);
     n = min(a.starts[seq + 1], a.T) - t0;
   }
-  const int len = min(a.lens[seq], a.max_len);
-  it.head = head;
+  if (a.joined) it.front = a.prefix_len;
+  const int len = it.front + min(a.lens[seq], a.max_len);
+  it.head = pair - rest * a.Hk;
   it.row0 = tile * TILE;
   it.rows = min(n, a.max_q) * a.G;
   it.token0 = t0;
   it.begin = part * a.part_s;
-  it.len = len;
   it.causal = n > 1;
   it.seen0 = len - n + 1;
-  // the tile's last token sees the most
+  // the tile's last token sees the most; what precedes the sequence's first token sees the prefix
   const int last = min(it.rows - 1, it.row0 + TILE - 1);
-  it.end = min(min(it.begin + a.part_s, len), it.seen0 + last / a.G);
+  it.end = min(min(it.begin + a.part_s, len), max(it.seen0 + last / a.G, it.front));
   it.table = a.pages + seq * a.ld_pages;
   it.slot = a.parts_p + part;
   // a part past the sequence is not asked for by the join; the first one always is
@@ -103,7 +128,9 @@ __device__ __forceinline__ bool attn_item(const AttnArgs& a, int id, AttnItem& i
 
 // Key t's row in 16-byte units from the first page; kNoRow for a page outside the cache.
 __device__ __forceinline__ uint32_t attn_row(const AttnArgs& a, const AttnItem& it, int t) {
-  const int page = t / a.page, off = t - page * a.page, id = it.table[page];
+  const int32_t* table = t < it.front ? a.prefix_pages : it.table;
+  if (t >= it.front) t -= it.front;
+  const int page = t / a.page, off = t - page * a.page, id = table[page];
   return id >= 0 && id < a.n_pages ? (uint32_t)id * a.c_page + (uint32_t)off * a.c_token : kNoRow;
 }
 
@@ -112,10 +139,6 @@ __device__ __forceinline__ uint32_t attn_row(const AttnArgs& a, const AttnItem& 
 __device__ __forceinline__ void attn_row_table(const AttnArgs& a, const AttnItem& it, uint32_t* tab, int tile) {
   const int n = max(it.end - it.begin, 0), padded = (n + tile - 1) / tile * tile;
   for (int i = threadIdx.x; i < padded; i += blockDim.x) tab[i] = i < n ? attn_row(a, it, it.begin + i) : kNoRow;
-}
-
-__device__ __forceinline__ uint4 attn_ld16(const uint8_t* base, uint32_t row, int unit) {
-  return *reinterpret_cast<const uint4*>(base + ((uint64_t)row + (uint32_t)unit) * 16);
 }
 
 // The transposing LDS reads: 16 lanes read 4 keys x 16 columns of 16 bits (8 keys of 8 bits), lanes 4 j .. 4 j + 3 (2 j, 2 j + 1)

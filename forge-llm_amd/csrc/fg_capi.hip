@@ -1236,16 +1236,17 @@ namespace {
 
 // The sizes of an attention call into `a`; a message for sizes that no plan is made for.
 const char* attn_sizes(fg::AttnArgs& a, int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
-                       int64_t prefix_len, int64_t max_seq_len, int64_t max_query_len, bool ragged) {
+                       int64_t prefix_len, int64_t max_seq_len, int64_t max_query_len, bool ragged, int item) {
   if (T < 0 || B < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || prefix_len < 0 || max_seq_len < 0 ||
       max_query_len <= 0)
     return "bad sizes";
   if (q_heads % kv_heads) return "q_heads is no multiple of kv_heads";
   if (!ragged && (T != B || max_query_len != 1)) return "without query_start each sequence has one query token";
-  if (T * q_heads >= kMaxDim || prefix_len >= kMaxDim - 4096 || max_seq_len >= kMaxDim - 4096 ||
+  if (T * q_heads >= kMaxDim || prefix_len >= kMaxDim / 2 - 4096 || max_seq_len >= kMaxDim / 2 - 4096 ||
       max_query_len * q_heads >= kMaxDim || B * max_query_len * q_heads >= kMaxDim)
     return "sizes past 32 bits";
   a.T = (int)T; a.B = (int)B; a.Hq = q_heads; a.Hk = kv_heads; a.G = q_heads / kv_heads; a.D = head_dim;
+  a.item = item;
   a.prefix_len = (int)prefix_len; a.max_len = (int)max_seq_len; a.max_q = (int)max_query_len;
   a.starts = ragged ? reinterpret_cast<const int32_t*>(1) : nullptr;  // the plan asks only whether there are any
   return nullptr;
@@ -1256,10 +1257,12 @@ const char* attn_sizes(fg::AttnArgs& a, int64_t T, int64_t B, int32_t q_heads, i
 extern "C" {
 
 size_t fg_prefix_attention_workspace_bytes(int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
-                                           int64_t prefix_len, int64_t max_seq_len, int64_t max_query_len,
-                                           int32_t ragged) {
+                                           int cache_dtype, int64_t prefix_len, int64_t max_seq_len,
+                                           int64_t max_query_len, int32_t ragged) {
   fg::AttnArgs a = {};
-  if (attn_sizes(a, T, B, q_heads, kv_heads, head_dim, prefix_len, max_seq_len, max_query_len, ragged != 0)) return 0;
+  if (attn_sizes(a, T, B, q_heads, kv_heads, head_dim, prefix_len, max_seq_len, max_query_len, ragged != 0,
+                 item_bytes(cache_dtype)))
+    return 0;
   return T == 0 ? 0 : fg::attn_plan(a);
 }
 
@@ -1272,7 +1275,7 @@ int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtyp
   if (bad) return bad;
   fg::AttnArgs a = {};
   if (const char* why = attn_sizes(a, T, B, q_heads, cache->kv_heads, cache->head_dim, prefix_len, max_seq_len,
-                                   max_query_len, query_start != nullptr))
+                                   max_query_len, query_start != nullptr, item_bytes(cache->dtype)))
     return fail(FG_EINVAL, "fg_prefix_attention: %s", why);
   if (T == 0) return FG_OK;
   if (dtype != FG_F16 && dtype != FG_BF16) return fail(FG_EINVAL, "fg_prefix_attention: q is fp16 or bf16");

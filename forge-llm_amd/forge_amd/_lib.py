@@ -92,7 +92,7 @@ SIGNATURES = {
                        INT),
     "fg_rope_append": ([P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, INT, P, I32_, P, I64, I64, I32_, I32_, P,
                         I32_, P, I64, I32_, P], INT),
-    "fg_prefix_attention_workspace_bytes": ([I64, I64, I32_, I32_, I32_, I64, I64, I64, I32_], SZ),
+    "fg_prefix_attention_workspace_bytes": ([I64, I64, I32_, I32_, I32_, INT, I64, I64, I64, I32_], SZ),
     "fg_prefix_attention": ([P, I64, I64, INT, P, P, I64, P, I64, P, P, I64, I64, I32_, I64, I64, F32_, P, I64, I64, P,
                              P, SZ, P], INT),
     "fg_version": ([], ctypes.c_char_p),

@@ -13,6 +13,7 @@ allocator, so a layer can be captured in a HIP graph.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import NamedTuple
 
@@ -23,13 +24,17 @@ from .errors import ConfigError
 from .ops_gemm import _as_rows, _check, _code_or_zero, _done, _ld, _on_gpu
 
 _16BIT = (torch.float16, torch.bfloat16)
+_FLOATS = (torch.float32, *_16BIT)
+_CODE = _lib.DTYPE_CODE
 _QUANT = {None: None, "int8": torch.int8, "fp8": torch.float8_e4m3fn, "fp8_block": torch.float8_e4m3fn}
 
 
-def _same_device(op: str, x: torch.Tensor, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != x.device:
-            raise ConfigError(f"{op}: {name} is on {t.device}, the call is on {x.device}")
+def _elsewhere(op: str, x: torch.Tensor, *tensors: torch.Tensor | None) -> None:
+    """Raise if one of ``tensors`` is not on ``x``'s GPU."""
+    dev = x.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ConfigError(f"{op}: a tensor is on {t.device}, the call is on {x.device}")
 
 
 # ================================================================================================ norm
@@ -54,54 +59,59 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Te
     _on_gpu(x, "add_rmsnorm")
     if quant not in _QUANT:
         raise ConfigError(f"add_rmsnorm: unknown quant {quant!r}: use None, int8, fp8 or fp8_block")
-    if not x.is_floating_point() or x.dtype not in (torch.float32, *_16BIT):
+    xdt = x.dtype
+    if xdt not in _FLOATS:
         raise ConfigError("add_rmsnorm: x must be an fp32, fp16 or bf16 tensor")
-    if x.dim() == 0:
+    shape = x.shape
+    if not shape:
         raise ConfigError("add_rmsnorm: x needs a last dimension to norm")
-    k = x.shape[-1]
-    _same_device("add_rmsnorm", x, weight=weight, residual=residual, residual_out=residual_out)
+    k = shape[-1]
+    _elsewhere("add_rmsnorm", x, weight, residual, residual_out)
     if weight is not None:
-        if weight.shape != (k,) or weight.dtype not in (torch.float32, *_16BIT):
+        if weight.shape != (k,) or weight.dtype not in _FLOATS:
             raise ConfigError(f"add_rmsnorm: weight must be an fp32, fp16 or bf16 tensor of [{k}]")
         weight = weight.contiguous()
     x2 = _as_rows(x)
     m = x2.shape[0]
     r2 = ro2 = None
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype not in (x.dtype, torch.float32):
+        rdt = residual.dtype
+        if residual.shape != shape or (rdt is not xdt and rdt is not torch.float32):
             raise ConfigError("add_rmsnorm: residual must have x's shape and x's type or fp32")
         r2 = _as_rows(residual)
         if residual_out is None:
-            residual_out = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-        elif residual_out.shape != x.shape or residual_out.dtype != residual.dtype:
+            residual_out = residual.new_empty(shape)
+            ro2 = residual_out if x2 is x else residual_out.view(m, k)
+        elif residual_out.shape != shape or residual_out.dtype is not rdt:
             raise ConfigError("add_rmsnorm: residual_out must be like residual")
-        ro2 = _as_rows(residual_out)
-        if m and ro2.data_ptr() != residual_out.data_ptr():
-            raise ConfigError("add_rmsnorm: residual_out must be rows of adjacent columns that do not overlap")
+        else:
+            ro2 = _as_rows(residual_out)
+            if m and ro2.data_ptr() != residual_out.data_ptr():
+                raise ConfigError("add_rmsnorm: residual_out must be rows of adjacent columns that do not overlap")
     elif residual_out is not None:
         raise ConfigError("add_rmsnorm: residual_out without a residual")
-    ydt = _QUANT[quant] or x.dtype
-    y = torch.empty((m, k), dtype=ydt, device=x.device)
+    ydt = _QUANT[quant] or xdt
+    y = x.new_empty((m, k), dtype=ydt)
     scale, s_row, s_block = None, 0, 0
     if quant == "fp8_block":
         if block < 8 or block > 512 or block & (block - 1):
             raise ConfigError("add_rmsnorm: block is a power of two from 8 to 512")
-        scale = torch.empty((-(-k // block), m), dtype=torch.float32, device=x.device).t()
+        scale = x.new_empty((-(-k // block), m), dtype=torch.float32).t()
         s_row, s_block = 1, max(m, 1)
     elif quant is not None:
-        scale, s_row = torch.empty(m, dtype=torch.float32, device=x.device), 1
+        scale, s_row = x.new_empty((m,), dtype=torch.float32), 1
     if m and k:
         _check(_lib.lib().fg_add_rmsnorm(
-            _lib.ptr(x2), _ld(x2), _lib.dtype_code(x2.dtype), _lib.ptr(r2), 0 if r2 is None else _ld(r2), _lib.ptr(ro2),
-            0 if ro2 is None else _ld(ro2), _code_or_zero(r2), _lib.ptr(weight), _code_or_zero(weight), eps, _lib.ptr(y),
-            k, _lib.dtype_code(ydt), _lib.ptr(scale), s_row, s_block, block if quant == "fp8_block" else 0, m, k,
+            x2.data_ptr(), _ld(x2), _CODE[xdt], _lib.ptr(r2), 0 if r2 is None else _ld(r2), _lib.ptr(ro2),
+            0 if ro2 is None else _ld(ro2), _code_or_zero(r2), _lib.ptr(weight), _code_or_zero(weight), eps, y.data_ptr(),
+            k, _CODE[ydt], _lib.ptr(scale), s_row, s_block, block if quant == "fp8_block" else 0, m, k,
             _lib.stream_of(x2)), "fg_add_rmsnorm")
     _done("add_rmsnorm")
-    return NormOutput(y if x.dim() == 2 else y.reshape(x.shape), scale, x if residual is None else residual_out)
+    return NormOutput(y if x2 is x else y.view(shape), scale, x if residual is None else residual_out)
 
 
 # ================================================================================================ paged cache
-@dataclass
+@dataclass(frozen=True)
 class PagedKVCache:
     """Keys and values of many sequences in pages: ``k`` and ``v`` are ``[pages, kv_heads, page_size, head_dim]`` (any
     strides of whole 16-byte units, the same for both, columns adjacent) in fp16, bf16 or float8_e4m3fn; an e4m3 value
@@ -146,34 +156,33 @@ class PagedKVCache:
     def page_size(self) -> int:
         return self.k.shape[2]
 
-    def _handle(self) -> _lib.KVCache:
-        pages, heads, page, dim = self.k.shape
-        sp, sh, st, _ = self.k.stride()
-        return _lib.KVCache(_lib.ptr(self.k), _lib.ptr(self.v), _lib.ptr(self.k_scale), _lib.ptr(self.v_scale), sp, sh, st,
-                            pages, _lib.dtype_code(self.k.dtype), heads, page, dim)
-
-
-def _heads(op: str, name: str, t: torch.Tensor, dim: int) -> None:
-    if t.dim() != 3 or t.shape[2] != dim:
-        raise ConfigError(f"{op}: {name} must be [tokens, heads, {dim}]")
-    if t.dtype not in _16BIT:
-        raise ConfigError(f"{op}: {name} must be fp16 or bf16")
-
-
-def _columns(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _fits_cache(op: str, q: torch.Tensor, cache: PagedKVCache) -> None:
-    _same_device(op, q, cache=cache.k)
-    if cache.k.dtype != q.dtype and cache.k.dtype != torch.float8_e4m3fn:
-        raise ConfigError(f"{op}: a {cache.k.dtype} cache does not take {q.dtype} queries")
+    def _handle(self) -> tuple[int, torch.dtype, tuple[int, ...]]:
+        """Address of the C description (made on first use, and again if a tensor's memory has moved), type and shape."""
+        got = self.__dict__.get("_made")
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        if got is None or got[0].k != k.data_ptr() or got[0].v != v.data_ptr() or (
+                ks is not None and (got[0].k_scale != ks.data_ptr() or got[0].v_scale != vs.data_ptr())):
+            shape, (sp, sh, st, _) = tuple(k.shape), k.stride()
+            made = _lib.KVCache(_lib.ptr(k), _lib.ptr(v), _lib.ptr(ks), _lib.ptr(vs), sp, sh, st, shape[0], _CODE[k.dtype],
+                                *shape[1:])
+            got = self.__dict__["_made"] = (made, (_lib.ctypes.addressof(made), k.dtype, shape))
+        return got[1]
 
 
 def _index(op: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
-    if t.dim() != 1 or t.shape[0] != n or t.dtype not in (torch.int32, torch.int64):
+    if t.shape != (n,) or (t.dtype is not torch.int64 and t.dtype is not torch.int32):
         raise ConfigError(f"{op}: {name} must be an int32 or int64 tensor of [{n}]")
     return t.contiguous()
+
+
+def _heads(op: str, name: str, t: torch.Tensor, dt: torch.dtype, shape: tuple[int | None, ...]) -> torch.Tensor:
+    """``t`` as ``[tokens, heads, dim]`` of 16-bit type ``dt`` with adjacent columns (copied only if they are not); None in
+    ``shape`` is any size."""
+    if t.dim() != 3 or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise ConfigError(f"{op}: {name} must be {['any' if n is None else n for n in shape]}, got {list(t.shape)}")
+    if t.dtype is not dt or dt not in _16BIT:
+        raise ConfigError(f"{op}: {name} must be fp16 or bf16, and of q's type")
+    return t if t.stride(2) == 1 or shape[2] == 1 else t.contiguous()
 
 
 # ================================================================================================ rotation and append
@@ -192,30 +201,29 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     """
     op = "rope_append"
     _on_gpu(q, op)
-    _fits_cache(op, q, cache)
-    dim, hk = cache.k.shape[3], cache.k.shape[1]
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _heads(op, name, t, dim)
-    t = q.shape[0]
-    if k.shape[:2] != (t, hk) or v.shape[:2] != (t, hk) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ConfigError(f"{op}: k and v must be [{t}, {hk}, {dim}] of q's type")
-    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.shape[1] % 2 or not 2 <= cos_sin.shape[1] <= dim:
+    handle, cdt, (_, hk, _, dim) = cache._handle()
+    _elsewhere(op, q, k, v, positions, cos_sin, slots, cache.k, q_out)
+    dt = q.dtype
+    if cdt is not dt and cdt is not torch.float8_e4m3fn:
+        raise ConfigError(f"{op}: a {cdt} cache does not take {dt} queries")
+    q = _heads(op, "q", q, dt, (None, None, dim))
+    t, h, _ = shape = q.shape
+    k, v = _heads(op, "k", k, dt, (t, hk, dim)), _heads(op, "v", v, dt, (t, hk, dim))
+    if cos_sin.dim() != 2 or cos_sin.dtype is not torch.float32 or cos_sin.shape[1] % 2 or not 2 <= cos_sin.shape[1] <= dim:
         raise ConfigError(f"{op}: cos_sin must be fp32 [positions, rot] with an even rot up to {dim}")
-    _same_device(op, q, k=k, v=v, positions=positions, cos_sin=cos_sin, slots=slots, q_out=q_out)
     positions, slots = _index(op, "positions", positions, t), _index(op, "slots", slots, t)
-    q, k, v, cos_sin = _columns(q), _columns(k), _columns(v), _columns(cos_sin)
+    if cos_sin.stride(1) != 1:
+        cos_sin = cos_sin.contiguous()
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif q_out.shape != q.shape or q_out.dtype != q.dtype or (q_out.stride(-1) != 1 and q_out.shape[-1] > 1):
+        q_out = q.new_empty(shape)
+    elif q_out.shape != shape or q_out.dtype is not dt or (q_out.stride(2) != 1 and dim > 1):
         raise ConfigError(f"{op}: q_out must be like q, with adjacent columns")
     if t:
-        handle = cache._handle()
+        (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), q_out.stride()
         _check(_lib.lib().fg_rope_append(
-            _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0),
-            v.stride(1), _lib.ptr(q_out), q_out.stride(0), q_out.stride(1), _lib.dtype_code(q.dtype), _lib.ptr(positions),
-            positions.dtype == torch.int64, _lib.ptr(cos_sin), _ld(cos_sin), cos_sin.shape[0], cos_sin.shape[1],
-            interleaved, _lib.ptr(slots), slots.dtype == torch.int64, _lib.ctypes.addressof(handle), t, q.shape[1],
-            _lib.stream_of(q)), "fg_rope_append")
+            q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, q_out.data_ptr(), o0, o1, _CODE[dt],
+            positions.data_ptr(), positions.dtype is torch.int64, cos_sin.data_ptr(), _ld(cos_sin), *cos_sin.shape, interleaved,
+            slots.data_ptr(), slots.dtype is torch.int64, handle, t, h, _lib.stream_of(q)), "fg_rope_append")
     _done(op)
     return q_out
 
@@ -246,19 +254,22 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     """
     op = "prefix_attention"
     _on_gpu(q, op)
-    _fits_cache(op, q, cache)
-    _, hk, page, dim = cache.k.shape
-    _heads(op, "q", q, dim)
-    t, h, _ = q.shape
+    handle, cdt, (_, hk, page, dim) = cache._handle()
+    _elsewhere(op, q, page_table, seq_lens, prefix_pages, query_start, cache.k, out)
+    dt = q.dtype
+    if cdt is not dt and cdt is not torch.float8_e4m3fn:
+        raise ConfigError(f"{op}: a {cdt} cache does not take {dt} queries")
+    q = _heads(op, "q", q, dt, (None, None, dim))
+    t, h, _ = shape = q.shape
     if h % hk or h == 0:
         raise ConfigError(f"{op}: {h} query heads are no multiple of {hk} key heads")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32:
+    if page_table.dim() != 2 or page_table.dtype is not torch.int32:
         raise ConfigError(f"{op}: page_table must be int32 [sequences, pages]")
     b, width = page_table.shape
-    if seq_lens.shape != (b,) or seq_lens.dtype != torch.int32:
+    if seq_lens.shape != (b,) or seq_lens.dtype is not torch.int32:
         raise ConfigError(f"{op}: seq_lens must be int32 [{b}]")
     ragged = query_start is not None
-    if ragged and (query_start.shape != (b + 1,) or query_start.dtype != torch.int32):
+    if ragged and (query_start.shape != (b + 1,) or query_start.dtype is not torch.int32):
         raise ConfigError(f"{op}: query_start must be int32 [{b + 1}]")
     if not ragged and (t != b or max_query_len != 1):
         raise ConfigError(f"{op}: without query_start each of the {b} sequences has one query token, got {t}")
@@ -268,30 +279,35 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
         max_seq_len = width * page
     elif not 0 <= max_seq_len <= width * page:
         raise ConfigError(f"{op}: max_seq_len {max_seq_len} is past the page table's {width} pages of {page}")
-    if prefix_len and (prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.dtype != torch.int32
+    if prefix_len and (prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.dtype is not torch.int32
                        or prefix_pages.shape[0] * page < prefix_len):
         raise ConfigError(f"{op}: a prefix of {prefix_len} tokens needs int32 prefix_pages that hold them")
-    _same_device(op, q, page_table=page_table, seq_lens=seq_lens, prefix_pages=prefix_pages, query_start=query_start, out=out)
     if out is None:
-        out = torch.empty((t, h, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or (out.stride(-1) != 1 and dim > 1):
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype is not dt or (out.stride(2) != 1 and dim > 1):
         raise ConfigError(f"{op}: out must be like q, with adjacent columns")
-    lse = torch.empty((t, h), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((t, h), dtype=torch.float32) if return_lse else None
     if t:
-        q = _columns(q)
-        page_table = page_table if page_table.stride(1) == 1 or width <= 1 else page_table.contiguous()
+        if width > 1 and page_table.stride(1) != 1:
+            page_table = page_table.contiguous()
         seq_lens = seq_lens.contiguous()
         prefix_pages = prefix_pages.contiguous() if prefix_len else None
         query_start = query_start.contiguous() if ragged else None
-        lib = _lib.lib()
-        need = lib.fg_prefix_attention_workspace_bytes(t, b, h, hk, dim, prefix_len, max_seq_len, max_query_len, ragged)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        handle = cache._handle()
-        _check(lib.fg_prefix_attention(
-            _lib.ptr(q), q.stride(0), q.stride(1), _lib.dtype_code(q.dtype), _lib.ctypes.addressof(handle),
-            _lib.ptr(prefix_pages), prefix_len, _lib.ptr(page_table), _ld(page_table), _lib.ptr(seq_lens),
-            _lib.ptr(query_start), t, b, h, max_seq_len, max_query_len, dim ** -0.5 if scale is None else scale,
-            _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(lse), _lib.ptr(ws), need, _lib.stream_of(q)),
-            "fg_prefix_attention")
+        need = _attention_workspace(q.get_device(), t, b, h, hk, dim, prefix_len, max_seq_len, max_query_len, ragged, cdt)
+        ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+        (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
+        _check(_lib.lib().fg_prefix_attention(
+            q.data_ptr(), q0, q1, _CODE[dt], handle, _lib.ptr(prefix_pages), prefix_len, page_table.data_ptr(),
+            _ld(page_table), seq_lens.data_ptr(), _lib.ptr(query_start), t, b, h, max_seq_len, max_query_len,
+            dim ** -0.5 if scale is None else scale, out.data_ptr(), o0, o1, _lib.ptr(lse), _lib.ptr(ws), need,
+            _lib.stream_of(q)), "fg_prefix_attention")
     _done(op)
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(_device: int, t: int, b: int, h: int, hk: int, dim: int, prefix_len: int, max_seq_len: int,
+                         max_query_len: int, ragged: bool, cdt: torch.dtype) -> int:
+    """Bytes of a call's partial sums, which follow from its sizes (and the GPU's CUs) alone."""
+    return _lib.lib().fg_prefix_attention_workspace_bytes(t, b, h, hk, dim, _CODE[cdt], prefix_len, max_seq_len, max_query_len,
+                                                          ragged)

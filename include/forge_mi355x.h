@@ -314,8 +314,8 @@ int fg_rope_append(const void* q, int64_t q_token, int64_t q_head, const void* k
  *   lse (may be NULL): float [T][q_heads], the natural logarithm of the softmax's sum.
  *   workspace: fg_prefix_attention_workspace_bytes bytes, 16-byte aligned. */
 size_t fg_prefix_attention_workspace_bytes(int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
-                                           int64_t prefix_len, int64_t max_seq_len, int64_t max_query_len,
-                                           int32_t ragged);
+                                           int cache_dtype, int64_t prefix_len, int64_t max_seq_len,
+                                           int64_t max_query_len, int32_t ragged);
 int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const fg_kv_cache* cache,
                         const int32_t* prefix_pages, int64_t prefix_len, const int32_t* page_table, int64_t ld_pages,
                         const int32_t* seq_lens, const int32_t* query_start, int64_t T, int64_t B, int32_t q_heads,

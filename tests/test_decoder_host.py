@@ -89,7 +89,11 @@ def test_attention_without_queries_is_no_error():
 
 
 def test_workspace_follows_the_plan():
-    ws = _lib.lib().fg_prefix_attention_workspace_bytes
+    query = _lib.lib().fg_prefix_attention_workspace_bytes
+
+    def ws(t, b, h, hk, d, *rest):
+        return query(t, b, h, hk, d, _lib.BF16, *rest)
+
     assert ws(0, 4, 8, 2, 64, 100, 100, 1, 1) == 0 and ws(4, 4, 7, 2, 64, 0, 100, 1, 0) == 0
     assert ws(64, 64, 32, 8, 128, 0, 100, 1, 0) == 0  # one part for each sequence: nothing to join
     row = 32 * (128 * 4 + 8)
@@ -105,7 +109,7 @@ def test_cache_descriptions():
     one = torch.ones(2)
     e4 = torch.zeros(4, 2, 16, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
     cache = ops.PagedKVCache(e4, e4, one, one)
-    assert cache.page_size == 16 and cache._handle().k == e4.data_ptr() and cache._handle().page_stride == 2048
+    assert cache.page_size == 16 and cache._handle()[1:] == (torch.float8_e4m3fn, (4, 2, 16, 64))
     for args in ((k, k[:3]), (k, k.half()), (k.float(), k.float()), (k[0], k[0]), (k, k.transpose(1, 2).contiguous().transpose(1, 2)),
                  (k.transpose(2, 3), k.transpose(2, 3)), (k, k, one, one), (e4, e4), (e4, e4, one), (e4, e4, one, torch.ones(3)),
                  (e4, e4, one, one.double())):
