@@ -71,6 +71,24 @@ __host__ __device__ __forceinline__ int64_t attn_count(int64_t pairs, int64_t ti
   return (pairs < (1 << 30) && attn_by_xcd((int)pairs) ? (pairs + 7) / 8 * 8 : pairs) * tiles;
 }
 
+// Rows of query tokens that no item computes, written where no join follows: tokens of no sequence give zeros (the first
+// sequence's workgroup takes those in front of it, the last one's those behind it), tokens past max_query_len NaN.
+__device__ __forceinline__ void attn_uncovered(const AttnArgs& a, int seq, int head) {
+  auto fill = [&](int from, int to, float out, float lse) {
+    for (int64_t i = (int64_t)from * a.G * a.D + threadIdx.x; i < (int64_t)to * a.G * a.D; i += blockDim.x) {
+      const int col = (int)(i % a.D), h = head * a.G + (int)(i / a.D % a.G);
+      const int64_t t = i / a.D / a.G;
+      a.out[t * a.o_t + h * a.o_h + col] = out == 0.f ? 0 : 0x7fff;  // a NaN of either type
+      if (a.lse && col == 0) a.lse[t * a.Hq + h] = lse;
+    }
+  };
+  const float nan = __builtin_nanf(""), inf = __builtin_inff();
+  const int first = max(a.starts[seq], 0), next = min(a.starts[seq + 1], a.T);
+  if (first + a.max_q < next) fill(first + a.max_q, next, nan, nan);
+  if (seq == 0 && first > 0) fill(0, min(first, a.T), 0.f, -inf);
+  if (seq == a.B - 1 && next < a.T) fill(max(next, 0), a.T, 0.f, -inf);
+}
+
 // Item `id` of the grid; false: nothing to do.  TILE rows per item.
 template <int TILE>
 __device__ __forceinline__ bool attn_item(const AttnArgs& a, int id, AttnItem& it) {
@@ -108,9 +126,10 @@ __device__ __forceinline__ bool attn_item(const AttnArgs& a, int id, AttnItem& i
     t0 = max(a.starts[seq], 0);
     n = min(a.starts[seq + 1], a.T) - t0;
   }
+  it.head = pair - rest * a.Hk;
+  if (a.starts && !a.acc && tile == 0 && part == 0) attn_uncovered(a, seq, it.head);
   if (a.joined) it.front = a.prefix_len;
   const int len = it.front + min(a.lens[seq], a.max_len);
-  it.head = pair - rest * a.Hk;
   it.row0 = tile * TILE;
   it.rows = min(n, a.max_q) * a.G;
   it.token0 = t0;

@@ -100,13 +100,13 @@ size_t attn_plan(AttnArgs& a) {
   a.parts_p = a.tiles_p = a.part_p = 0;
   int64_t items_p = 0;
   if (a.prefix_len && !a.joined)
-    items_p = plan_segment(a.prefix_len, rows_p, a.Hk, a.tile_p, a.tile_p ? (a.tile_s || a.lead ? 2 : 1) : 4, &a.tiles_p, &a.parts_p,
+    items_p = plan_segment(a.prefix_len, rows_p, a.Hk, a.tile_p, a.tile_p && (a.tile_s || a.lead) ? 2 : 1, &a.tiles_p, &a.parts_p,
                            &a.part_p);
   const int64_t items = items_p + plan_segment((a.joined ? (int64_t)a.prefix_len : 0) + a.max_len, rows_s, (int64_t)a.Hk * a.B,
-                                               a.tile_s, a.tile_s || !items_p ? 2 : 4, &a.tiles_s, &a.parts_s, &a.part_s);
+                                               a.tile_s, a.tile_s ? 2 : (a.tile_p && items_p ? 4 : 1), &a.tiles_s, &a.parts_s, &a.part_s);
   a.items_p = (int)items_p;
   a.items = items < (1LL << 31) - 64 ? (int)items : -1;
-  if (a.parts_p + a.parts_s == 1 && !a.starts) return 0;
+  if (a.parts_p + a.parts_s == 1 && a.B > 0) return 0;  // nothing to join
   return (size_t)(a.parts_p + a.parts_s) * a.T * a.Hq * ((size_t)a.D * 4 + sizeof(float2));
 }
 

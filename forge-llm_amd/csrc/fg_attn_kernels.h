@@ -7,7 +7,7 @@
 namespace fg {
 
 template <bool BF16, bool FP8, int DP>
-__global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attn_rows_kernel(const AttnArgs a) {
   __shared__ __align__(16) uint8_t lds[RowsLds<FP8, DP>::kBytes];
   attn_rows<BF16, FP8, DP>(a, blockIdx.x, lds);
 }

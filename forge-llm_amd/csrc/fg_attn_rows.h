@@ -1,5 +1,5 @@
 // attn_rows: work items of up to 16 rows (decoding).  What bounds them is the read of the keys and values, so each wavefront
-// works by itself on tiles of 32 keys, without a barrier, and loads the next tile while it computes this one.
+// works by itself on tiles of 32 keys, without a barrier, with the loads of the next tile and the one after on their way.
 //   S^T = K Q^T   (A: 16 keys x 32 columns straight from global memory, 16 bytes per lane; B: the rows, in registers)
 //   O^T += V^T P^T
 // S^T comes out with a row in each lane and keys 4 g + i (g the lane's group of 16) in its registers, which is the order in
@@ -70,48 +70,46 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int id, uint8_t* ld
 
   const int n = max(it.end - it.begin, 0), step = kRowsTile * kRowsWaves;
   uint8_t* vl = lds + wave * L::kV;
-  uint4 kr[2][KU], vr[2][KU];
-  uint32_t rows[2] = {kNoRow, kNoRow}, ok = 0;  // bit t of ok: key t of the tile is there
-  auto find = [&](int t0) __attribute__((always_inline)) {
-    rows[0] = tab[t0 + l16];
-    rows[1] = tab[t0 + 16 + l16];
-    ok = (uint32_t)(__ballot(rows[0] != kNoRow) & 0xffff) | (uint32_t)(__ballot(rows[1] != kNoRow) & 0xffff) << 16;
-  };
-  auto fetch = [&](const uint8_t* base, uint4(&to)[2][KU]) __attribute__((always_inline)) {
-    if (ok == 0xffffffffu && a.D == DP) {
+  // NB tiles in registers: with two, one is computed while the other is on its way (256 columns leave room for one: the next
+  // is loaded behind the products that used it)
+  constexpr int NB = DP > 128 ? 1 : 2;
+  uint4 kr[NB][2][KU], vr[NB][2][KU];
+  uint32_t ok[NB];  // bit t: key t of the tile is there
+  auto fetch = [&](int b, int t0) __attribute__((always_inline)) {
+    const uint32_t rows[2] = {tab[t0 + l16], tab[t0 + 16 + l16]};
+    ok[b] = (uint32_t)(__ballot(rows[0] != kNoRow) & 0xffff) | (uint32_t)(__ballot(rows[1] != kNoRow) & 0xffff) << 16;
+    if (ok[b] == 0xffffffffu && a.D == DP) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int c = 0; c < KU; ++c) to[h][c] = *reinterpret_cast<const uint4*>(base + (uint64_t)rows[h] * 16 + c * 64);
+        for (int c = 0; c < KU; ++c) {
+          const uint64_t at = (uint64_t)rows[h] * 16 + c * 64;
+          kr[b][h][c] = *reinterpret_cast<const uint4*>(kb + at);
+          vr[b][h][c] = *reinterpret_cast<const uint4*>(vb + at);
+        }
     } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int c = 0; c < KU; ++c) {
-          to[h][c] = make_uint4(0, 0, 0, 0);
-          if (rows[h] != kNoRow && 4 * c + grp < units) to[h][c] = *reinterpret_cast<const uint4*>(base + (uint64_t)rows[h] * 16 + c * 64);
+          kr[b][h][c] = vr[b][h][c] = make_uint4(0, 0, 0, 0);
+          if (rows[h] != kNoRow && 4 * c + grp < units) {
+            const uint64_t at = (uint64_t)rows[h] * 16 + c * 64;
+            kr[b][h][c] = *reinterpret_cast<const uint4*>(kb + at);
+            vr[b][h][c] = *reinterpret_cast<const uint4*>(vb + at);
+          }
         }
     }
   };
-  if (wave * kRowsTile < n) {
-    find(wave * kRowsTile);
-    fetch(vb, vr);
-    fetch(kb, kr);
-  }
-  for (int t0 = wave * kRowsTile; t0 < n; t0 += step) {
-    const uint32_t here = ok;
-    const bool more = t0 + step < n;
+  auto turn = [&](int b, int t0) __attribute__((always_inline)) {
+    const uint32_t here = ok[b];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int c = 0; c < KU; ++c) {
         const int t = 16 * h + l16;
-        *reinterpret_cast<uint4*>(vl + (t * U + rows_unit<U>(t, 4 * c + grp)) * 16) = vr[h][c];
+        *reinterpret_cast<uint4*>(vl + (t * U + rows_unit<U>(t, 4 * c + grp)) * 16) = vr[b][h][c];
       }
-    if (more) {
-      find(t0 + step);
-      fetch(vb, vr);
-    }
     f32x4 s[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -119,14 +117,14 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int id, uint8_t* ld
       for (int c = 0; c < C; ++c) {
         s16x8 kf;
         if constexpr (FP8) {
-          const uint4& u = kr[h][c / 2];
+          const uint4& u = kr[b][h][c / 2];
           kf = c % 2 ? e4m3_to_16<BF16>(u.z, u.w) : e4m3_to_16<BF16>(u.x, u.y);
         } else {
-          kf = __builtin_bit_cast(s16x8, kr[h][c]);
+          kf = __builtin_bit_cast(s16x8, kr[b][h][c]);
         }
         s[h] = mfma16<BF16>(kf, qf[c], c ? s[h] : (f32x4)(0.f));
       }
-    if (more) fetch(kb, kr);
+    if (t0 + NB * step < n) fetch(b, t0 + NB * step);
     float x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = s[j / 4][j % 4];
@@ -180,6 +178,14 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int id, uint8_t* ld
       o[d] = mfma16<BF16>(vf, p, o[d]);
     }
     __builtin_amdgcn_wave_barrier();
+  };
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    if (wave * kRowsTile + b * step < n) fetch(b, wave * kRowsTile + b * step);
+  for (int t0 = wave * kRowsTile; t0 < n; t0 += NB * step) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (t0 + b * step < n) turn(b, t0 + b * step);
   }
 
   // join the wavefronts: maxima and sums first, then each adds up a quarter of the columns
