@@ -256,7 +256,10 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int id, uint8_t* ld
     }
     if (i + 1 < tiles) store(nxt);
   };
-  for (int i = 0; i < tiles; ++i) step(i, lds + (i & 1) * 2 * kBuf, lds + (~i & 1) * 2 * kBuf);
+  for (int i = 0; i < tiles; i += 2) {  // the buffers' places are constants of the reads' addresses
+    step(i, lds, lds + 2 * kBuf);
+    if (i + 1 < tiles) step(i + 1, lds + 2 * kBuf, lds);
+  }
 
   const float sum = l + __shfl_xor(l, 32, kWave), vs = FP8 ? a.vs[it.head] : 1.f;
   if (row >= it.rows) return;
