@@ -82,7 +82,7 @@ static int64_t plan_segment(int64_t len, int64_t rows, int64_t sets, bool tile, 
   return attn_count(*parts * sets, n);
 }
 
-// Fills in the plan; returns the partial sums' bytes.  items is -1 where the workgroups would pass 32 bits.  More than 16 rows
+// Fills in the plan; returns the partial sums' bytes.  items is -1 where the threads of a launch would pass 32 bits.  More than 16 rows
 // go to the kernel of many rows, which waits for nothing but memory even where most of its 128 rows are empty.
 size_t attn_plan(AttnArgs& a) {
   const int64_t rows_p = (int64_t)a.T * a.G, rows_s = (int64_t)a.max_q * a.G;
@@ -105,7 +105,7 @@ size_t attn_plan(AttnArgs& a) {
   const int64_t items = items_p + plan_segment((a.joined ? (int64_t)a.prefix_len : 0) + a.max_len, rows_s, (int64_t)a.Hk * a.B,
                                                a.tile_s, a.tile_s ? 2 : (a.tile_p && items_p ? 4 : 1), &a.tiles_s, &a.parts_s, &a.part_s);
   a.items_p = (int)items_p;
-  a.items = items < (1LL << 31) - 64 ? (int)items : -1;
+  a.items = items < (1LL << 24) - 64 ? (int)items : -1;
   if (a.parts_p + a.parts_s == 1 && a.B > 0) return 0;  // nothing to join
   return (size_t)(a.parts_p + a.parts_s) * a.T * a.Hq * ((size_t)a.D * 4 + sizeof(float2));
 }

@@ -85,3 +85,34 @@ def assert_attention(got, lse, ref, dtype):
         fine = torch.isfinite(ref_lse)
         assert torch.equal(fine, torch.isfinite(lse)) and torch.equal(lse[~fine], ref_lse[~fine])
         assert bool(((lse - ref_lse)[fine].abs() <= 2.0 ** -13 * (1 + ref_lse[fine].abs())).all())
+
+
+def attention_ref_fast(q, cache, page_table, seq_lens, prefix_pages, prefix_len, query_start, scale):
+    """attention_ref with a sequence's rows at once, in fp64 where q is (for sizes that row by row would take minutes); pages
+    are all in the cache."""
+    t, h, d = q.shape
+    hk = cache.k.shape[1]
+    out, mag = torch.zeros(t, h, d, dtype=torch.float64, device=q.device), torch.zeros(t, h, d, dtype=torch.float64, device=q.device)
+    lse = torch.full((t, h), -math.inf, dtype=torch.float64, device=q.device)
+
+    def tokens(name, pages, n):
+        x, s = getattr(cache, name), getattr(cache, name + "_scale")
+        pages = pages[:-(-n // x.shape[2])].long()
+        rows = x.view(torch.uint8)[pages].view(x.dtype) if x.element_size() == 1 else x[pages]
+        rows = rows.double().transpose(0, 1).reshape(hk, -1, d)[:, :n]
+        return rows if s is None else rows * s.double().view(-1, 1, 1)
+
+    starts = list(range(len(seq_lens) + 1)) if query_start is None else query_start.tolist()
+    for b, n in enumerate(seq_lens.tolist()):
+        k, v = (torch.cat((tokens(x, prefix_pages, prefix_len), tokens(x, page_table[b], n)), 1) for x in ("k", "v"))
+        a, c = starts[b], starts[b + 1]
+        if a == c or k.shape[1] == 0:
+            continue
+        sees = torch.arange(k.shape[1], device=q.device) < (prefix_len + n - (c - a) + 1 + torch.arange(c - a, device=q.device)).view(-1, 1)
+        for head in range(h):
+            s = (q[a:c, head].double() @ k[head // (h // hk)].t() * scale).masked_fill(~sees, -math.inf)
+            z = torch.logsumexp(s, 1)
+            p = torch.exp(s - z.view(-1, 1)).nan_to_num(0.0)
+            lse[a:c, head], out[a:c, head] = z, p @ v[head // (h // hk)]
+            mag[a:c, head] = p @ v[head // (h // hk)].abs()
+    return out.cpu(), lse.cpu(), mag.cpu()
