@@ -57,7 +57,8 @@ struct AttnItem {
   int token0;       // first query token of the segment
   int begin, end;   // its keys
   int front;        // keys in front that are the prefix's (an item of a sequence that takes both)
-  int seen0;        // keys that the segment's first query token sees; each further one sees one more (prefix: all see all)
+  int seen0;        // keys that the segment's first query token sees, each further one sees one more, and none fewer than
+                    // the front (not causal: all see all)
   bool causal;
   const int32_t* table;
   int slot;  // part index

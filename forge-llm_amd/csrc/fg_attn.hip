@@ -74,10 +74,17 @@ static int split_keys(int64_t len, int64_t items, int64_t want, int64_t unit, in
   return (int)std::max<int64_t>(1, (len + p - 1) / p);
 }
 
-// `want`: workgroups per CU.
+// `want`: workgroups per CU.  Up to kOnePart keys are one part of attn_rows, which needs no second launch (250 keys: 8.7 us
+// against 9.4 in two parts; 500: 12.1 against 9.5).
+constexpr int kOnePart = 256;
 static int64_t plan_segment(int64_t len, int64_t rows, int64_t sets, bool tile, int want, int* tiles, int* parts, int* part) {
   const int64_t per = tile ? kTileRows : 16, n = (rows + per - 1) / per;
   *tiles = (int)n;
+  if (!tile && len <= kOnePart) {
+    *part = (int)std::max<int64_t>(len, 1);
+    *parts = 1;
+    return attn_count(sets, n);
+  }
   *parts = split_keys(len, n * sets, (int64_t)want * device_cus(), tile ? 64 : kRowsTile * kRowsWaves, tile ? 1 << 30 : kMaxPart, part);
   return attn_count(*parts * sets, n);
 }
@@ -91,6 +98,14 @@ size_t attn_plan(AttnArgs& a) {
   // Sequences that fill two row tiles each on average take the prefix along with their own keys: the rows that packing the
   // whole batch's into tiles would save cost less than the parts' sums (4 prompts of 500 tokens x 4 heads: XX us, YY apart).
   a.joined = a.tile_s && a.prefix_len && rows_p >= 2 * kTileRows * (int64_t)a.B;
+  if (!a.tile_s && a.prefix_len) {
+    // So do single queries where all keys make one part, or where the sequences fill the CUs by themselves and reading the
+    // prefix again for each (at 8 TB/s, from L2) takes less than a second launch and two parts' sums.  (us, graph replays,
+    // 32 + 2 x 8 heads of 128, apart / along: 4 sequences, 100 + 130 tokens 9.3 / 8.4, 64 sequences 19.8 / 12.9, 64 x (250 +
+    // 130) 20.0 / 16.5, 64 x (500 + 130) 22.2 / 23.2, 4 x (500 + 130), which does not fill the CUs, 9.5 / 13.7.)
+    const double again = (double)a.B * a.prefix_len * a.Hk * a.D * 2 * a.item / 8e6, sums = 4 + 2.0 * a.T * a.Hq * a.D * 8 / 4e6;
+    a.joined = a.prefix_len + a.max_len <= kOnePart || ((int64_t)a.B * a.Hk >= device_cus() && again < sums);
+  }
   // The prefix's items go first where their products (1.2 us per tile of 64 keys, two at a time on a CU) outlast the reads of
   // the sequences' keys at 4 TB/s, and make two workgroups per CU.  Else they spread among the sequences' items, and one per
   // CU leaves fewer sums to join (64 sequences behind 8192 tokens: 59 us against 64 with two; 256 behind 32768, which go

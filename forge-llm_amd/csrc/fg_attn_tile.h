@@ -81,8 +81,8 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int id, uint8_t* ld
     u.x ^= sign; u.y ^= sign; u.z ^= sign; u.w ^= sign;
     qf[c] = __builtin_bit_cast(s16x8, u);
   }
-  const int seen = it.causal ? it.seen0 + tok : it.end;
-  const int min_seen = it.causal ? it.seen0 + row0 / a.G : it.end;  // what the wavefront's first row sees
+  const int seen = it.causal ? max(it.seen0 + tok, it.front) : it.end;
+  const int min_seen = it.causal ? max(it.seen0 + row0 / a.G, it.front) : it.end;  // what the wavefront's first row sees
   const float sc = fabsf(a.scale_log2) * (FP8 ? a.ks[it.head] : 1.f);
 
   f32x16 o[DB];

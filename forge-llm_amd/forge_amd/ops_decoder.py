@@ -172,17 +172,19 @@ class PagedKVCache:
 def _index(op: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
     if t.shape != (n,) or (t.dtype is not torch.int64 and t.dtype is not torch.int32):
         raise ConfigError(f"{op}: {name} must be an int32 or int64 tensor of [{n}]")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _heads(op: str, name: str, t: torch.Tensor, dt: torch.dtype, shape: tuple[int | None, ...]) -> torch.Tensor:
-    """``t`` as ``[tokens, heads, dim]`` of 16-bit type ``dt`` with adjacent columns (copied only if they are not); None in
-    ``shape`` is any size."""
-    if t.dim() != 3 or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise ConfigError(f"{op}: {name} must be {['any' if n is None else n for n in shape]}, got {list(t.shape)}")
-    if t.dtype is not dt or dt not in _16BIT:
-        raise ConfigError(f"{op}: {name} must be fp16 or bf16, and of q's type")
-    return t if t.stride(2) == 1 or shape[2] == 1 else t.contiguous()
+def _queries(op: str, q: torch.Tensor, cdt: torch.dtype, dim: int) -> torch.Tensor:
+    """``q`` as ``[tokens, heads, dim]`` with adjacent columns (copied only if they are not), of a type that the cache takes."""
+    if q.dim() != 3 or q.shape[2] != dim:
+        raise ConfigError(f"{op}: q must be [tokens, heads, {dim}], got {list(q.shape)}")
+    dt = q.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise ConfigError(f"{op}: q must be fp16 or bf16")
+    if cdt is not dt and cdt is not torch.float8_e4m3fn:
+        raise ConfigError(f"{op}: a {cdt} cache does not take {dt} queries")
+    return q if q.stride(2) == 1 or dim == 1 else q.contiguous()
 
 
 # ================================================================================================ rotation and append
@@ -203,27 +205,33 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     _on_gpu(q, op)
     handle, cdt, (_, hk, _, dim) = cache._handle()
     _elsewhere(op, q, k, v, positions, cos_sin, slots, cache.k, q_out)
+    q = _queries(op, q, cdt, dim)
     dt = q.dtype
-    if cdt is not dt and cdt is not torch.float8_e4m3fn:
-        raise ConfigError(f"{op}: a {cdt} cache does not take {dt} queries")
-    q = _heads(op, "q", q, dt, (None, None, dim))
     t, h, _ = shape = q.shape
-    k, v = _heads(op, "k", k, dt, (t, hk, dim)), _heads(op, "v", v, dt, (t, hk, dim))
-    if cos_sin.dim() != 2 or cos_sin.dtype is not torch.float32 or cos_sin.shape[1] % 2 or not 2 <= cos_sin.shape[1] <= dim:
-        raise ConfigError(f"{op}: cos_sin must be fp32 [positions, rot] with an even rot up to {dim}")
+    if k.shape != (t, hk, dim) or v.shape != (t, hk, dim) or k.dtype is not dt or v.dtype is not dt:
+        raise ConfigError(f"{op}: k and v must be [{t}, {hk}, {dim}] of q's type")
+    if cos_sin.dim() != 2 or cos_sin.dtype is not torch.float32:
+        raise ConfigError(f"{op}: cos_sin must be fp32 [positions, rot]")
+    max_pos, rot = cos_sin.shape
+    if rot % 2 or not 2 <= rot <= dim:
+        raise ConfigError(f"{op}: cos_sin's rot must be even and up to {dim}, got {rot}")
     positions, slots = _index(op, "positions", positions, t), _index(op, "slots", slots, t)
-    if cos_sin.stride(1) != 1:
-        cos_sin = cos_sin.contiguous()
+    (k0, k1, kc), (v0, v1, vc), (ld, tc) = k.stride(), v.stride(), cos_sin.stride()
+    if kc != 1 or vc != 1 or tc != 1 or max_pos <= 1:
+        k, v, cos_sin = k.contiguous() if kc != 1 else k, v.contiguous() if vc != 1 else v, cos_sin.contiguous()
+        (k0, k1, _), (v0, v1, _), ld = k.stride(), v.stride(), rot
     if q_out is None:
         q_out = q.new_empty(shape)
     elif q_out.shape != shape or q_out.dtype is not dt or (q_out.stride(2) != 1 and dim > 1):
         raise ConfigError(f"{op}: q_out must be like q, with adjacent columns")
     if t:
-        (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), q_out.stride()
-        _check(_lib.lib().fg_rope_append(
+        (q0, q1, _), (o0, o1, _) = q.stride(), q_out.stride()
+        status = _lib.lib().fg_rope_append(
             q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, q_out.data_ptr(), o0, o1, _CODE[dt],
-            positions.data_ptr(), positions.dtype is torch.int64, cos_sin.data_ptr(), _ld(cos_sin), *cos_sin.shape, interleaved,
-            slots.data_ptr(), slots.dtype is torch.int64, handle, t, h, _lib.stream_of(q)), "fg_rope_append")
+            positions.data_ptr(), positions.dtype is torch.int64, cos_sin.data_ptr(), ld, max_pos, rot, interleaved,
+            slots.data_ptr(), slots.dtype is torch.int64, handle, t, h, _lib.stream_of(q))
+        if status:
+            _check(status, "fg_rope_append")
     _done(op)
     return q_out
 
@@ -256,10 +264,8 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     _on_gpu(q, op)
     handle, cdt, (_, hk, page, dim) = cache._handle()
     _elsewhere(op, q, page_table, seq_lens, prefix_pages, query_start, cache.k, out)
+    q = _queries(op, q, cdt, dim)
     dt = q.dtype
-    if cdt is not dt and cdt is not torch.float8_e4m3fn:
-        raise ConfigError(f"{op}: a {cdt} cache does not take {dt} queries")
-    q = _heads(op, "q", q, dt, (None, None, dim))
     t, h, _ = shape = q.shape
     if h % hk or h == 0:
         raise ConfigError(f"{op}: {h} query heads are no multiple of {hk} key heads")
@@ -288,19 +294,23 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
         raise ConfigError(f"{op}: out must be like q, with adjacent columns")
     lse = q.new_empty((t, h), dtype=torch.float32) if return_lse else None
     if t:
-        if width > 1 and page_table.stride(1) != 1:
-            page_table = page_table.contiguous()
-        seq_lens = seq_lens.contiguous()
+        ld, column = page_table.stride()
+        if column != 1 or b <= 1:
+            page_table, ld = page_table.contiguous(), width
+        if not seq_lens.is_contiguous():
+            seq_lens = seq_lens.contiguous()
         prefix_pages = prefix_pages.contiguous() if prefix_len else None
         query_start = query_start.contiguous() if ragged else None
         need = _attention_workspace(q.get_device(), t, b, h, hk, dim, prefix_len, max_seq_len, max_query_len, ragged, cdt)
         ws = q.new_empty((need,), dtype=torch.uint8) if need else None
         (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
-        _check(_lib.lib().fg_prefix_attention(
-            q.data_ptr(), q0, q1, _CODE[dt], handle, _lib.ptr(prefix_pages), prefix_len, page_table.data_ptr(),
-            _ld(page_table), seq_lens.data_ptr(), _lib.ptr(query_start), t, b, h, max_seq_len, max_query_len,
+        status = _lib.lib().fg_prefix_attention(
+            q.data_ptr(), q0, q1, _CODE[dt], handle, _lib.ptr(prefix_pages), prefix_len, page_table.data_ptr(), ld,
+            seq_lens.data_ptr(), _lib.ptr(query_start), t, b, h, max_seq_len, max_query_len,
             dim ** -0.5 if scale is None else scale, out.data_ptr(), o0, o1, _lib.ptr(lse), _lib.ptr(ws), need,
-            _lib.stream_of(q)), "fg_prefix_attention")
+            _lib.stream_of(q))
+        if status:
+            _check(status, "fg_prefix_attention")
     _done(op)
     return (out, lse) if return_lse else out
 

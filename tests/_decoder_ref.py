@@ -108,7 +108,8 @@ def attention_ref_fast(q, cache, page_table, seq_lens, prefix_pages, prefix_len,
         a, c = starts[b], starts[b + 1]
         if a == c or k.shape[1] == 0:
             continue
-        sees = torch.arange(k.shape[1], device=q.device) < (prefix_len + n - (c - a) + 1 + torch.arange(c - a, device=q.device)).view(-1, 1)
+        own = (n - (c - a) + 1 + torch.arange(c - a, device=q.device)).clamp_min(0)
+        sees = torch.arange(k.shape[1], device=q.device) < (prefix_len + own).view(-1, 1)
         for head in range(h):
             s = (q[a:c, head].double() @ k[head // (h // hk)].t() * scale).masked_fill(~sees, -math.inf)
             z = torch.logsumexp(s, 1)

@@ -68,7 +68,7 @@ def test_cache_refusals(bad, status):
 
 
 def _attention(cache=None, **kw):
-    a = dict(q=P, qt=256, qh=64, dt=_lib.BF16, cache=ctypes.byref(_cache() if cache is None else cache), pp=P, prefix=40,
+    a = dict(q=P, qt=256, qh=64, dt=_lib.BF16, cache=ctypes.byref(_cache() if cache is None else cache), pp=P, prefix=4000,
              table=P, ld=2, lens=P, starts=None, t=3, b=3, heads=4, seq=32, maxq=1, scale=0.1, out=P, ot=256, oh=64, lse=None,
              ws=None, bytes=0, stream=None)
     a.update(kw)
@@ -97,8 +97,9 @@ def test_workspace_follows_the_plan():
     assert ws(0, 4, 8, 2, 64, 100, 100, 1, 1) == 0 and ws(4, 4, 7, 2, 64, 0, 100, 1, 0) == 0
     assert ws(64, 64, 32, 8, 128, 0, 100, 1, 0) == 0  # one part for each sequence: nothing to join
     row = 32 * (128 * 4 + 8)
-    short = ws(1, 1, 32, 8, 128, 100, 100, 1, 0)
-    assert short % row == 0 and short // row >= 2  # a prefix makes two parts at least
+    assert ws(1, 1, 32, 8, 128, 100, 100, 1, 0) == 0  # few keys: one part with the prefix's in it
+    short = ws(1, 1, 32, 8, 128, 400, 100, 1, 0)
+    assert short % row == 0 and short // row >= 2  # a longer prefix makes parts of its own
     assert ws(1, 1, 32, 8, 128, 0, 8192, 1, 0) > short
     assert ws(3, 0, 8, 2, 64, 0, 0, 1, 1) > 0  # tokens of no sequence
 

@@ -72,6 +72,16 @@ def test_prompts_take_the_prefix_along(dt, cdt):
     assert bool((out[-5:] == 0).all()) and bool((lse[-5:] == float("-inf")).all())
 
 
+@pytest.mark.parametrize("h,hk", [(4, 2), (32, 2)])
+def test_queries_in_front_of_their_sequence_see_the_prefix_taken_along(h, hk):
+    """More query tokens than cached ones: the first stand before the sequence and see the whole prefix, no less."""
+    for prefix in (20, 300):
+        call, ref = _call([40, 33, 35], [2, 0, 34], prefix, h, hk, 64)
+        call2, ref2 = _call([3, 2], [1, 0], prefix, 4, 4, 64)
+        assert_attention(*ops.prefix_attention(**call), ref, BF)
+        assert_attention(*ops.prefix_attention(**call2), ref2, BF)
+
+
 def test_prompts_take_the_prefix_along_in_parts():
     _check("attn_tile_kernel parts=0+", [300], [350], 2500, 4, 1, 128, gain=4.0)
     assert "join" in _lib.last_kernel()
