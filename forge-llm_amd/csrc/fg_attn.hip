@@ -11,12 +11,14 @@
 
 namespace fg {
 
-// Joins the parts of each row: one wavefront per (query token, query head); L lanes hold a row of D columns, four each, and
-// 64 / L parts are read at a time.
-template <bool BF16, int L>
+// Joins the parts of each row, (query token, query head): L lanes hold a row of D columns, four each, so that a wavefront reads
+// 64 / L parts at a time; W wavefronts share a row of many parts (33 parts of 256 rows: XJ1 us with one, XJ4 with four).
+template <bool BF16, int L, int W>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), all = (int64_t)a.T * a.Hq;
-  const int lane = threadIdx.x & 63, col = 4 * (lane % L), first = lane / L;
+  __shared__ f32x4 part_o[W > 1 ? W : 1][L];
+  __shared__ float part_sum[W];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = 4 * (lane % L), first = lane / L + (W > 1 ? wave * (64 / L) : 0);
+  const int64_t id = (int64_t)blockIdx.x * (4 / W) + (W > 1 ? 0 : wave), all = (int64_t)a.T * a.Hq;
   if (id >= all) return;
   const int t = (int)(id / a.Hq), h = (int)(id - (int64_t)t * a.Hq);
   int seq = t;
@@ -41,7 +43,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
   float sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = first; i < n; i += 64 / L) {
+  for (int i = first; i < n; i += W * 64 / L) {
     const float2 p = a.ml[i * all + id];
     const f32x4 v = col < a.D ? *reinterpret_cast<const f32x4*>(a.acc + (i * all + id) * a.D + col) : o;
     const float f = __builtin_amdgcn_exp2f(p.x - base);
@@ -55,9 +57,20 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], off, kWave);
   }
+  if constexpr (W > 1) {
+    if (lane < L) part_o[wave][lane] = o;
+    if (lane == 0) part_sum[wave] = sum;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      sum += part_sum[w];
+      o += part_o[w][lane % L];
+    }
+  }
   // a row that saw no key gives zeros; one past max_query_len, which no item computed, shows as NaN
   const float f = !served ? __builtin_nanf("") : (sum == 0.f ? 0.f : 1.f / sum);
-  if (first == 0 && col < a.D) {
+  if (lane < L && col < a.D) {
     const uint2 w = make_uint2(pack2<BF16>(o[0] * f, o[1] * f), pack2<BF16>(o[2] * f, o[3] * f));
     __builtin_memcpy(__builtin_assume_aligned(a.out + t * a.o_t + h * a.o_h + col, 2), &w, 8);
   }
@@ -74,13 +87,14 @@ static int split_keys(int64_t len, int64_t items, int64_t want, int64_t unit, in
   return (int)std::max<int64_t>(1, (len + p - 1) / p);
 }
 
-// `want`: workgroups per CU.  Up to kOnePart keys are one part of attn_rows, which needs no second launch (250 keys: 8.7 us
-// against 9.4 in two parts; 500: 12.1 against 9.5).
+// `want`: workgroups per CU; `alone`: no other segment's parts are joined to these.  Then up to kOnePart keys are one part of
+// attn_rows, which needs no second launch (250 keys: 8.7 us against 9.4 in two parts; 500: 12.1 against 9.5).
 constexpr int kOnePart = 256;
-static int64_t plan_segment(int64_t len, int64_t rows, int64_t sets, bool tile, int want, int* tiles, int* parts, int* part) {
+static int64_t plan_segment(int64_t len, int64_t rows, int64_t sets, bool tile, bool alone, int want, int* tiles, int* parts,
+                            int* part) {
   const int64_t per = tile ? kTileRows : 16, n = (rows + per - 1) / per;
   *tiles = (int)n;
-  if (!tile && len <= kOnePart) {
+  if (!tile && alone && len <= kOnePart) {
     *part = (int)std::max<int64_t>(len, 1);
     *parts = 1;
     return attn_count(sets, n);
@@ -115,10 +129,10 @@ size_t attn_plan(AttnArgs& a) {
   a.parts_p = a.tiles_p = a.part_p = 0;
   int64_t items_p = 0;
   if (a.prefix_len && !a.joined)
-    items_p = plan_segment(a.prefix_len, rows_p, a.Hk, a.tile_p, a.tile_p && (a.tile_s || a.lead) ? 2 : 1, &a.tiles_p, &a.parts_p,
+    items_p = plan_segment(a.prefix_len, rows_p, a.Hk, a.tile_p, false, a.tile_p && (a.tile_s || a.lead) ? 2 : 1, &a.tiles_p, &a.parts_p,
                            &a.part_p);
   const int64_t items = items_p + plan_segment((a.joined ? (int64_t)a.prefix_len : 0) + a.max_len, rows_s, (int64_t)a.Hk * a.B,
-                                               a.tile_s, a.tile_s ? 2 : (a.tile_p && items_p ? 4 : 1), &a.tiles_s, &a.parts_s, &a.part_s);
+                                               a.tile_s, !items_p, a.tile_s ? 2 : (a.tile_p && items_p ? 4 : 1), &a.tiles_s, &a.parts_s, &a.part_s);
   a.items_p = (int)items_p;
   a.items = items < (1LL << 24) - 64 ? (int)items : -1;
   if (a.parts_p + a.parts_s == 1 && a.B > 0) return 0;  // nothing to join
@@ -146,15 +160,21 @@ hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, hipStream_t s
   }
   note_kernel("%s parts=%d+%d%s", names[kind], a.parts_p, a.parts_s, bytes ? " + attn_join_kernel" : "");
   if (!bytes) return hipSuccess;
-  auto join = [&](auto b_tag) {
+  const int many = a.parts_p + a.parts_s >= 8 ? 4 : 1;  // wavefronts per row
+  auto join = [&](auto b_tag, auto l_tag) {
     constexpr bool B = decltype(b_tag)::value;
-    const dim3 grid((unsigned)(((int64_t)a.T * a.Hq + 3) / 4));
-    if (a.D <= 64) hipLaunchKernelGGL((attn_join_kernel<B, 16>), grid, dim3(256), 0, st, a);
-    else if (a.D <= 128) hipLaunchKernelGGL((attn_join_kernel<B, 32>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((attn_join_kernel<B, 64>), grid, dim3(256), 0, st, a);
+    constexpr int L = decltype(l_tag)::value;
+    const dim3 grid((unsigned)(((int64_t)a.T * a.Hq * many + 3) / 4));
+    if (many == 1) hipLaunchKernelGGL((attn_join_kernel<B, L, 1>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attn_join_kernel<B, L, 4>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
   };
-  return bf16 ? join(std::true_type{}) : join(std::false_type{});
+  auto by_d = [&](auto b_tag) {
+    if (a.D <= 64) return join(b_tag, std::integral_constant<int, 16>{});
+    if (a.D <= 128) return join(b_tag, std::integral_constant<int, 32>{});
+    return join(b_tag, std::integral_constant<int, 64>{});
+  };
+  return bf16 ? by_d(std::true_type{}) : by_d(std::false_type{});
 }
 
 }  // namespace fg

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .errors import ConfigError
-from .ops_gemm import _as_rows, _check, _code_or_zero, _done, _ld, _on_gpu
+from .ops_gemm import _as_rows, _check, _done, _ld, _on_gpu
 
 _16BIT = (torch.float16, torch.bfloat16)
 _FLOATS = (torch.float32, *_16BIT)
@@ -38,6 +38,16 @@ def _elsewhere(op: str, x: torch.Tensor, *tensors: torch.Tensor | None) -> None:
 
 
 # ================================================================================================ norm
+def _rows(t: torch.Tensor, k: int) -> tuple[torch.Tensor, int]:
+    """``t [..., k]`` as rows of adjacent columns that do not overlap (copied only if they are not), and their stride."""
+    if t.dim() == 2:
+        ld, column = t.stride()
+        if column == 1 and ld >= k:
+            return t, ld
+    t = _as_rows(t)
+    return t, _ld(t)
+
+
 class NormOutput(NamedTuple):
     y: torch.Tensor
     scale: torch.Tensor | None
@@ -70,22 +80,24 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Te
     if weight is not None:
         if weight.shape != (k,) or weight.dtype not in _FLOATS:
             raise ConfigError(f"add_rmsnorm: weight must be an fp32, fp16 or bf16 tensor of [{k}]")
-        weight = weight.contiguous()
-    x2 = _as_rows(x)
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+    x2, ldx = _rows(x, k)
     m = x2.shape[0]
-    r2 = ro2 = None
+    r2 = ro2 = rdt = None
+    ldr = ldro = 0
     if residual is not None:
         rdt = residual.dtype
         if residual.shape != shape or (rdt is not xdt and rdt is not torch.float32):
             raise ConfigError("add_rmsnorm: residual must have x's shape and x's type or fp32")
-        r2 = _as_rows(residual)
+        r2, ldr = _rows(residual, k)
         if residual_out is None:
-            residual_out = residual.new_empty(shape)
-            ro2 = residual_out if x2 is x else residual_out.view(m, k)
+            residual_out, ldro = residual.new_empty(shape), k
+            ro2 = residual_out  # contiguous: the address and k say all
         elif residual_out.shape != shape or residual_out.dtype is not rdt:
             raise ConfigError("add_rmsnorm: residual_out must be like residual")
         else:
-            ro2 = _as_rows(residual_out)
+            ro2, ldro = _rows(residual_out, k)
             if m and ro2.data_ptr() != residual_out.data_ptr():
                 raise ConfigError("add_rmsnorm: residual_out must be rows of adjacent columns that do not overlap")
     elif residual_out is not None:
@@ -101,11 +113,12 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Te
     elif quant is not None:
         scale, s_row = x.new_empty((m,), dtype=torch.float32), 1
     if m and k:
-        _check(_lib.lib().fg_add_rmsnorm(
-            x2.data_ptr(), _ld(x2), _CODE[xdt], _lib.ptr(r2), 0 if r2 is None else _ld(r2), _lib.ptr(ro2),
-            0 if ro2 is None else _ld(ro2), _code_or_zero(r2), _lib.ptr(weight), _code_or_zero(weight), eps, y.data_ptr(),
-            k, _CODE[ydt], _lib.ptr(scale), s_row, s_block, block if quant == "fp8_block" else 0, m, k,
-            _lib.stream_of(x2)), "fg_add_rmsnorm")
+        status = _lib.lib().fg_add_rmsnorm(
+            x2.data_ptr(), ldx, _CODE[xdt], _lib.ptr(r2), ldr, _lib.ptr(ro2), ldro, 0 if rdt is None else _CODE[rdt],
+            _lib.ptr(weight), 0 if weight is None else _CODE[weight.dtype], eps, y.data_ptr(), k, _CODE[ydt], _lib.ptr(scale),
+            s_row, s_block, block if quant == "fp8_block" else 0, m, k, _lib.stream_of(x2))
+        if status:
+            _check(status, "fg_add_rmsnorm")
     _done("add_rmsnorm")
     return NormOutput(y if x2 is x else y.view(shape), scale, x if residual is None else residual_out)
 
