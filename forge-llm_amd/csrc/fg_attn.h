@@ -37,7 +37,7 @@ struct AttnArgs {
 };
 
 size_t attn_plan(AttnArgs& a);
-hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, hipStream_t st);
+hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, size_t bytes, hipStream_t st);
 
 constexpr uint32_t kNoRow = 0xffffffffu;  // an entry of the row table that stands for no key
 constexpr int kMaxPart = 2048;            // attn_rows: tokens per part, entries of its row table

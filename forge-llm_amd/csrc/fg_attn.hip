@@ -12,7 +12,7 @@
 namespace fg {
 
 // Joins the parts of each row, (query token, query head): L lanes hold a row of D columns, four each, so that a wavefront reads
-// 64 / L parts at a time; W wavefronts share a row of many parts (33 parts of 256 rows: XJ1 us with one, XJ4 with four).
+// 64 / L parts at a time; W wavefronts share a row of many parts (33 parts of 256 rows: 12.8 us with one, 6.1 with four).
 template <bool BF16, int L, int W>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
   __shared__ f32x4 part_o[W > 1 ? W : 1][L];
@@ -78,39 +78,56 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
     a.lse[id] = !served ? f : (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
 }
 
-// Cuts the keys of `items` row tiles into parts, a workgroup each: about `want` of them in all, whole multiples of `unit` keys
-// and at most `most`.  Host lengths only: a sequence shorter than max_len leaves parts that end at once.
-static int split_keys(int64_t len, int64_t items, int64_t want, int64_t unit, int64_t most, int* part) {
-  const int64_t parts = std::max<int64_t>(1, want / std::max<int64_t>(items, 1));
-  const int64_t p = std::min(most, std::max<int64_t>(unit, ((len + parts - 1) / parts + unit - 1) / unit * unit));
+// Parts of whole tiles of `unit` keys for `items` row tiles and key heads, a workgroup each.  Host lengths only: a sequence
+// shorter than max_len leaves parts that end at once.
+static int cut(int64_t len, int64_t parts, int64_t unit, int* part) {
+  const int64_t p = std::max<int64_t>(unit, ((len + parts - 1) / parts + unit - 1) / unit * unit);
   *part = (int)p;
   return (int)std::max<int64_t>(1, (len + p - 1) / p);
 }
 
-// `want`: workgroups per CU; `alone`: no other segment's parts are joined to these.  Then up to kOnePart keys are one part of
-// attn_rows, which needs no second launch (250 keys: 8.7 us against 9.4 in two parts; 500: 12.1 against 9.5).
+// attn_rows: about `want` workgroups per CU (one; four among a prefix's items of many rows, where the sequences' lengths
+// should even out), parts as long as the row table at most.  Where nothing is joined to them (`alone`), up to kOnePart keys are
+// one part, which needs no second launch (250 keys: 8.7 us against 9.4 in two parts; 500: 12.1 against 9.5).
 constexpr int kOnePart = 256;
-static int64_t plan_segment(int64_t len, int64_t rows, int64_t sets, bool tile, bool alone, int want, int* tiles, int* parts,
-                            int* part) {
-  const int64_t per = tile ? kTileRows : 16, n = (rows + per - 1) / per;
-  *tiles = (int)n;
-  if (!tile && alone && len <= kOnePart) {
-    *part = (int)std::max<int64_t>(len, 1);
-    *parts = 1;
-    return attn_count(sets, n);
-  }
-  *parts = split_keys(len, n * sets, (int64_t)want * device_cus(), tile ? 64 : kRowsTile * kRowsWaves, tile ? 1 << 30 : kMaxPart, part);
-  return attn_count(*parts * sets, n);
+static int cut_rows(int64_t len, int64_t items, bool alone, int64_t want, int* part) {
+  if (alone && len <= kOnePart) return cut(len, 1, kOnePart, part);
+  const int64_t parts = std::max<int64_t>(want * device_cus() / std::max<int64_t>(items, 1), (len + kMaxPart - 1) / kMaxPart);
+  return cut(len, std::max<int64_t>(parts, 1), kRowsTile * kRowsWaves, part);
 }
 
-// Fills in the plan; returns the partial sums' bytes.  items is -1 where the threads of a launch would pass 32 bits.  More than 16 rows
-// go to the kernel of many rows, which waits for nothing but memory even where most of its 128 rows are empty.
+// attn_tile: the number of parts with the least time in us, where a tile of 64 keys takes 1.6 alone on a CU and 1.2 by each
+// workgroup there beside others, and a part's sums (`sums` values in all) are written and read back at 4 TB/s, with 4 for the
+// second launch where one part would need none.  (Graph replays, us, by parts of the prefix: 64 sequences behind 8192 tokens 8 /
+// 16 / 32: 68 / 60 / 64; 16 sequences 16 / 64: 20.8 / 23.6; 256 behind 32768 2 / 4 / 8: 400 / 350 / 370.)
+static int cut_tile(int64_t len, int64_t items, int64_t sums, bool alone, int* part) {
+  const int64_t tiles = std::max<int64_t>((len + 63) / 64, 1), cus = device_cus();
+  const int64_t most = std::min(tiles, std::max<int64_t>(1, 4 * cus / std::max<int64_t>(items, 1)));
+  double best = 0;
+  int64_t parts = 1;
+  for (int64_t p = 1; p <= most; p += std::max<int64_t>(1, p / 8)) {
+    const int64_t per_cu = (items * p + cus - 1) / cus, each = (tiles + p - 1) / p;
+    const double t = each * (per_cu <= 1 ? 1.6 : 1.2 * per_cu) + (p == 1 && alone ? 0 : 4 + p * (double)sums * 8 / 4e6);
+    if (p == 1 || t < best) {
+      best = t;
+      parts = p;
+    }
+  }
+  return cut(len, parts, 64, part);
+}
+
+// Fills in the plan; returns the partial sums' bytes.  items is -1 where the threads of a launch would pass 32 bits.  Rows past
+// 16 go to attn_tile, which is ahead even where most of its 128 rows are empty (16 sequences of 2000 tokens with 8 queries of 4
+// heads: 23.2 us against 35.6 in two row tiles), but for 17 to 32 rows of a prefix in e4m3, which attn_rows converts as it
+// computes and attn_tile in front of that (8 sequences of one query behind 8192 tokens: 15.4 us against 19.1; 16-bit 18.1
+// against 16.2).
 size_t attn_plan(AttnArgs& a) {
   const int64_t rows_p = (int64_t)a.T * a.G, rows_s = (int64_t)a.max_q * a.G;
   a.tile_s = rows_s > 16;
-  a.tile_p = a.tile_s || rows_p > 16;
+  a.tile_p = a.tile_s || rows_p > (a.item == 1 ? 32 : 16);
   // Sequences that fill two row tiles each on average take the prefix along with their own keys: the rows that packing the
-  // whole batch's into tiles would save cost less than the parts' sums (4 prompts of 500 tokens x 4 heads: XX us, YY apart).
+  // whole batch's into tiles would save cost less than the parts' sums (4 prompts of up to 500 tokens,
+  // 32 + 2 x 8 heads, behind 4000: 139 us, 159 apart).
   a.joined = a.tile_s && a.prefix_len && rows_p >= 2 * kTileRows * (int64_t)a.B;
   if (!a.tile_s && a.prefix_len) {
     // So do single queries where all keys make one part, or where the sequences fill the CUs by themselves and reading the
@@ -120,19 +137,25 @@ size_t attn_plan(AttnArgs& a) {
     const double again = (double)a.B * a.prefix_len * a.Hk * a.D * 2 * a.item / 8e6, sums = 4 + 2.0 * a.T * a.Hq * a.D * 8 / 4e6;
     a.joined = a.prefix_len + a.max_len <= kOnePart || ((int64_t)a.B * a.Hk >= device_cus() && again < sums);
   }
-  // The prefix's items go first where their products (1.2 us per tile of 64 keys, two at a time on a CU) outlast the reads of
-  // the sequences' keys at 4 TB/s, and make two workgroups per CU.  Else they spread among the sequences' items, and one per
-  // CU leaves fewer sums to join (64 sequences behind 8192 tokens: 59 us against 64 with two; 256 behind 32768, which go
-  // first: 350 against 400 with one).
-  const double products = (double)((rows_p + kTileRows - 1) / kTileRows) * a.Hk * ((a.prefix_len + 63) / 64) * 1.2 / device_cus();
+  // The prefix's items go first where their products (1.2 us per tile of 64 keys) outlast the reads of the sequences' keys at
+  // 4 TB/s (256 sequences behind 32768 tokens: 350 us, 450 spread); else they spread among the sequences' items (64 behind 8192:
+  // 61 us, 68 first).
+  const int64_t per_p = a.tile_p ? kTileRows : 16, per_s = a.tile_s ? kTileRows : 16, sums = (int64_t)a.T * a.Hq * a.D;
+  a.tiles_p = (int)((rows_p + per_p - 1) / per_p);
+  a.tiles_s = (int)((rows_s + per_s - 1) / per_s);
+  const double products = (double)a.tiles_p * a.Hk * ((a.prefix_len + 63) / 64) * 1.2 / device_cus();
   a.lead = products > (double)a.B * a.max_len * a.Hk * a.D * 2 * a.item / 4e6;
-  a.parts_p = a.tiles_p = a.part_p = 0;
-  int64_t items_p = 0;
-  if (a.prefix_len && !a.joined)
-    items_p = plan_segment(a.prefix_len, rows_p, a.Hk, a.tile_p, false, a.tile_p && (a.tile_s || a.lead) ? 2 : 1, &a.tiles_p, &a.parts_p,
-                           &a.part_p);
-  const int64_t items = items_p + plan_segment((a.joined ? (int64_t)a.prefix_len : 0) + a.max_len, rows_s, (int64_t)a.Hk * a.B,
-                                               a.tile_s, !items_p, a.tile_s ? 2 : (a.tile_p && items_p ? 4 : 1), &a.tiles_s, &a.parts_s, &a.part_s);
+  const bool apart = a.prefix_len && !a.joined;
+  const int64_t sets = (int64_t)a.Hk * a.B, own = (a.joined ? (int64_t)a.prefix_len : 0) + a.max_len;
+  a.parts_p = a.part_p = 0;
+  if (apart) {
+    const int64_t n = (int64_t)a.tiles_p * a.Hk;
+    a.parts_p = a.tile_p ? cut_tile(a.prefix_len, n, sums, false, &a.part_p) : cut_rows(a.prefix_len, n, false, 1, &a.part_p);
+  }
+  a.parts_s = a.tile_s ? cut_tile(own, a.tiles_s * sets, sums, !apart, &a.part_s)
+                       : cut_rows(own, a.tiles_s * sets, !apart, apart && a.tile_p ? 4 : 1, &a.part_s);
+  const int64_t items_p = apart ? attn_count((int64_t)a.parts_p * a.Hk, a.tiles_p) : 0;
+  const int64_t items = items_p + attn_count(a.parts_s * sets, a.tiles_s);
   a.items_p = (int)items_p;
   a.items = items < (1LL << 24) - 64 ? (int)items : -1;
   if (a.parts_p + a.parts_s == 1 && a.B > 0) return 0;  // nothing to join
@@ -142,9 +165,8 @@ size_t attn_plan(AttnArgs& a) {
 hipError_t launch_attn_bf16(const AttnArgs& a, bool fp8, int kind, hipStream_t st);
 hipError_t launch_attn_fp16(const AttnArgs& a, bool fp8, int kind, hipStream_t st);
 
-hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, hipStream_t st) {
-  const size_t bytes = attn_plan(a);
-  if (a.items < 0) return hipErrorInvalidValue;
+// A planned call; `bytes`: what attn_plan returned for it.
+hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, size_t bytes, hipStream_t st) {
   a.acc = nullptr;
   a.ml = nullptr;
   if (bytes) {

@@ -1284,9 +1284,10 @@ int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtyp
   if (B > 0 && ld_pages * cache->page_size < max_seq_len)
     return fail(FG_EINVAL, "fg_prefix_attention: max_seq_len is past the page table's columns");
   const size_t need = fg::attn_plan(a);
+  if (a.items < 0) return fail(FG_EINVAL, "fg_prefix_attention: more work items than a launch takes");
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(FG_EINVAL, "fg_prefix_attention: the workspace needs %zu bytes, 16-byte aligned", need);
-  const int64_t item = item_bytes(cache->dtype);
+  const int64_t item = a.item;
   a.q = static_cast<const uint16_t*>(q); a.q_t = q_token; a.q_h = q_head;
   a.out = static_cast<uint16_t*>(out); a.o_t = o_token; a.o_h = o_head; a.lse = lse;
   a.k = static_cast<const uint8_t*>(cache->k); a.v = static_cast<const uint8_t*>(cache->v);
@@ -1297,7 +1298,7 @@ int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtyp
   a.page = cache->page_size; a.n_pages = (int)cache->num_pages;
   // a scale of zero would make the masked scores 0 * -inf; the smallest normal number gives the same equal weights
   a.scale_log2 = (scale == 0.f ? 1.17549435e-38f : scale) * 1.4426950408889634f;
-  return hip_status(fg::launch_attn(a, dtype == FG_BF16, cache->dtype == FG_E4M3, workspace,
+  return hip_status(fg::launch_attn(a, dtype == FG_BF16, cache->dtype == FG_E4M3, workspace, need,
                                     static_cast<hipStream_t>(stream)),
                     "fg_prefix_attention launch");
 }
