@@ -1,4 +1,5 @@
-// attn_rows: work items of up to 16 rows (decoding).  What bounds them is the read of the keys and values, so each wavefront
+// attn_rows: work items of up to 16 rows (decoding).  What bounds them is the read of the keys and values (256 sequences of 256
+// to 2048 tokens, 8 key heads of 128 in bf16: 225 us, 5.4 TB/s; a workgroup by itself reads about 34 bytes per ns), so each wavefront
 // works by itself on tiles of 32 keys, without a barrier, with the loads of the next tile and the one after on their way.
 //   S^T = K Q^T   (A: 16 keys x 32 columns straight from global memory, 16 bytes per lane; B: the rows, in registers)
 //   O^T += V^T P^T

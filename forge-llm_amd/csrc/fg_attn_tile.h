@@ -9,8 +9,9 @@
 // Bound by the matrix products and, beside them, by the exponentials: per 64 keys and wavefront 32 products (1024 cycles) and
 // 128 other vector instructions, 32 of them exponentials.  A fragment is read from LDS two steps before its product, the
 // exponentials of 16 keys stand between the products of the 16 before, and two workgroups per CU fill each other's waits.
-// Measured on 2048 rows x 8 key heads x 32768 keys of 128 columns: 290 us, 950 TFLOP/s; 64 rows per wavefront, which would
-// halve the LDS reads, needs more than 256 registers and spends what it gains on moves to and from the accumulation file.
+// Measured on 2048 rows x 8 key heads x 32768 keys of 128 columns: about 265 us, 1.0 PFLOP/s (a large library product: 1.2).  64
+// rows per wavefront, which would halve the LDS reads, needs more than 256 registers and spends what it gains on moves to and
+// from the accumulation registers; through registers instead of straight to LDS a tile costs 10% more.
 #pragma once
 
 #include "fg_attn.h"
