@@ -130,7 +130,7 @@ __device__ __forceinline__ bool attn_item(const AttnArgs& a, int id, AttnItem& i
   it.head = pair - rest * a.Hk;
   if (a.starts && !a.acc && tile == 0 && part == 0) attn_uncovered(a, seq, it.head);
   if (a.joined) it.front = a.prefix_len;
-  const int len = it.front + min(a.lens[seq], a.max_len);
+  const int len = it.front + max(min(a.lens[seq], a.max_len), 0);
   it.row0 = tile * TILE;
   it.rows = min(n, a.max_q) * a.G;
   it.token0 = t0;

@@ -107,6 +107,13 @@ def test_one_part_with_tokens_of_no_sequence_and_past_the_longest():
     assert torch.equal(got[served], out[served]) and bool(got[~served].isnan().all()) and bool(got_lse[~served].isnan().all())
 
 
+@pytest.mark.parametrize("prefix,lens", [(0, [20, 0, 31]), (100, [20, 0, 31]), (1000, [20, 0, 31]), (9000, [700, 0, 900])])
+def test_negative_lengths_are_no_tokens(prefix, lens):
+    call, ref = _call([1, 1, 1], lens, prefix, 4, 2, 64)
+    call["seq_lens"][1] = -40
+    assert_attention(*ops.prefix_attention(**call), ref, BF)
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30])
 def test_scales_that_are_not_positive(scale):
     for queries, lens, prefix, h in (([1, 1], [40, 300], 70, 4), ([70, 30], [100, 300], 90, 8)):
