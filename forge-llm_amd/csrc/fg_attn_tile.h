@@ -255,7 +255,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int id, uint8_t* ld
         }
       }
     }
-    if (i + 1 < tiles) store(nxt);
+    if (DIRECT || i + 1 < tiles) store(nxt);  // DIRECT: its wait stands on every path to the barrier
   };
   for (int i = 0; i < tiles; i += 2) {  // the buffers' places are constants of the reads' addresses
     step(i, lds, lds + 2 * kBuf);
