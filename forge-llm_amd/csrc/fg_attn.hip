@@ -116,6 +116,9 @@ static int cut_tile(int64_t len, int64_t items, int64_t sums, bool alone, int* p
   return cut(len, parts, 64, part);
 }
 
+// Wavefronts that join a row.
+static int join_waves(const AttnArgs& a) { return a.parts_p + a.parts_s >= 8 ? 4 : 1; }
+
 // Fills in the plan; returns the partial sums' bytes.  items is -1 where the threads of a launch would pass 32 bits.  Rows past
 // 16 go to attn_tile, which is ahead even where most of its 128 rows are empty (16 sequences of 2000 tokens with 8 queries of 4
 // heads: 23.2 us against 35.6 in two row tiles), but for 17 to 32 rows of a prefix in e4m3, which attn_rows converts as it
@@ -159,6 +162,7 @@ size_t attn_plan(AttnArgs& a) {
   a.items_p = (int)items_p;
   a.items = items < (1LL << 24) - 64 ? (int)items : -1;
   if (a.parts_p + a.parts_s == 1 && a.B > 0) return 0;  // nothing to join
+  if ((int64_t)a.T * a.Hq * join_waves(a) >= 1LL << 26) a.items = -1;
   return (size_t)(a.parts_p + a.parts_s) * a.T * a.Hq * ((size_t)a.D * 4 + sizeof(float2));
 }
 
@@ -182,7 +186,7 @@ hipError_t launch_attn(AttnArgs& a, bool bf16, bool fp8, void* ws, size_t bytes,
   }
   note_kernel("%s parts=%d+%d%s", names[kind], a.parts_p, a.parts_s, bytes ? " + attn_join_kernel" : "");
   if (!bytes) return hipSuccess;
-  const int many = a.parts_p + a.parts_s >= 8 ? 4 : 1;  // wavefronts per row
+  const int many = join_waves(a);
   auto join = [&](auto b_tag, auto l_tag) {
     constexpr bool B = decltype(b_tag)::value;
     constexpr int L = decltype(l_tag)::value;

@@ -1284,7 +1284,7 @@ int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtyp
   if (B > 0 && ld_pages * cache->page_size < max_seq_len)
     return fail(FG_EINVAL, "fg_prefix_attention: max_seq_len is past the page table's columns");
   const size_t need = fg::attn_plan(a);
-  if (a.items < 0) return fail(FG_EINVAL, "fg_prefix_attention: more work items than a launch takes");
+  if (a.items < 0) return fail(FG_EINVAL, "fg_prefix_attention: more work items or rows than a launch takes");
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(FG_EINVAL, "fg_prefix_attention: the workspace needs %zu bytes, 16-byte aligned", need);
   const int64_t item = a.item;

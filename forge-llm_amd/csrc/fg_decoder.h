@@ -7,6 +7,9 @@ namespace fg {
 
 constexpr int kNormMaxK = 32768;  // four units for each of 1024 threads
 
+// A launch has fewer than 2^32 threads.
+inline bool launchable(int64_t blocks, int threads) { return blocks * threads < (1LL << 32); }
+
 struct NormArgs {
   const void* x;
   int64_t ldx;

@@ -157,6 +157,7 @@ hipError_t launch_rope_append(const RopeAppendArgs& a, int64_t T, bool bf16, boo
   const int turns = (H * items + kRopeThreads - 1) / kRopeThreads, rows = std::max(1, std::min((H + turns - 1) / turns, kRopeThreads / items));
   const unsigned threads = (unsigned)(items * rows + 63) / 64 * 64;
   const unsigned gy = T <= 2 * device_cus() ? (unsigned)((H + rows - 1) / rows) : 1u;
+  if (!launchable(T * gy, (int)threads)) return hipErrorInvalidConfiguration;
   auto go = [&](auto b_tag, auto f_tag, auto i_tag, auto v_tag) {
     note_kernel("rope_append_kernel<V=%d> heads/%u", V, gy);
     hipLaunchKernelGGL((rope_append_kernel<decltype(b_tag)::value, decltype(f_tag)::value, decltype(i_tag)::value,

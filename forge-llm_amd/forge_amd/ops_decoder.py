@@ -182,6 +182,11 @@ class PagedKVCache:
         return got[1]
 
 
+def _overlaps(token: int, head: int, t: int, h: int, dim: int) -> bool:
+    """Whether rows of ``dim`` columns at these strides (one expanded from fewer, say) share elements."""
+    return (t > 1 and token < dim) or (h > 1 and head < dim)
+
+
 def _index(op: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
     if t.shape != (n,) or (t.dtype is not torch.int64 and t.dtype is not torch.int32):
         raise ConfigError(f"{op}: {name} must be an int32 or int64 tensor of [{n}]")
@@ -239,6 +244,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
         raise ConfigError(f"{op}: q_out must be like q, with adjacent columns")
     if t:
         (q0, q1, _), (o0, o1, _) = q.stride(), q_out.stride()
+        if _overlaps(o0, o1, t, h, dim):
+            raise ConfigError(f"{op}: q_out's rows overlap")
         status = _lib.lib().fg_rope_append(
             q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, q_out.data_ptr(), o0, o1, _CODE[dt],
             positions.data_ptr(), positions.dtype is torch.int64, cos_sin.data_ptr(), ld, max_pos, rot, interleaved,
@@ -307,6 +314,9 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
         raise ConfigError(f"{op}: out must be like q, with adjacent columns")
     lse = q.new_empty((t, h), dtype=torch.float32) if return_lse else None
     if t:
+        (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
+        if _overlaps(o0, o1, t, h, dim):
+            raise ConfigError(f"{op}: out's rows overlap")
         ld, column = page_table.stride()
         if column != 1 or b <= 1:
             page_table, ld = page_table.contiguous(), width
@@ -316,7 +326,6 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
         query_start = query_start.contiguous() if ragged else None
         need = _attention_workspace(q.get_device(), t, b, h, hk, dim, prefix_len, max_seq_len, max_query_len, ragged, cdt)
         ws = q.new_empty((need,), dtype=torch.uint8) if need else None
-        (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
         status = _lib.lib().fg_prefix_attention(
             q.data_ptr(), q0, q1, _CODE[dt], handle, _lib.ptr(prefix_pages), prefix_len, page_table.data_ptr(), ld,
             seq_lens.data_ptr(), _lib.ptr(query_start), t, b, h, max_seq_len, max_query_len,

@@ -131,3 +131,18 @@ def test_no_cpu_path(monkeypatch):
     monkeypatch.setenv("FORGE_FORCE_REF", "1")
     with pytest.raises(HardwareUnsupported, match="FORGE_FORCE_REF"):
         ops.add_rmsnorm(x, None)
+
+
+def test_more_threads_than_a_launch_takes():
+    for status in (_norm(m=2 ** 26), _append(t=2 ** 26), _append(t=2 ** 31 - 1, heads=1)):
+        assert status == _lib.EHIP and "configuration" in _lib.last_error()
+    assert _attention(t=2 ** 24, b=2 ** 24) == _lib.EINVAL and "more work items" in _lib.last_error()
+    # 2^26 rows to join in 2^20 work items
+    assert _attention(t=2 ** 24, b=2 ** 18, starts=P, maxq=64) == _lib.EINVAL and "more work items" in _lib.last_error()
+    assert _attention(t=2 ** 24 - 1, b=2 ** 18, starts=P, maxq=64) == _lib.EINVAL and "workspace" in _lib.last_error()
+
+
+@pytest.mark.parametrize("token,head,t,h,bad", [(256, 64, 3, 4, False), (64, 192, 3, 4, False), (0, 64, 3, 4, True), (256, 0, 3, 4, True),
+                                                (0, 64, 1, 4, False), (256, 32, 3, 4, True), (256, 0, 3, 1, False)])
+def test_rows_that_overlap(token, head, t, h, bad):
+    assert ops._overlaps(token, head, t, h, 64) is bad

@@ -158,3 +158,14 @@ def test_no_tokens_and_refusals():
     odd = torch.zeros(2, 2, 4, 68, dtype=BF, device=DEV)[..., :64]
     with pytest.raises(Exception, match="16-byte"):
         ops.rope_append(**{**call, "cache": ops.PagedKVCache(odd, odd)})
+
+
+def test_outputs_whose_rows_overlap_are_refused():
+    cache = ops.PagedKVCache.allocate(2, 2, 4, 64, BF, DEV)
+    q, k = torch.zeros(3, 4, 64, dtype=BF, device=DEV), torch.zeros(3, 2, 64, dtype=BF, device=DEV)
+    i, table = torch.arange(3, device=DEV), _table(4, 64).to(DEV)
+    for out in (q[:1].expand(3, 4, 64), q[:, :1].expand(3, 4, 64)):
+        with pytest.raises(ConfigError, match="overlap"):
+            ops.rope_append(q, k, k, i, table, cache, i, q_out=out)
+        with pytest.raises(ConfigError, match="overlap"):
+            ops.prefix_attention(q, cache, torch.zeros(3, 1, dtype=torch.int32, device=DEV), i.int(), out=out)
