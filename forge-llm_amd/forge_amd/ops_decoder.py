@@ -169,17 +169,24 @@ class PagedKVCache:
     def page_size(self) -> int:
         return self.k.shape[2]
 
-    def _handle(self) -> tuple[int, torch.dtype, tuple[int, ...]]:
-        """Address of the C description (made on first use, and again if a tensor's memory has moved), type and shape."""
-        got = self.__dict__.get("_made")
+    def _handle(self) -> tuple[object, torch.dtype, tuple[int, ...]]:
+        """The C description (made on first use, and again where a tensor's memory, shape or order has changed), type and
+        shape (``v`` has ``k``'s: of the two, ``k``'s are compared).  The description comes as the reference that the C call
+        takes, which keeps it alive: another thread may make it again during the call."""
         k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
-        if got is None or got[0].k != k.data_ptr() or got[0].v != v.data_ptr() or (
-                ks is not None and (got[0].k_scale != ks.data_ptr() or got[0].v_scale != vs.data_ptr())):
+        now = (k.data_ptr(), v.data_ptr(), k.shape, k.stride(), None if ks is None else (ks.data_ptr(), vs.data_ptr()))
+        got = self.__dict__.get("_made")
+        if got is None or got[0] != now:
+            self.__post_init__()
             shape, (sp, sh, st, _) = tuple(k.shape), k.stride()
             made = _lib.KVCache(_lib.ptr(k), _lib.ptr(v), _lib.ptr(ks), _lib.ptr(vs), sp, sh, st, shape[0], _CODE[k.dtype],
                                 *shape[1:])
-            got = self.__dict__["_made"] = (made, (_lib.ctypes.addressof(made), k.dtype, shape))
+            got = self.__dict__["_made"] = (now, (_lib.ctypes.byref(made), k.dtype, shape))
         return got[1]
+
+    def __getstate__(self) -> dict:
+        """What a copy or a pickle holds: the tensors.  The description is of this object's memory."""
+        return {n: t for n, t in self.__dict__.items() if n != "_made"}
 
 
 def _overlaps(token: int, head: int, t: int, h: int, dim: int) -> bool:

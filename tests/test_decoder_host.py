@@ -2,7 +2,11 @@
 launch (the pointers are placeholders that no kernel sees), and the workspace query follows the plan."""
 from __future__ import annotations
 
+import copy
 import ctypes
+import gc
+import pickle
+import weakref
 
 import pytest
 import torch
@@ -146,3 +150,81 @@ def test_more_threads_than_a_launch_takes():
                                                 (0, 64, 1, 4, False), (256, 32, 3, 4, True), (256, 0, 3, 1, False)])
 def test_rows_that_overlap(token, head, t, h, bad):
     assert ops._overlaps(token, head, t, h, 64) is bad
+
+
+class _Tensors(ops.PagedKVCache):
+    """A cache whose tensors move as a program's may: into new memory, to another shape or order."""
+
+    def move(self, **to):
+        for t in (self.k, self.v):
+            x = torch.zeros(to.get("shape", t.shape), dtype=t.dtype)
+            t.set_(x.transpose(1, 2) if to.get("turn") else x)
+
+
+def _two_heads():
+    return _Tensors(*(torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16) for _ in range(2)))
+
+
+@pytest.mark.parametrize("op", ["append", "attention"])
+def test_a_cache_description_lives_through_its_call(op, monkeypatch):
+    """The C call reads it without the interpreter's lock, and another thread may have it made again meanwhile."""
+    freed = []
+
+    class Watched(_lib.KVCache):
+        def __init__(self, *a):
+            super().__init__(*a)
+            weakref.finalize(self, freed.append, ctypes.addressof(self))
+
+    cache, calls = _two_heads(), []
+
+    class Lib:
+        def call(self, *a):
+            cache.move()
+            cache._handle()  # what another thread's call does
+            gc.collect()
+            calls.append(list(freed))
+            return _lib.OK
+
+        fg_rope_append = fg_prefix_attention = call
+
+        def fg_prefix_attention_workspace_bytes(self, *a):
+            return 0
+
+    for owner, name, value in ((_lib, "KVCache", Watched), (_lib, "lib", Lib), (_lib, "stream_of", lambda t: 0),
+                               (ops, "_on_gpu", lambda *a: None)):
+        monkeypatch.setattr(owner, name, value)
+    q, k, i = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 64, dtype=torch.bfloat16), torch.arange(3)
+    if op == "append":
+        ops.rope_append(q, k, k, i, torch.zeros(4, 64), cache, i)
+    else:
+        ops.prefix_attention(q, cache, torch.zeros(3, 1, dtype=torch.int32), i.int())
+    assert calls == [[]]
+
+
+def test_a_used_cache_can_be_copied_and_pickled():
+    cache = ops.PagedKVCache.allocate(3, 2, 16, 64, torch.float8_e4m3fn, "cpu")
+    assert cache._handle()[2] == (3, 2, 16, 64)
+    for other in (copy.deepcopy(cache), copy.copy(cache)):
+        assert other._handle()[1:] == cache._handle()[1:] and other.k_scale.tolist() == [1, 1]
+    assert copy.deepcopy(cache).k.data_ptr() != cache.k.data_ptr()
+    cache = ops.PagedKVCache.allocate(3, 2, 16, 64, device="cpu")  # torch unpickles no e4m3 tensors
+    assert cache._handle()[1:] == pickle.loads(pickle.dumps(cache))._handle()[1:]
+
+
+def _described(cache):
+    made = cache._handle()[0]._obj
+    return [getattr(made, f) for f, _ in _lib.KVCache._fields_]
+
+
+def test_a_cache_description_follows_its_tensors():
+    cache = _two_heads()
+    first = _described(cache)
+    assert first[4:8] == [2 * 16 * 64, 16 * 64, 64, 4]
+    for t in (cache.k, cache.v):  # in place, at the same address
+        t.resize_(2, 2, 16, 64)
+    assert _described(cache)[:2] == first[:2] and _described(cache)[7] == 2 and cache._handle()[2] == (2, 2, 16, 64)
+    cache.move(turn=True, shape=(2, 16, 2, 64))
+    assert _described(cache)[4:7] == [2 * 16 * 64, 64, 2 * 64]
+    cache.k.resize_(1, 2, 16, 64)
+    with pytest.raises(ConfigError):
+        cache._handle()
