@@ -1242,8 +1242,9 @@ const char* attn_sizes(fg::AttnArgs& a, int64_t T, int64_t B, int32_t q_heads, i
     return "bad sizes";
   if (q_heads % kv_heads) return "q_heads is no multiple of kv_heads";
   if (!ragged && (T != B || max_query_len != 1)) return "without query_start each sequence has one query token";
-  if (T * q_heads >= kMaxDim || prefix_len >= kMaxDim / 2 - 4096 || max_seq_len >= kMaxDim / 2 - 4096 ||
-      max_query_len * q_heads >= kMaxDim || B * max_query_len * q_heads >= kMaxDim)
+  max_query_len = std::min(max_query_len, std::max<int64_t>(T, 1));  // no sequence has more query tokens than there are
+  if (T >= kMaxDim || B >= kMaxDim || T * q_heads >= kMaxDim || prefix_len >= kMaxDim / 2 - 4096 ||
+      max_seq_len >= kMaxDim / 2 - 4096 || (double)B * max_query_len * q_heads >= kMaxDim)
     return "sizes past 32 bits";
   a.T = (int)T; a.B = (int)B; a.Hq = q_heads; a.Hk = kv_heads; a.G = q_heads / kv_heads; a.D = head_dim;
   a.item = item;

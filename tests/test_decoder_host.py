@@ -228,3 +228,15 @@ def test_a_cache_description_follows_its_tensors():
     cache.k.resize_(1, 2, 16, 64)
     with pytest.raises(ConfigError):
         cache._handle()
+
+
+def test_a_query_bound_past_the_queries_is_the_queries():
+    """No sequence has more query tokens than there are, so a looser bound asks for no other plan."""
+    query = _lib.lib().fg_prefix_attention_workspace_bytes
+    for t in (7, 300):
+        want = query(t, 3, 8, 2, 64, _lib.BF16, 0, 5000, t, 1)
+        for bound in (t + 1, 65536, 2 ** 31 - 2, 2 ** 62):
+            assert query(t, 3, 8, 2, 64, _lib.BF16, 0, 5000, bound, 1) == want > 0
+    # refused for the workspace, which comes after the sizes
+    assert _attention(t=512, b=512, heads=64, starts=P, maxq=65536) == _lib.EINVAL and "workspace" in _lib.last_error()
+    assert _attention(t=2 ** 62, b=2, starts=P, maxq=1) == _lib.EINVAL and "32 bits" in _lib.last_error()
