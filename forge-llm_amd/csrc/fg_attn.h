@@ -72,6 +72,9 @@ __host__ __device__ __forceinline__ int64_t attn_count(int64_t pairs, int64_t ti
   return (pairs < (1 << 30) && attn_by_xcd((int)pairs) ? (pairs + 7) / 8 * 8 : pairs) * tiles;
 }
 
+// Where sequence i's query tokens start: offsets outside the queries count as their begin or end.
+__device__ __forceinline__ int attn_start(const AttnArgs& a, int i) { return min(max(a.starts[i], 0), a.T); }
+
 // Rows of query tokens that no item computes, written where no join follows: tokens of no sequence give zeros (the first
 // sequence's workgroup takes those in front of it, the last one's those behind it), tokens past max_query_len NaN.
 __device__ __forceinline__ void attn_uncovered(const AttnArgs& a, int seq, int head) {
@@ -84,10 +87,10 @@ __device__ __forceinline__ void attn_uncovered(const AttnArgs& a, int seq, int h
     }
   };
   const float nan = __builtin_nanf(""), inf = __builtin_inff();
-  const int first = max(a.starts[seq], 0), next = min(a.starts[seq + 1], a.T);
-  if (first + a.max_q < next) fill(first + a.max_q, next, nan, nan);
-  if (seq == 0 && first > 0) fill(0, min(first, a.T), 0.f, -inf);
-  if (seq == a.B - 1 && next < a.T) fill(max(next, 0), a.T, 0.f, -inf);
+  const int first = attn_start(a, seq), next = attn_start(a, seq + 1);
+  if (next - first > a.max_q) fill(first + a.max_q, next, nan, nan);
+  if (seq == 0) fill(0, first, 0.f, -inf);
+  if (seq == a.B - 1) fill(next, a.T, 0.f, -inf);
 }
 
 // Item `id` of the grid; false: nothing to do.  TILE rows per item.
@@ -124,8 +127,8 @@ __device__ __forceinline__ bool attn_item(const AttnArgs& a, int id, AttnItem& i
   tile = a.tiles_s - 1 - tile;  // the tiles that see the most first
   int t0 = seq, n = 1;  // the sequence's query tokens
   if (a.starts) {
-    t0 = max(a.starts[seq], 0);
-    n = min(a.starts[seq + 1], a.T) - t0;
+    t0 = attn_start(a, seq);
+    n = attn_start(a, seq + 1) - t0;
   }
   it.head = pair - rest * a.Hk;
   if (a.starts && !a.acc && tile == 0 && part == 0) attn_uncovered(a, seq, it.head);

@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
     }
     seq = lo;
     inside = a.B > 0 && a.starts[seq] <= t && t < a.starts[seq + 1];
-    served = !inside || t - a.starts[seq] < a.max_q;
+    served = !inside || t - attn_start(a, seq) < a.max_q;
   }
   const int len = inside ? (a.joined ? a.prefix_len : 0) + max(min(a.lens[seq], a.max_len), 0) : 0;
   const int own = max((len + a.part_s - 1) / a.part_s, 1), n = inside ? a.parts_p + own : 0;

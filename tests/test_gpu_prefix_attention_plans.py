@@ -150,3 +150,20 @@ def test_a_graph_of_both_kinds_follows_its_inputs():
         torch.cuda.synchronize()
         eager = ops.prefix_attention(**call)
         assert torch.equal(out, eager[0]) and torch.equal(lse, eager[1]) and not torch.equal(out, want[0])
+
+
+@pytest.mark.parametrize("prefix,lens,h", [(0, [60, 2, 90], 8), (100, [60, 2, 90], 8), (3000, [60, 2, 90], 2), (3000, [900, 2, 1500], 64)])
+def test_query_offsets_outside_the_queries(prefix, lens, h):
+    """They count as the queries' begin or end: sequences in front and behind that have no queries there change nothing."""
+    call, ref = _call([3, 2, 4], lens, prefix, h, 2, 64)
+    want = ops.prefix_attention(**call)
+    assert_attention(*want, ref, BF)
+    far = 2 ** 31 - 1
+    for front, back in (([-5], []), ([-far - 1, -7], [far]), ([], [far, far - 3, far])):
+        # the first sequence's own tokens start in front of the queries
+        starts = [*(front or [0]), *call["query_start"].tolist()[1:], *back]
+        none = [torch.zeros(n, dtype=torch.int64) for n in (max(len(front) - 1, 0), len(back))]
+        rows = torch.cat((none[0], torch.arange(3), none[1])).to(DEV)
+        got = ops.prefix_attention(**{**call, "query_start": torch.tensor(starts, dtype=torch.int32, device=DEV),
+                                      "page_table": call["page_table"][rows], "seq_lens": call["seq_lens"][rows]})
+        assert_attention(*got, ref, BF)
