@@ -218,6 +218,18 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
   }
 }
 
+// What makes a score an exponent of 2: the softmax's scale and, in e4m3, the key head's.  Masked scores are -inf, which a factor
+// of zero would make NaN and one below zero +inf: the rows change their sign instead, and the smallest normal number, which
+// leaves all weights equal, stands for anything under it.
+struct AttnFactor {
+  float value;
+  uint32_t sign;  // of two 16-bit values of a row
+};
+__device__ __forceinline__ AttnFactor attn_factor(float scale_log2, float key_scale) {
+  const float f = scale_log2 * key_scale, size = fabsf(f);
+  return {size < 0x1p-126f ? 0x1p-126f : size, f < 0.f ? 0x80008000u : 0u};
+}
+
 // A row whose running maximum is still -inf has seen no key: its exponents count from 0, so that they are exp2(-inf) = 0.
 __device__ __forceinline__ float attn_base(float m) { return m == -__builtin_inff() ? 0.f : m; }
 

@@ -46,7 +46,8 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int id, uint8_t* ld
   // this lane's row: the fragment of Q, and the keys it sees
   const int row = it.row0 + l16, tok = row / a.G, g = row - tok * a.G;
   const uint16_t* qp = a.q + (int64_t)(it.token0 + tok) * a.q_t + (int64_t)(it.head * a.G + g) * a.q_h;
-  const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale turns the rows instead
+  const AttnFactor factor = attn_factor(a.scale_log2, FP8 ? a.ks[it.head] : 1.f);
+  const uint32_t sign = factor.sign;
   s16x8 qf[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -59,7 +60,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int id, uint8_t* ld
   }
   const int seen = it.causal ? max(it.seen0 + tok, it.front) : it.end;
   const int min_seen = it.causal ? max(it.seen0 + it.row0 / a.G, it.front) : it.end;  // what the tile's first row sees
-  const float sc = fabsf(a.scale_log2) * (FP8 ? a.ks[it.head] : 1.f);
+  const float sc = factor.value;
   const uint8_t *kb = a.k + it.head * a.c_head + grp * 16, *vb = a.v + it.head * a.c_head + grp * 16;
   const int units = a.D * IT / 16;
 

@@ -69,7 +69,8 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int id, uint8_t* ld
 
   const int row0 = it.row0 + 32 * wave, row = row0 + l32, tok = row / a.G, g = row - tok * a.G;
   const bool live = row0 < it.rows;  // this wavefront has rows
-  const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale turns the rows instead
+  const AttnFactor factor = attn_factor(a.scale_log2, FP8 ? a.ks[it.head] : 1.f);
+  const uint32_t sign = factor.sign;
   s16x8 qf[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -84,7 +85,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int id, uint8_t* ld
   }
   const int seen = it.causal ? max(it.seen0 + tok, it.front) : it.end;
   const int min_seen = it.causal ? max(it.seen0 + row0 / a.G, it.front) : it.end;  // what the wavefront's first row sees
-  const float sc = fabsf(a.scale_log2) * (FP8 ? a.ks[it.head] : 1.f);
+  const float sc = factor.value;
 
   f32x16 o[DB];
   float m = -__builtin_inff(), l = 0.f;

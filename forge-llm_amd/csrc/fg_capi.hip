@@ -1297,8 +1297,7 @@ int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtyp
   a.ks = cache->k_scale; a.vs = cache->v_scale;
   a.prefix_pages = prefix_pages; a.pages = page_table; a.ld_pages = ld_pages; a.lens = seq_lens; a.starts = query_start;
   a.page = cache->page_size; a.n_pages = (int)cache->num_pages;
-  // a scale of zero would make the masked scores 0 * -inf; the smallest normal number gives the same equal weights
-  a.scale_log2 = (scale == 0.f ? 1.17549435e-38f : scale) * 1.4426950408889634f;
+  a.scale_log2 = scale * 1.4426950408889634f;
   return hip_status(fg::launch_attn(a, dtype == FG_BF16, cache->dtype == FG_E4M3, workspace, need,
                                     static_cast<hipStream_t>(stream)),
                     "fg_prefix_attention launch");

@@ -167,3 +167,19 @@ def test_query_offsets_outside_the_queries(prefix, lens, h):
         got = ops.prefix_attention(**{**call, "query_start": torch.tensor(starts, dtype=torch.int32, device=DEV),
                                       "page_table": call["page_table"][rows], "seq_lens": call["seq_lens"][rows]})
         assert_attention(*got, ref, BF)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("queries,lens,prefix,h,kernel", [
+    ([1, 1], [40, 301], 70, 4, "attn_rows_kernel"), ([70, 30], [100, 300], 90, 8, "attn_tile_kernel"),
+    ([1] * 40, [(37 * i) % 300 for i in range(40)], 700, 16, "attn_mixed_kernel"), ([1], [77], 0, 4, "attn_rows_kernel")])
+def test_key_scales_and_scales_that_are_not_positive(queries, lens, prefix, h, kernel, dt):
+    """A cached key is code * scale of its head, whatever the scale: zero gives equal weights, a negative one turns the scores."""
+    for key_scale, scale in ((0.0, 0.125), (-0.05, 0.125), (0.05, -0.125), (-0.05, -0.125), (-0.05, 0.0), (2.0 ** -120, 2.0 ** -20)):
+        call, _ = _call(queries, lens, prefix, h, 2, 64, 16, dt, E4)
+        call["cache"].k_scale[1] = key_scale
+        starts = call["query_start"] if call["query_start"] is not None else torch.arange(len(lens) + 1)
+        ref = attention_ref_fast(call["q"], call["cache"], call["page_table"], call["seq_lens"], call["prefix_pages"], prefix, starts, scale)
+        got = ops.prefix_attention(**call, scale=scale)
+        assert kernel in _lib.last_kernel()
+        assert_attention(*got, ref, dt)
