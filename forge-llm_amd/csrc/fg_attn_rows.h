@@ -141,7 +141,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int id, uint8_t* ld
     float top = x[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-    top *= sc;
+    top = attn_top<BF16>(top, sc);
     if (__any(top > m + kSlack)) {
       top = fmaxf(top, __shfl_xor(top, 16, kWave));
       top = fmaxf(top, __shfl_xor(top, 32, kWave));

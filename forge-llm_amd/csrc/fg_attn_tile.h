@@ -204,7 +204,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, int id, uint8_t* ld
       for (int b = 0; b < TB; ++b)
 #pragma unroll
         for (int j = 0; j < 16; ++j) top = fmaxf(top, s[b][j]);
-      top *= sc;
+      top = attn_top<BF16>(top, sc);
       if (__any(top > m + kSlack)) {
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
         const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - attn_base(mn));

@@ -183,3 +183,28 @@ def test_key_scales_and_scales_that_are_not_positive(queries, lens, prefix, h, k
         got = ops.prefix_attention(**call, scale=scale)
         assert kernel in _lib.last_kernel()
         assert_attention(*got, ref, dt)
+
+
+@pytest.mark.parametrize("t,h,n,kernel", [(1, 4, 2048, "attn_rows_kernel"), (1, 4, 131072, "attn_rows_kernel"), (3, 4, 250, "attn_rows_kernel"),
+                                          (40, 8, 5000, "attn_tile_kernel"), (1024, 64, 131072, "attn_tile_kernel parts=0+1")])
+@pytest.mark.parametrize("cdt", [HF, E4])
+def test_one_key_above_many_in_fp16(t, h, n, kernel, cdt):
+    """Each of the others has 2^-25 of its weight, all of them up to 0.4% of the result.  A weight is rounded by 2^-11 of itself
+    and by no more than 2^-32 of the largest (half of fp16's smallest step, counted from 2^7 below that)."""
+    page, score = 256, 17.25  # e^-17.25 = 2^-24.9
+    pages = -(-n // page)
+    k, v = torch.zeros(pages, 1, page, 64, device=DEV), torch.ones(pages, 1, page, 64, device=DEV)
+    k[0, 0, 5, 0], v[0, 0, 5] = (16.0 if cdt == E4 else score), 0.0
+    scales = [torch.full((1,), x, device=DEV) for x in (score / 16, 1.0)] if cdt == E4 else []
+    cache = ops.PagedKVCache(k.to(cdt), v.to(cdt), *scales)
+    q = torch.zeros(t, h, 64, dtype=HF, device=DEV)
+    q[..., 0] = 8.0
+    i32 = dict(dtype=torch.int32, device=DEV)
+    out, lse = ops.prefix_attention(q, cache, torch.arange(pages, **i32).view(1, -1), torch.tensor([n], **i32), scale=0.125,
+                                    query_start=torch.tensor([0, t], **i32), max_query_len=t, max_seq_len=n, return_lse=True)
+    assert kernel in _lib.last_kernel(), _lib.last_kernel()
+    others = (n - t + torch.arange(t, dtype=torch.float64)) * torch.exp(torch.tensor(-score, dtype=torch.float64))
+    want = (others / (1 + others)).view(t, 1, 1)
+    err = (out.cpu().double() - want).abs()
+    assert bool((err <= (2.0 ** -10 + 2.0 ** -12) * want + n * 2.0 ** -32 + 2.0 ** -25).all()), (err.max(), want.max())
+    assert bool(((lse.cpu().double() - score - torch.log1p(others).view(t, 1)).abs() <= 2.0 ** -13 * (1 + score)).all())
