@@ -1146,6 +1146,39 @@ namespace {
 
 int item_bytes(int dt) { return dt == FG_F32 ? 4 : (dt == FG_E4M3 ? 1 : 2); }
 
+struct Axis {
+  int64_t stride, count;
+};
+
+// Whether rows of `dim` adjacent elements, one for each index of three axes, share an element.  The places of two rows differ
+// by a sum of whole multiples i of the strides, |i| < count and not all zero; the rows overlap if it is below dim.
+bool rows_overlap(Axis x, Axis y, Axis z, int64_t dim) {
+  Axis a[3];
+  int n = 0;
+  for (Axis v : {x, y, z})
+    if (v.count > 1) a[n++] = {v.stride < 0 ? -v.stride : v.stride, v.count};
+  for (int i = n; i < 3; ++i) a[i] = {0, 1};
+  std::sort(a, a + n, [](const Axis& l, const Axis& r) { return l.stride < r.stride; });
+  // each axis steps over all that the ones before it hold
+  __int128 extent = dim;
+  bool nested = true;
+  for (int i = 0; i < n; ++i) {
+    if (a[i].stride < dim) return true;
+    nested = nested && a[i].stride >= extent;
+    extent += (__int128)a[i].stride * (a[i].count - 1);
+  }
+  if (nested) return false;
+  // axes that interleave: for each pair of multiples of the two short ones, the nearest one of the longest
+  std::sort(a, a + n, [](const Axis& l, const Axis& r) { return l.count > r.count; });
+  for (int64_t j = 0; j < a[1].count; ++j)
+    for (int64_t k = 1 - a[2].count; k < a[2].count; ++k) {
+      const __int128 at = (__int128)j * a[1].stride + (__int128)k * a[2].stride, far = at < 0 ? -at : at;
+      const __int128 near = std::min<__int128>((far + a[0].stride / 2) / a[0].stride, a[0].count - 1) * a[0].stride;
+      if ((j || k) && far - near < dim && near - far < dim) return true;
+    }
+  return false;
+}
+
 // Whether `cache` can hold 16-bit values of `dtype`, or e4m3 codes, as the kernels read them.
 int check_cache(const fg_kv_cache* c, int dtype, const char* op) {
   if (!c || !c->k || !c->v) return fail(FG_EINVAL, "%s: null cache", op);
@@ -1210,6 +1243,11 @@ int fg_rope_append(const void* q, int64_t q_token, int64_t q_head, const void* k
   if (dtype != FG_F16 && dtype != FG_BF16) return fail(FG_EINVAL, "fg_rope_append: q, k and v are fp16 or bf16");
   const int bad = check_cache(cache, dtype, "fg_rope_append");
   if (bad) return bad;
+  if (rows_overlap({qo_token, T}, {qo_head, q_heads}, {0, 1}, cache->head_dim))
+    return fail(FG_EINVAL, "fg_rope_append: q_out's rows overlap");
+  if (rows_overlap({cache->page_stride, cache->num_pages}, {cache->head_stride, cache->kv_heads},
+                   {cache->token_stride, cache->page_size}, cache->head_dim))
+    return fail(FG_EINVAL, "fg_rope_append: the cache's rows overlap");
   if (!q || !k || !v || !q_out || !positions || !table || !slots) return fail(FG_EINVAL, "fg_rope_append: null tensor");
   if (rot < 2 || rot % 2 || rot > cache->head_dim || ld_table < rot)
     return fail(FG_EINVAL, "fg_rope_append: rot is even, at most head_dim and at most the table's columns");
@@ -1282,6 +1320,8 @@ int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtyp
   if (dtype != FG_F16 && dtype != FG_BF16) return fail(FG_EINVAL, "fg_prefix_attention: q is fp16 or bf16");
   if (!q || !out || (B > 0 && !seq_lens) || (max_seq_len > 0 && B > 0 && !page_table) || (prefix_len > 0 && !prefix_pages))
     return fail(FG_EINVAL, "fg_prefix_attention: null tensor");
+  if (rows_overlap({o_token, T}, {o_head, q_heads}, {0, 1}, cache->head_dim))
+    return fail(FG_EINVAL, "fg_prefix_attention: out's rows overlap");
   if (B > 0 && ld_pages * cache->page_size < max_seq_len)
     return fail(FG_EINVAL, "fg_prefix_attention: max_seq_len is past the page table's columns");
   const size_t need = fg::attn_plan(a);

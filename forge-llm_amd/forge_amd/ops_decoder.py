@@ -129,7 +129,8 @@ class PagedKVCache:
     """Keys and values of many sequences in pages: ``k`` and ``v`` are ``[pages, kv_heads, page_size, head_dim]`` (any
     strides of whole 16-byte units, the same for both, columns adjacent) in fp16, bf16 or float8_e4m3fn; an e4m3 value
     stands for ``code * k_scale[head]`` (``v_scale``), fp32 ``[kv_heads]``.  A page holds each key head's tokens next to
-    each other (:meth:`allocate`), the order in which attention reads them."""
+    each other (:meth:`allocate`), the order in which attention reads them.  Rows that share memory, as those of keys expanded
+    over heads, can be read but not appended to."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -190,8 +191,16 @@ class PagedKVCache:
 
 
 def _overlaps(token: int, head: int, t: int, h: int, dim: int) -> bool:
-    """Whether rows of ``dim`` columns at these strides (one expanded from fewer, say) share elements."""
-    return (t > 1 and token < dim) or (h > 1 and head < dim)
+    """Whether rows of ``dim`` columns at these strides (expanded from fewer, or windows that slide, say) share elements."""
+    if head >= dim and token >= (h - 1) * head + dim:
+        return False  # a token steps over its heads
+    if (t > 1 and token < dim) or (h > 1 and head < dim):
+        return True
+    if t <= 1 or h <= 1:
+        return False
+    (n, few), (m, many) = sorted(((t, token), (h, head)))
+    # steps of the short axis, and the nearest step of the long one
+    return any(abs(i * few - min((i * few + many // 2) // many, m - 1) * many) < dim for i in range(1, n))
 
 
 def _index(op: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:

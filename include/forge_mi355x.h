@@ -268,7 +268,8 @@ int fg_quant_fp8_row_blocks(const void* x, int64_t ldx, int x_dtype, uint8_t* q,
  * A paged cache: pages of page_size tokens for each key head, element (page, head, token, column) of k and of v at
  * page * page_stride + head * head_stride + token * token_stride + column (elements).  dtype FG_F16 | FG_BF16 |
  * FG_E4M3; e4m3 values stand for code * k_scale[head] (v_scale[head]), device float[kv_heads].  k, v and every stride
- * are whole 16-byte units, head_dim is a multiple of 8 (of 16 for FG_E4M3) up to 256.
+ * are whole 16-byte units, head_dim is a multiple of 8 (of 16 for FG_E4M3) up to 256.  fg_rope_append refuses a cache, and
+ * both operators an output, whose rows share elements.
  * ------------------------------------------------------------------------------------------------------------- */
 typedef struct fg_kv_cache {
   void* k;

@@ -238,5 +238,45 @@ def test_a_query_bound_past_the_queries_is_the_queries():
         for bound in (t + 1, 65536, 2 ** 31 - 2, 2 ** 62):
             assert query(t, 3, 8, 2, 64, _lib.BF16, 0, 5000, bound, 1) == want > 0
     # refused for the workspace, which comes after the sizes
-    assert _attention(t=512, b=512, heads=64, starts=P, maxq=65536) == _lib.EINVAL and "workspace" in _lib.last_error()
+    assert _attention(t=512, b=512, heads=64, ot=4096, starts=P, maxq=65536) == _lib.EINVAL and "workspace" in _lib.last_error()
     assert _attention(t=2 ** 62, b=2, starts=P, maxq=1) == _lib.EINVAL and "32 bits" in _lib.last_error()
+
+
+def _cover(strides, counts, dim):
+    """Whether the rows share an element, by listing all elements."""
+    at = torch.zeros(1, dtype=torch.int64)
+    for s, n in zip(strides, counts):
+        at = (at.view(-1, 1) + s * torch.arange(n)).flatten()
+    at = (at.view(-1, 1) + torch.arange(dim)).flatten()
+    return len(at.unique()) < len(at)
+
+
+@pytest.mark.parametrize("token,head,t,h,bad", [(64, 64, 3, 4, True), (192, 64, 3, 4, True), (64, 128, 3, 4, True), (128, 64, 1, 4, False),
+                                                (192, 128, 2, 3, False), (192, 128, 2, 2, False), (192, 128, 3, 4, True), (100, 164, 2, 2, False),
+                                                (100, 163, 2, 2, True), (63, 1000, 1, 4, False), (64, 256, 5, 4, True)])
+def test_rows_that_overlap_across_tokens_and_heads(token, head, t, h, bad):
+    assert _cover((token, head), (t, h), 64) is bad
+    assert ops._overlaps(token, head, t, h, 64) is bad
+    status = _append(t=t, heads=h, qot=token, qoh=head, pos=None)  # refused for its output first, for its positions else
+    assert status == _lib.EINVAL and ("overlap" in _lib.last_error()) is bad
+    status = _attention(_cache(kv_heads=1), t=t, b=t, heads=h, ot=token, oh=head)
+    assert status == _lib.EINVAL and ("overlap" in _lib.last_error()) is bad and (bad or "workspace" in _lib.last_error())
+
+
+def test_rows_that_overlap_by_their_elements():
+    for token in (0, 8, 60, 64, 65, 100, 128, 192, 200):
+        for head in (0, 50, 64, 72, 128, 130, 256):
+            for t, h in ((1, 1), (1, 3), (2, 2), (3, 2), (2, 4), (5, 3)):
+                assert ops._overlaps(token, head, t, h, 64) is _cover((token, head), (t, h), 64), (token, head, t, h)
+
+
+@pytest.mark.parametrize("strides,pages,bad", [((2048, 0, 64), 4, True), ((0, 1024, 64), 4, True), ((0, 1024, 64), 1, False),
+                                               ((1024, 1024, 64), 4, True), ((2048, 64, 128), 4, False), ((2048, 64, 64), 4, True),
+                                               ((64, 4096, 256), 4, False), ((64, 2048, 192), 4, True), ((2112, 1056, 64), 4, False),
+                                               ((2048, 1056, 64), 4, True)])
+def test_caches_whose_rows_overlap_take_no_tokens(strides, pages, bad):
+    """Such a cache can be read (keys expanded over heads, say), not written."""
+    c = _cache(page_stride=strides[0], head_stride=strides[1], token_stride=strides[2], num_pages=pages)
+    assert _cover(strides, (pages, 2, 16), 64) is bad
+    assert _append(c, pos=None) == _lib.EINVAL and ("overlap" in _lib.last_error()) is bad
+    assert _attention(c) == _lib.EINVAL and "workspace" in _lib.last_error()
