@@ -1302,7 +1302,9 @@ size_t fg_prefix_attention_workspace_bytes(int64_t T, int64_t B, int32_t q_heads
   if (attn_sizes(a, T, B, q_heads, kv_heads, head_dim, prefix_len, max_seq_len, max_query_len, ragged != 0,
                  item_bytes(cache_dtype)))
     return 0;
-  return T == 0 ? 0 : fg::attn_plan(a);
+  if (T == 0) return 0;
+  const size_t need = fg::attn_plan(a);
+  return a.items < 0 ? 0 : need;  // a plan that the call refuses takes no memory
 }
 
 int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const fg_kv_cache* cache,

@@ -280,3 +280,14 @@ def test_caches_whose_rows_overlap_take_no_tokens(strides, pages, bad):
     assert _cover(strides, (pages, 2, 16), 64) is bad
     assert _append(c, pos=None) == _lib.EINVAL and ("overlap" in _lib.last_error()) is bad
     assert _attention(c) == _lib.EINVAL and "workspace" in _lib.last_error()
+
+
+@pytest.mark.parametrize("t,b,h,hk,d,prefix,seq,maxq", [(2 ** 24, 2 ** 18, 4, 2, 64, 4000, 32, 64), (2 ** 24, 2 ** 24, 4, 2, 64, 4000, 32, 1),
+                                                        (2 ** 20, 2 ** 16, 64, 8, 128, 0, 8192, 511)])
+def test_a_plan_that_is_refused_asks_for_no_workspace(t, b, h, hk, d, prefix, seq, maxq):
+    """The caller would allocate it in front of the call, tens of GiB."""
+    query = _lib.lib().fg_prefix_attention_workspace_bytes
+    assert query(t, b, h, hk, d, _lib.BF16, prefix, seq, maxq, 1) == 0
+    cache = _cache(kv_heads=hk, head_dim=d, head_stride=16 * d, token_stride=d, page_stride=16 * d * hk)
+    status = _attention(cache, t=t, b=b, heads=h, ot=h * d, oh=d, prefix=prefix, seq=seq, ld=-(-seq // 16), starts=P, maxq=maxq)
+    assert status == _lib.EINVAL and "more work items" in _lib.last_error()
