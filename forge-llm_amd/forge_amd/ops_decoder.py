@@ -334,7 +334,7 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
         if _overlaps(o0, o1, t, h, dim):
             raise ConfigError(f"{op}: out's rows overlap")
         ld, column = page_table.stride()
-        if column != 1 or b <= 1:
+        if column != 1 or b <= 1 or ld < width:
             page_table, ld = page_table.contiguous(), width
         if not seq_lens.is_contiguous():
             seq_lens = seq_lens.contiguous()

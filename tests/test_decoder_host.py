@@ -291,3 +291,27 @@ def test_a_plan_that_is_refused_asks_for_no_workspace(t, b, h, hk, d, prefix, se
     cache = _cache(kv_heads=hk, head_dim=d, head_stride=16 * d, token_stride=d, page_stride=16 * d * hk)
     status = _attention(cache, t=t, b=b, heads=h, ot=h * d, oh=d, prefix=prefix, seq=seq, ld=-(-seq // 16), starts=P, maxq=maxq)
     assert status == _lib.EINVAL and "more work items" in _lib.last_error()
+
+
+@pytest.mark.parametrize("expanded", [False, True])
+def test_one_page_list_for_all_sequences(expanded, monkeypatch):
+    """A page table expanded over the sequences goes to the C call as rows of its own width, as any other."""
+    seen = []
+
+    class Lib:
+        def fg_prefix_attention(self, *a):
+            seen.append((a[7], a[8], a[14]))
+            return _lib.OK
+
+        def fg_prefix_attention_workspace_bytes(self, *a):
+            return 0
+
+    for owner, name, value in ((_lib, "lib", Lib), (_lib, "stream_of", lambda t: 0), (ops, "_on_gpu", lambda *a: None)):
+        monkeypatch.setattr(owner, name, value)
+    ops._attention_workspace.cache_clear()
+    one = torch.arange(2, dtype=torch.int32).view(1, 2)
+    table = one.expand(3, 2) if expanded else one.repeat(3, 1)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    ops.prefix_attention(q, _two_heads(), table, torch.full((3,), 20, dtype=torch.int32))
+    assert len(seen) == 1 and seen[0][1] == 2 and seen[0][2] == 32
+    ops._attention_workspace.cache_clear()

@@ -274,3 +274,15 @@ def test_refusals():
     odd = ops.PagedKVCache.allocate(1, 2, 16, 72, E4, DEV)
     with pytest.raises(Exception, match="head_dim"):
         ops.prefix_attention(torch.zeros(2, 4, 72, dtype=BF, device=DEV), odd, c.table, c.lens)
+
+
+def test_one_page_list_for_all_sequences():
+    c = _Call([1] * 3, [33, 20, 40], 0, 8, 2, 64, 16)
+    c.table = torch.tensor([[7, 1, 4]], dtype=torch.int32, device=DEV)
+    for x in (c.cache.k, c.cache.v):
+        x[[7, 1, 4]] = 1.0
+        x[[7, 1, 4], :, 3] = -0.5
+    c.table = c.table.repeat(3, 1)
+    want = c.check()
+    c.table = c.table[:1].expand(3, 3)
+    assert all(torch.equal(a, b) for a, b in zip(want, c.run()))
