@@ -7,7 +7,8 @@
 //
 // One workgroup per row, 8 columns per thread and unit, the row in registers from its one read to its one write.  With the
 // weight multiplied in first, y = t rs for t = h w and the row's rs: rounding is monotonic, so max |y| = |max |t| rs| exactly,
-// and one exchange between the wavefronts carries both the sum of squares and the maximum.  What bounds it is the latency of
+// and one exchange between the wavefronts carries both the sum of squares and the maximum.  A row with a product past fp32's
+// range takes a second turn, h rs w.  What bounds it is the latency of
 // that chain for few rows and HBM for many.
 //
 // Rows need no alignment: 16-byte accesses at any address of their element type (the hardware takes them), and the last
@@ -121,6 +122,16 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, int64_t i, int n, const
   }
 }
 
+// Weights of the columns [i, i + n): ones without a weight.
+__device__ __forceinline__ void weights8(const NormArgs& a, int i, int n, float (&w)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = 1.f;
+  if (!a.w) return;
+  if (a.wdt == FG_F32) widen8<FG_F32>(load_raw8<FG_F32>(a.w, i, n), w);
+  else if (a.wdt == FG_BF16) widen8<FG_BF16>(load_raw8<FG_BF16>(a.w, i, n), w);
+  else widen8<FG_F16>(load_raw8<FG_F16>(a.w, i, n), w);
+}
+
 }  // namespace
 
 // RT: the residual's type, -1 for none.  A thread holds the row's units t, t + T, .. (C of them at most, T threads).
@@ -167,13 +178,7 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const NormArgs a) {
       store_raw8<HT>(static_cast<char*>(a.ro) + row * a.ldro * (HT == FG_F32 ? 4 : 2), at(c), n, kept);
     }
     float w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = 1.f;
-    if (a.w) {
-      if (a.wdt == FG_F32) widen8<FG_F32>(load_raw8<FG_F32>(a.w, at(c), n), w);
-      else if (a.wdt == FG_BF16) widen8<FG_BF16>(load_raw8<FG_BF16>(a.w, at(c), n), w);
-      else widen8<FG_F16>(load_raw8<FG_F16>(a.w, at(c), n), w);
-    }
+    weights8(a, at(c), n, w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       ss = __builtin_fmaf(h[j], h[j], ss);
@@ -200,7 +205,38 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const NormArgs a) {
       top = max(top, red_max[w]);
     }
   }
-  const float rs = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)K) + a.eps));
+  float rs = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)K) + a.eps));
+  if (top >= 0x7f800000u) {
+    // a product h w passed fp32's range (or is no number): y as it is defined, h rs first, from what this thread kept or read
+    top = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int n = K - at(c);
+      if (n <= 0) continue;
+      float h[8], w[8];
+      if constexpr (RT >= 0)
+        widen8<HT>(load_raw8<HT>(static_cast<char*>(a.ro) + row * a.ldro * (HT == FG_F32 ? 4 : 2), at(c), n), h);
+      else
+        widen8<XT>(load_raw8<XT>(xrow, at(c), n), h);
+      weights8(a, at(c), n, w);
+      m[c] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        t[c][j] = h[j] * rs * w[j];
+        m[c] = max(m[c], __float_as_uint(t[c][j]) & 0x7fffffffu);
+      }
+      top = max(top, m[c]);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, kWave));
+    if (waves > 1) {
+      __syncthreads();  // everyone has read the first maxima
+      if (lane == 0) red_max[wave] = top;
+      __syncthreads();
+      for (int w = 0; w < waves; ++w) top = max(top, red_max[w]);
+    }
+    rs = 1.f;
+  }
   const bool int8 = a.ydt == FG_I8;
   auto scale_of = [&](uint32_t bits) {  // a NaN is not above 0: such rows take scale 1
     const float amax = __uint_as_float(bits) * rs;

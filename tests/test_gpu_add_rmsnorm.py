@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from forge_amd import _lib
 from forge_amd import ops_decoder as ops
 from forge_amd import ops_gemm
 from forge_amd.errors import ConfigError
@@ -154,3 +155,37 @@ def test_refusals():
         ops.add_rmsnorm(x.cpu(), w.cpu())
     with pytest.raises(Exception, match="32768"):
         ops.add_rmsnorm(torch.zeros(1, 32769, dtype=BF, device=DEV), None)
+
+
+@pytest.mark.parametrize("quant", QUANTS)
+@pytest.mark.parametrize("dt,rdt", [(BF, BF), (BF, FP), (BF, None), (FP, FP), (FP, None)])
+def test_products_with_the_weight_past_the_type(dt, rdt, quant):
+    """h w passes fp32's range where h / rms * w does not: in some rows, in a few columns of a row, in the last odd unit."""
+    for m, k in ((4, 64), (3, 1000), (5, 5001), (2, 20000), (600, 1030)):
+        x, r, w = _data(m, k, dt, rdt)
+        w = w.float()
+        w[k // 2], w[k - 1] = 2e23, -1e24
+        x[1] = (x[1].float() * 1e15).to(dt)  # the squares' sum stays below 2^127
+        x[0, k - 1] = 3.0
+        got = ops.add_rmsnorm(x.to(DEV), w.to(DEV), None if r is None else r.to(DEV), eps=EPS, quant=quant)
+        _check(x, r, w, got, quant)
+
+
+def test_squares_past_the_type_behind_a_large_weight():
+    """The norm of such a row is infinite, as that of any row whose squares overflow, and its finite values are zeros."""
+    x, w = torch.full((2, 520), 3e38, dtype=BF, device=DEV), torch.full((520,), 2.0, dtype=BF, device=DEV)
+    for quant in QUANTS:
+        got = ops.add_rmsnorm(x, w, quant=quant)
+        assert bool((got.y.float() == 0).all()) and (got.scale is None or bool((got.scale == 1).all()))
+
+
+def test_products_past_the_type_in_place():
+    x, _, w = _data(3, 777, BF, None)
+    w = w.float()
+    w[5] = 1e24
+    x[2] *= 1e15
+    y = x.to(DEV)
+    status = _lib.lib().fg_add_rmsnorm(y.data_ptr(), 777, _lib.BF16, None, 0, None, 0, 0, w.to(DEV).data_ptr(), _lib.F32, EPS,
+                                       y.data_ptr(), 777, _lib.BF16, None, 0, 0, 0, 3, 777, _lib.stream_of(y))
+    assert status == _lib.OK
+    _check(x, None, w, ops.NormOutput(y, None, x), None)
