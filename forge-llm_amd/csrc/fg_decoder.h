@@ -48,6 +48,7 @@ struct RopeAppendArgs {
   int Hq, Hk, D, rot;
 };
 
+bool norm_fits(int64_t M, int64_t K);  // whether one launch takes M rows of K columns
 hipError_t launch_add_rmsnorm(const NormArgs& a, int xdt, int rdt, int64_t M, hipStream_t st);
 hipError_t launch_rope_append(const RopeAppendArgs& a, int64_t T, bool bf16, bool fp8, bool inter, hipStream_t st);
 

@@ -296,10 +296,14 @@ static int norm_plan(int64_t M, int64_t K, int* C) {
   return (int)t;
 }
 
+bool norm_fits(int64_t M, int64_t K) {
+  int C = 0;
+  return launchable(M, norm_plan(M, K, &C));
+}
+
 hipError_t launch_add_rmsnorm(const NormArgs& a, int xdt, int rdt, int64_t M, hipStream_t st) {
   int C = 0;
   const int T = norm_plan(M, a.K, &C);
-  if (!launchable(M, T)) return hipErrorInvalidConfiguration;
   auto go = [&](auto x_tag, auto r_tag, auto c_tag) {
     constexpr int XT = decltype(x_tag)::value, RT = decltype(r_tag)::value, CC = decltype(c_tag)::value;
     note_kernel("add_rmsnorm_kernel<%d,%d,%d> T=%d", XT, RT, CC, T);

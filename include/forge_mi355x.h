@@ -285,7 +285,9 @@ typedef struct fg_kv_cache {
  * y = h * weight / sqrt(mean(h^2) + eps) in fp32, stored as y_dtype: x_dtype, or FG_I8 / FG_E4M3 codes by the largest
  * |y| of a row (block = 0) or of each 1 x block columns (a power of two, 8..512): s = amax / 127 or amax / 448 (1 if
  * amax is not > 0), code = y /_IEEE s rounded half to even; the scale of (row, block) at s[row * s_row + b * s_block].
- * residual_dtype: x_dtype or FG_F32.  weight may be NULL.  residual_out may be residual itself, and y x.  K <= 32768. */
+ * residual_dtype: x_dtype or FG_F32.  weight may be NULL.  K <= 32768.
+ * residual_out may stand in residual's or x's place, and y, where it is no codes, in x's or residual's: with its type and
+ * stride (else, and for y in residual_out's place, FG_EINVAL). */
 int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual, int64_t ldr, void* residual_out,
                    int64_t ldro, int residual_dtype, const void* weight, int weight_dtype, float eps, void* y,
                    int64_t ldy, int y_dtype, float* s, int64_t s_row, int64_t s_block, int32_t block, int64_t M,

@@ -315,3 +315,14 @@ def test_one_page_list_for_all_sequences(expanded, monkeypatch):
     ops.prefix_attention(q, _two_heads(), table, torch.full((3,), 20, dtype=torch.int32))
     assert len(seen) == 1 and seen[0][1] == 2 and seen[0][2] == 32
     ops._attention_workspace.cache_clear()
+
+
+@pytest.mark.parametrize("bad,why", [(dict(y=1), "y"), (dict(y=1, ydt=_lib.BF16, ldy=72), "y"), (dict(y=2), "y"), (dict(y=2, ydt=_lib.BF16, rdt=_lib.F32), "y"),
+                                     (dict(ro=2, ldro=72), "residual_out"), (dict(ro=1, rdt=_lib.F32), "residual_out"),
+                                     (dict(y=3, ydt=_lib.BF16), "y"), (dict(y=3), "y")])
+def test_norm_outputs_in_the_place_of_other_rows(bad, why):
+    """An output in an input's place needs its type and stride: else a row lands where another, unread one stands."""
+    place = {i: ctypes.c_void_p(4096 * i) for i in (1, 2, 3, 4)}  # of x, the residual, residual_out, y
+    kw = dict(x=place[1], r=place[2], ro=place[3], y=place[4])
+    kw.update({k: place[v] if k in ("y", "ro") else v for k, v in bad.items()})
+    assert _norm(**kw) == _lib.EINVAL and f"{why} in the place of" in _lib.last_error()
