@@ -1259,6 +1259,8 @@ int fg_rope_append(const void* q, int64_t q_token, int64_t q_head, const void* k
   if (bad) return bad;
   if (rows_overlap({qo_token, T}, {qo_head, q_heads}, {0, 1}, cache->head_dim))
     return fail(FG_EINVAL, "fg_rope_append: q_out's rows overlap");
+  if (q_out == q && ((T > 1 && qo_token != q_token) || (q_heads > 1 && qo_head != q_head)))
+    return fail(FG_EINVAL, "fg_rope_append: q_out in the place of q's rows with other strides");
   if (rows_overlap({cache->page_stride, cache->num_pages}, {cache->head_stride, cache->kv_heads},
                    {cache->token_stride, cache->page_size}, cache->head_dim))
     return fail(FG_EINVAL, "fg_rope_append: the cache's rows overlap");

@@ -232,8 +232,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     ``cos_sin``: fp32 ``[max_position, rot]``, the cosines of the ``rot / 2`` pairs, then their sines; the first ``rot``
     columns of a head turn, in pairs ``(i, i + rot / 2)`` or, ``interleaved``, ``(2 i, 2 i + 1)``; the others pass through.
     The rotation is fp32, rounded once to the result's type; an e4m3 cache takes ``value / scale`` of its key head, clamped
-    to +-448.  ``q``, ``k``, ``v`` may be views of one projection's output.  A position outside the table gives NaN.  Two
-    tokens of one slot: either may stay.
+    to +-448.  ``q``, ``k``, ``v`` may be views of one projection's output.  A position outside the table gives NaN.  What a
+    slot given to two tokens then holds is undefined: each head's columns may come from either.
     """
     op = "rope_append"
     _on_gpu(q, op)

@@ -296,10 +296,10 @@ int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual
 /* Rotary embedding and cache append of T tokens: q [T][q_heads][head_dim], k and v [T][kv_heads][head_dim] (dtype
  * FG_F16 | FG_BF16, element strides of tokens and heads, columns adjacent).  Columns (i, i + rot / 2), or (2 i, 2 i + 1)
  * with interleaved, i < rot / 2, turn by the angle whose cosine is table[pos * ld_table + i] and sine
- * table[pos * ld_table + rot / 2 + i] (fp32); the other columns pass through.  Rotated q goes to q_out (may be q),
- * rotated k and v to the cache's slot page * page_size + token; a slot outside the cache (negative: padding) is not
- * written.  A position outside [0, max_pos) gives NaN in the rotated columns.  positions and slots are int32 or, with
- * the flag, int64. */
+ * table[pos * ld_table + rot / 2 + i] (fp32); the other columns pass through.  Rotated q goes to q_out (may be q, with
+ * its strides), rotated k and v to the cache's slot page * page_size + token; a slot outside the cache (negative:
+ * padding) is not written, and what one slot given to two tokens then holds is undefined.  A position outside
+ * [0, max_pos) gives NaN in the rotated columns.  positions and slots are int32 or, with the flag, int64. */
 int fg_rope_append(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
                    const void* v, int64_t v_token, int64_t v_head, void* q_out, int64_t qo_token, int64_t qo_head,
                    int dtype, const void* positions, int32_t positions_int64, const float* table, int64_t ld_table,

@@ -326,3 +326,11 @@ def test_norm_outputs_in_the_place_of_other_rows(bad, why):
     kw = dict(x=place[1], r=place[2], ro=place[3], y=place[4])
     kw.update({k: place[v] if k in ("y", "ro") else v for k, v in bad.items()})
     assert _norm(**kw) == _lib.EINVAL and f"{why} in the place of" in _lib.last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(qot=512), dict(qot=64, qoh=192), dict(qoh=72, qot=512)])
+def test_rotated_queries_in_the_place_of_other_rows(bad):
+    """In place means the rows' own strides: else a token lands where another, unread one stands."""
+    assert _append(pos=None, **bad) == _lib.EINVAL and "in the place of" in _lib.last_error()
+    assert _append(pos=None, qo=ctypes.c_void_p(4096), **bad) == _lib.EINVAL and "null" in _lib.last_error()
+    assert _append(pos=None, t=1, qot=512) == _lib.EINVAL and "null" in _lib.last_error()
