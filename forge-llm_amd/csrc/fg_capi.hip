@@ -1303,7 +1303,6 @@ const char* attn_sizes(fg::AttnArgs& a, int64_t T, int64_t B, int32_t q_heads, i
   a.T = (int)T; a.B = (int)B; a.Hq = q_heads; a.Hk = kv_heads; a.G = q_heads / kv_heads; a.D = head_dim;
   a.item = item;
   a.prefix_len = (int)prefix_len; a.max_len = (int)max_seq_len; a.max_q = (int)max_query_len;
-  a.starts = ragged ? reinterpret_cast<const int32_t*>(1) : nullptr;  // the plan asks only whether there are any
   return nullptr;
 }
 

@@ -32,11 +32,6 @@ struct Raw8 {
   u32x4_any w[DT == FG_F32 ? 2 : 1];
 };
 
-template <int DT>
-__device__ __forceinline__ float elem_f(const void* p, int64_t i) {
-  return load_f(p, DT, i);
-}
-
 // Columns [i, i + n) of a row, n = 8 or, in its last unit, fewer (the rest are zeros).
 template <int DT>
 __device__ __forceinline__ Raw8<DT> load_raw8(const void* p, int64_t i, int n) {
