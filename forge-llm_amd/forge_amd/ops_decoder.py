@@ -209,16 +209,31 @@ def _index(op: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _queries(op: str, q: torch.Tensor, cdt: torch.dtype, dim: int) -> torch.Tensor:
-    """``q`` as ``[tokens, heads, dim]`` with adjacent columns (copied only if they are not), of a type that the cache takes."""
-    if q.dim() != 3 or q.shape[2] != dim:
-        raise ConfigError(f"{op}: q must be [tokens, heads, {dim}], got {list(q.shape)}")
+def _queries(op: str, q: torch.Tensor, cdt: torch.dtype, dim: int) -> tuple[torch.Tensor, torch.Size]:
+    """``q`` as ``[tokens, heads, dim]`` with adjacent columns (copied only if they are not), of a type that the cache takes,
+    and its shape."""
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != dim:
+        raise ConfigError(f"{op}: q must be [tokens, heads, {dim}], got {list(shape)}")
     dt = q.dtype
     if dt is not torch.bfloat16 and dt is not torch.float16:
         raise ConfigError(f"{op}: q must be fp16 or bf16")
     if cdt is not dt and cdt is not torch.float8_e4m3fn:
         raise ConfigError(f"{op}: a {cdt} cache does not take {dt} queries")
-    return q if q.stride(2) == 1 or dim == 1 else q.contiguous()
+    return q if q.stride(2) == 1 or dim == 1 else q.contiguous(), shape
+
+
+def _result(op: str, name: str, out: torch.Tensor | None, q: torch.Tensor, shape: torch.Size) -> tuple[torch.Tensor, int, int]:
+    """``out``, or a new tensor like ``q``, and its strides of tokens and heads."""
+    t, h, dim = shape
+    if out is None:
+        return q.new_empty(shape), h * dim, dim
+    if out.shape != shape or out.dtype is not q.dtype or (out.stride(2) != 1 and dim > 1):
+        raise ConfigError(f"{op}: {name} must be like q, with adjacent columns")
+    token, head, _ = out.stride()
+    if t and _overlaps(token, head, t, h, dim):
+        raise ConfigError(f"{op}: {name}'s rows overlap")
+    return out, token, head
 
 
 # ================================================================================================ rotation and append
@@ -239,14 +254,15 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     _on_gpu(q, op)
     handle, cdt, (_, hk, _, dim) = cache._handle()
     _elsewhere(op, q, k, v, positions, cos_sin, slots, cache.k, q_out)
-    q = _queries(op, q, cdt, dim)
+    q, shape = _queries(op, q, cdt, dim)
     dt = q.dtype
-    t, h, _ = shape = q.shape
+    t, h, _ = shape
     if k.shape != (t, hk, dim) or v.shape != (t, hk, dim) or k.dtype is not dt or v.dtype is not dt:
         raise ConfigError(f"{op}: k and v must be [{t}, {hk}, {dim}] of q's type")
-    if cos_sin.dim() != 2 or cos_sin.dtype is not torch.float32:
+    table = cos_sin.shape
+    if len(table) != 2 or cos_sin.dtype is not torch.float32:
         raise ConfigError(f"{op}: cos_sin must be fp32 [positions, rot]")
-    max_pos, rot = cos_sin.shape
+    max_pos, rot = table
     if rot % 2 or not 2 <= rot <= dim:
         raise ConfigError(f"{op}: cos_sin's rot must be even and up to {dim}, got {rot}")
     positions, slots = _index(op, "positions", positions, t), _index(op, "slots", slots, t)
@@ -254,14 +270,9 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     if kc != 1 or vc != 1 or tc != 1 or max_pos <= 1:
         k, v, cos_sin = k.contiguous() if kc != 1 else k, v.contiguous() if vc != 1 else v, cos_sin.contiguous()
         (k0, k1, _), (v0, v1, _), ld = k.stride(), v.stride(), rot
-    if q_out is None:
-        q_out = q.new_empty(shape)
-    elif q_out.shape != shape or q_out.dtype is not dt or (q_out.stride(2) != 1 and dim > 1):
-        raise ConfigError(f"{op}: q_out must be like q, with adjacent columns")
+    q_out, o0, o1 = _result(op, "q_out", q_out, q, shape)
     if t:
-        (q0, q1, _), (o0, o1, _) = q.stride(), q_out.stride()
-        if _overlaps(o0, o1, t, h, dim):
-            raise ConfigError(f"{op}: q_out's rows overlap")
+        q0, q1, _ = q.stride()
         status = _lib.lib().fg_rope_append(
             q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, q_out.data_ptr(), o0, o1, _CODE[dt],
             positions.data_ptr(), positions.dtype is torch.int64, cos_sin.data_ptr(), ld, max_pos, rot, interleaved,
@@ -300,14 +311,15 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     _on_gpu(q, op)
     handle, cdt, (_, hk, page, dim) = cache._handle()
     _elsewhere(op, q, page_table, seq_lens, prefix_pages, query_start, cache.k, out)
-    q = _queries(op, q, cdt, dim)
+    q, shape = _queries(op, q, cdt, dim)
     dt = q.dtype
-    t, h, _ = shape = q.shape
+    t, h, _ = shape
     if h % hk or h == 0:
         raise ConfigError(f"{op}: {h} query heads are no multiple of {hk} key heads")
-    if page_table.dim() != 2 or page_table.dtype is not torch.int32:
+    pages = page_table.shape
+    if len(pages) != 2 or page_table.dtype is not torch.int32:
         raise ConfigError(f"{op}: page_table must be int32 [sequences, pages]")
-    b, width = page_table.shape
+    b, width = pages
     if seq_lens.shape != (b,) or seq_lens.dtype is not torch.int32:
         raise ConfigError(f"{op}: seq_lens must be int32 [{b}]")
     ragged = query_start is not None
@@ -324,15 +336,10 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     if prefix_len and (prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.dtype is not torch.int32
                        or prefix_pages.shape[0] * page < prefix_len):
         raise ConfigError(f"{op}: a prefix of {prefix_len} tokens needs int32 prefix_pages that hold them")
-    if out is None:
-        out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype is not dt or (out.stride(2) != 1 and dim > 1):
-        raise ConfigError(f"{op}: out must be like q, with adjacent columns")
+    out, o0, o1 = _result(op, "out", out, q, shape)
     lse = q.new_empty((t, h), dtype=torch.float32) if return_lse else None
     if t:
-        (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
-        if _overlaps(o0, o1, t, h, dim):
-            raise ConfigError(f"{op}: out's rows overlap")
+        q0, q1, _ = q.stride()
         ld, column = page_table.stride()
         if column != 1 or b <= 1 or ld < width:
             page_table, ld = page_table.contiguous(), width
