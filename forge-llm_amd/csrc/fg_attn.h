@@ -205,7 +205,8 @@ __device__ __forceinline__ s16x8 e4m3_to_16(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(s16x8, make_uint4(w[0], w[1], w[2], w[3]));
 }
 
-// Two fp32 values rounded to nearest even as one packed pair.
+// Two fp32 values rounded to nearest even as one packed pair.  The weights of the second product go through it, since the
+// matrix cores take 16-bit operands: each is off by half a unit in its last place, their sum is of the fp32 values.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
   typedef float f2 __attribute__((ext_vector_type(2)));

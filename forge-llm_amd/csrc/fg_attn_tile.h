@@ -7,8 +7,9 @@
 // e4m3 ones, and heads that do not fill DP columns, pass through registers, where e4m3 becomes 16-bit, once per workgroup.
 //
 // Bound by the matrix products and, beside them, by the vector instructions: per 64 keys and wavefront 32 products (1024
-// cycles) and about 240 others (by the counters), 32 of them exponentials.  A fragment is read from LDS two steps before its product, the
-// exponentials of 16 keys stand between the products of the 16 before, and two workgroups per CU fill each other's waits.
+// cycles) and about 240 others (by the counters), 32 of them exponentials.  A fragment is read from LDS two steps before its
+// product, the exponentials of 16 keys stand between the products of the 16 before, and two workgroups per CU fill each
+// other's waits.
 // Measured on 2048 rows x 8 key heads x 32768 keys of 128 columns: about 265 us, 1.0 PFLOP/s (a large library product: 1.2).  64
 // rows per wavefront, which would halve the LDS reads, needs more than 256 registers and spends what it gains on moves to and
 // from the accumulation registers; through registers instead of straight to LDS a tile costs 10% more.

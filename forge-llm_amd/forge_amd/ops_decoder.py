@@ -65,6 +65,10 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Te
     (``[M]``), ``"fp8_block"`` e4m3 codes with one per 1 x ``block`` columns (``[M, ceil(K / block)]``, the scales of a
     block of columns next to each other, as ``fp8_linear`` reads them fastest): what ``int8_linear`` does to its input,
     and what ``fp8_linear`` takes as ``x`` and ``x_scale``.
+
+    ``ops_gemm.quantize_act_fp8(rms_eps=...)`` norms and quantises per token too, without a residual and with the weight
+    after 1 / rms; here ``h * weight`` comes first, so codes and scales of the two can differ in their last step.  A row
+    whose squares overflow fp32 gives zeros.
     """
     _on_gpu(x, "add_rmsnorm")
     if quant not in _QUANT:
@@ -128,7 +132,7 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Te
 class PagedKVCache:
     """Keys and values of many sequences in pages: ``k`` and ``v`` are ``[pages, kv_heads, page_size, head_dim]`` (any
     strides of whole 16-byte units, the same for both, columns adjacent) in fp16, bf16 or float8_e4m3fn; an e4m3 value
-    stands for ``code * k_scale[head]`` (``v_scale``), fp32 ``[kv_heads]``.  A page holds each key head's tokens next to
+    stands for ``code * k_scale[head]`` (``v_scale``), fp32 ``[kv_heads]``, of any sign.  A page holds each key head's tokens next to
     each other (:meth:`allocate`), the order in which attention reads them.  Rows that share memory, as those of keys expanded
     over heads, can be read but not appended to."""
 
@@ -297,14 +301,15 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     * ``page_table`` int32 ``[B, pages]``, ``seq_lens`` int32 ``[B]``: each sequence's own pages after the prefix, and how many
       tokens they hold, those of the queries included (appended before, with :func:`rope_append`).  Entries past the length,
       and what stands in their slots, are not read;
-    * ``query_start`` int32 ``[B + 1]``: sequence b's queries are tokens ``query_start[b] .. query_start[b + 1]`` of ``q``, and the
-      last of its tokens; ``max_query_len`` bounds their number.  ``None``: one query token per sequence (decoding);
+    * ``query_start`` int32 ``[B + 1]``: sequence b's queries are tokens ``query_start[b] .. query_start[b + 1]`` of ``q`` (offsets
+      outside ``q`` count as its begin or end), and the last of its tokens; ``max_query_len`` bounds their number.  ``None``: one
+      query token per sequence (decoding);
     * ``max_seq_len``: a host bound of ``seq_lens`` (default: what the page table can hold), by which the work is split;
     * ``heads`` is a multiple of the cache's ``kv_heads``; ``scale`` defaults to ``1 / sqrt(dim)``.
 
     Lengths are read on the GPU only.  Scores, softmax and sums are fp32; the probabilities are rounded to ``q``'s type for
-    the product with the values.  A row that sees no token gives zeros (lse -inf), as do query tokens of no sequence.  A
-    query token past ``max_query_len`` gives NaN.  A NaN or infinity in a value that some query token of a sequence sees can
+    the product with the values, which adds about a third to the result's own rounding (fp16 keeps keys down to 2^-32 of the
+    largest weight).  A row that sees no token gives zeros (lse -inf), as do query tokens of no sequence.  A query token past ``max_query_len`` gives NaN.  A NaN or infinity in a value that some query token of a sequence sees can
     show in that sequence's earlier query tokens too.
     """
     op = "prefix_attention"

@@ -312,10 +312,11 @@ int fg_rope_append(const void* q, int64_t q_token, int64_t q_head, const void* k
  * sees the own tokens up to itself; query_start NULL: one query token per sequence (T = B).  Query heads h of key head
  * h / (q_heads / kv_heads).
  *   seq_lens int32 [B] and query_start int32 [B + 1] are device memory; max_seq_len and max_query_len bound them
- *   (longer sequences are cut, later query tokens give NaN); page ids outside the cache stand for no tokens.
+ *   (longer sequences are cut, later query tokens give NaN); offsets outside [0, T] count as 0 or T; page ids outside
+ *   the cache stand for no tokens.
  *   A row that sees no token gives zeros and -inf; so do query tokens of no sequence.
  *   lse (may be NULL): float [T][q_heads], the natural logarithm of the softmax's sum.
- *   workspace: fg_prefix_attention_workspace_bytes bytes, 16-byte aligned. */
+ *   workspace: fg_prefix_attention_workspace_bytes bytes, 16-byte aligned; 0 also for sizes that the call refuses. */
 size_t fg_prefix_attention_workspace_bytes(int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                            int cache_dtype, int64_t prefix_len, int64_t max_seq_len,
                                            int64_t max_query_len, int32_t ragged);
