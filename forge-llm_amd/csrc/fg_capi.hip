@@ -1225,16 +1225,19 @@ int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual
     return fail(FG_EINVAL, "fg_add_rmsnorm: leading dimensions too small");
   if (codes && (s_row < 0 || s_block < 0)) return fail(FG_EINVAL, "fg_add_rmsnorm: bad scale strides");
   if (!fg::norm_fits(M, K)) return hip_status(hipErrorInvalidConfiguration, "fg_add_rmsnorm launch");
-  // an output may stand in an input's place where each element is written by the thread that has read it
+  // an output may stand in an input's place where each element is written by the thread that has read it; y, whose row is written
+  // behind all reads of it, also where that is the only row
   struct Rows {
     const void* p;
     int64_t ld;
     int dt;
   };
-  auto misplaced = [](const Rows& out, const Rows& in) { return out.p && out.p == in.p && (out.ld != in.ld || out.dt != in.dt); };
+  auto misplaced = [M](const Rows& out, const Rows& in) {
+    return out.p && out.p == in.p && ((M > 1 && out.ld != in.ld) || out.dt != in.dt);
+  };
   const Rows xr = {x, ldx, x_dtype}, rr = {residual, ldr, residual_dtype}, yr = {y, ldy, y_dtype};
   const Rows ror = {residual ? residual_out : nullptr, ldro, residual_dtype};
-  if (misplaced(yr, xr) || misplaced(yr, rr) || y == ror.p)
+  if ((M > 1 && (misplaced(yr, xr) || misplaced(yr, rr))) || y == ror.p)
     return fail(FG_EINVAL, "fg_add_rmsnorm: y in the place of rows of another type or stride, or of residual_out");
   if (misplaced(ror, rr) || misplaced(ror, xr))
     return fail(FG_EINVAL, "fg_add_rmsnorm: residual_out in the place of rows of another type or stride");

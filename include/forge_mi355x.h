@@ -287,7 +287,7 @@ typedef struct fg_kv_cache {
  * amax is not > 0), code = y /_IEEE s rounded half to even; the scale of (row, block) at s[row * s_row + b * s_block].
  * residual_dtype: x_dtype or FG_F32.  weight may be NULL.  K <= 32768.
  * residual_out may stand in residual's or x's place, and y, where it is no codes, in x's or residual's: with its type and
- * stride (else, and for y in residual_out's place, FG_EINVAL). */
+ * stride (else, and for y in residual_out's place, FG_EINVAL; one row has no stride, and its y any type). */
 int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual, int64_t ldr, void* residual_out,
                    int64_t ldro, int residual_dtype, const void* weight, int weight_dtype, float eps, void* y,
                    int64_t ldy, int y_dtype, float* s, int64_t s_row, int64_t s_block, int32_t block, int64_t M,

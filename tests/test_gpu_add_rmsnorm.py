@@ -189,3 +189,16 @@ def test_products_past_the_type_in_place():
                                        y.data_ptr(), 777, _lib.BF16, None, 0, 0, 0, 3, 777, _lib.stream_of(y))
     assert status == _lib.OK
     _check(x, None, w, ops.NormOutput(y, None, x), None)
+
+
+def test_one_row_in_the_place_of_its_input():
+    """Codes too, whatever the strides: the row is read before any of it is written."""
+    x, _, w = _data(1, 5001, BF, None)
+    wd = w.to(DEV)
+    for ydt in (_lib.BF16, _lib.I8, _lib.E4M3):
+        y, s = x.to(DEV), torch.zeros(1, device=DEV)
+        status = _lib.lib().fg_add_rmsnorm(y.data_ptr(), 6000, _lib.BF16, None, 0, None, 0, 0, wd.data_ptr(), _lib.BF16, EPS, y.data_ptr(),
+                                           7000, ydt, s.data_ptr(), 1, 0, 0, 1, 5001, _lib.stream_of(y))
+        assert status == _lib.OK
+        raw = y.view(torch.int8 if ydt == _lib.I8 else torch.float8_e4m3fn)[:, :5001] if ydt != _lib.BF16 else y
+        _check(x, None, w, ops.NormOutput(raw, None if ydt == _lib.BF16 else s, x), {_lib.I8: "int8", _lib.E4M3: "fp8"}.get(ydt))
