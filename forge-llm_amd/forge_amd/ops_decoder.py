@@ -132,9 +132,9 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Te
 class PagedKVCache:
     """Keys and values of many sequences in pages: ``k`` and ``v`` are ``[pages, kv_heads, page_size, head_dim]`` (any
     strides of whole 16-byte units, the same for both, columns adjacent) in fp16, bf16 or float8_e4m3fn; an e4m3 value
-    stands for ``code * k_scale[head]`` (``v_scale``), fp32 ``[kv_heads]``, of any sign.  A page holds each key head's tokens next to
-    each other (:meth:`allocate`), the order in which attention reads them.  Rows that share memory, as those of keys expanded
-    over heads, can be read but not appended to."""
+    stands for ``code * k_scale[head]`` (``v_scale``), fp32 ``[kv_heads]``, of any sign.  A page holds each key head's tokens
+    next to each other (:meth:`allocate`), the order in which attention reads them.  Rows that share memory, as those of keys
+    expanded over heads, can be read but not appended to."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -309,8 +309,9 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
 
     Lengths are read on the GPU only.  Scores, softmax and sums are fp32; the probabilities are rounded to ``q``'s type for
     the product with the values, which adds about a third to the result's own rounding (fp16 keeps keys down to 2^-32 of the
-    largest weight).  A row that sees no token gives zeros (lse -inf), as do query tokens of no sequence.  A query token past ``max_query_len`` gives NaN.  A NaN or infinity in a value that some query token of a sequence sees can
-    show in that sequence's earlier query tokens too.
+    largest weight).  A row that sees no token gives zeros (lse -inf), as do query tokens of no sequence.  A query token past
+    ``max_query_len`` gives NaN.  A NaN or infinity in a value that some query token of a sequence sees can show in that
+    sequence's earlier query tokens too.
     """
     op = "prefix_attention"
     _on_gpu(q, op)
