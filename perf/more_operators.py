@@ -1,0 +1,612 @@
+"""Performance cases of what a serving step needs beside its linears in a decoder that norms its blocks on both sides, keeps
+its keys and values in 4 or 8 bits with a power-of-two scale for each 32 columns, caps its scores and draws its tokens.
+
+* ``op = "norm"``: ``ops_decoder.postnorm_add_rmsnorm``, the norm behind a block, its gate and residual scale, the residual's
+  addition, the norm in front of the next block and the 8-bit codes that its linear takes;
+* ``op = "append"``: ``ops_mx.mx_append`` and ``ops_mx.mx_read``, the rotation of queries and keys by positions of one or
+  several axes, the keys' and values' way into a block-scaled cache, and back out of it;
+* ``op = "attention"``: ``ops_mx.mx_attention``, the attention that reads this cache, with a tanh cap and a window;
+* ``op = "sample"``: ``ops_sampling.sample_tokens``, the next tokens from their logits and given random numbers.
+
+Sizes are those of the Llama-3-8B / 70B layers of the benchmark (32 or 64 query heads over 8 key heads of 128, hidden
+sizes 4096 and 8192) and generic ones around them.
+"""
+from __future__ import annotations
+
+import importlib
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False
+
+EPS = 1e-5
+E4M3_MAX = 448.0
+BLOCK = 32  # columns of a cached row that share a scale
+DTYPE = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32, "fp8": torch.float8_e4m3fn}
+ITEM = {"bf16": 2, "fp16": 2, "fp32": 4, "fp8": 1}
+BITS = {"mxfp4": 4, "mxfp8": 8}
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+_MODULES = {}
+
+
+def _package(name: str):
+    if name not in _MODULES:
+        path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "forge-llm_amd")
+        if path not in sys.path:
+            sys.path.insert(0, path)
+        _MODULES[name] = importlib.import_module("forge_amd." + name)
+    return _MODULES[name]
+
+
+# ------------------------------------------------------------------------------------------------------------- cases
+def _norm(m: int, k: int, **kw) -> dict:
+    return {"op": "norm", "m": m, "k": k, "x": "bf16", "residual": "bf16", "quant": "none", "gate": "none",
+            "residual_scale": 1.0, **kw}
+
+
+def _append(tokens: int, heads: int, kv_heads: int, dim: int, **kw) -> dict:
+    return {"op": "append", "tokens": tokens, "heads": heads, "kv_heads": kv_heads, "dim": dim, "rot": dim, "page": 16,
+            "x": "bf16", "cache": "mxfp4", "interleaved": False, "padded": 0, "axes": 1, **kw}
+
+
+def _attention(batch: int, heads: int, kv_heads: int, dim: int, seq_max: int, **kw) -> dict:
+    return {"op": "attention", "batch": batch, "heads": heads, "kv_heads": kv_heads, "dim": dim, "seq_max": seq_max,
+            "query_max": 1, "page": 16, "x": "bf16", "cache": "mxfp4", "softcap": 0.0, "window": 0, "lse": False, **kw}
+
+
+def _sample(rows: int, vocab: int, **kw) -> dict:
+    return {"op": "sample", "rows": rows, "vocab": vocab, "x": "bf16", "top_k": 0, "top_p": 1.0, "min_p": 0.0,
+            "temperature": 1.0, "mixed": False, **kw}
+
+
+def listed() -> list[dict]:
+    cases = [
+        # one token of one sequence between an attention and an INT8 gate+up projection: latency
+        ("norms int8, 1 token", _norm(1, 4096, quant="int8", gate="columns")),
+        # a prompt of no round length, a hidden size off every tile, a gate for each token, 16-bit out
+        ("norms 16-bit, ragged prompt", _norm(1111, 5001, x="fp16", residual="fp32", gate="rows", residual_scale=0.22)),
+        # a long prompt in front of an FP8 linear with 128 x 128 weight blocks
+        ("norms fp8 blocks, long prompt", _norm(8192, 4096, quant="fp8_block")),
+        # a decode batch of 61 sequences padded to a graph's 64 rows, 70B heads
+        ("append fp4, decode batch", _append(64, 64, 8, 128, padded=3)),
+        # a long prompt written into its pages and read back, as for a copy into another pool
+        ("append fp4, long prompt", _append(8192, 32, 8, 128)),
+        # an image between texts: positions of time, height and width, heads of 96, interleaved pairs, fp16
+        ("append fp8, three axes", _append(777, 12, 4, 96, rot=64, page=48, x="fp16", cache="mxfp8", interleaved=True, axes=3)),
+        # one user's chat of some thousand tokens: latency, the cache's length is what there is to split
+        ("attention fp4, 1 sequence", _attention(1, 32, 8, 128, 5000)),
+        # prompts of several hundred tokens, each of its own length, capped scores and a window, fp16
+        ("attention fp8, capped prompts", _attention(4, 16, 8, 256, 3001, query_max=300, x="fp16", cache="mxfp8", softcap=30.0,
+                                                     window=1024, lse=True)),
+        # a decode batch over long contexts: the largest
+        ("attention fp4, 64 sequences", _attention(64, 64, 8, 128, 16384, page=64)),
+        # one row, usual settings: latency
+        ("sample, 1 row", _sample(1, 32000, top_k=50, top_p=0.9, temperature=0.8)),
+        # a batch of requests of one kind: a nucleus without a bound on its tokens
+        ("sample, 32 rows, nucleus", _sample(32, 128000, x="fp32", top_p=0.95)),
+        # a large batch of requests with settings of their own, greedy ones among them, a vocabulary of odd size
+        ("sample, 256 rows, mixed", _sample(256, 150001, x="fp32", mixed=True)),
+    ]
+    return [dict(c, name=name) for name, c in cases]
+
+
+_NORM_MOST, _APPEND_MOST, _SAMPLE_MOST = 8192 * 4096, 8192 * 48 * 128, 256 * 150001
+
+
+def _log(rng: random.Random, lo: int, hi: int) -> int:
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.5)))))))
+
+
+def draw(rng: random.Random) -> dict:
+    op = rng.choice(("norm", "append", "attention", "attention", "sample"))
+    x = rng.choice(("bf16", "bf16", "fp16"))
+    if op == "norm":
+        # hidden sizes of whole 128-column blocks, and in one case of three any
+        k = _log(rng, 500, 16384) if rng.random() < 0.33 else 128 * _log(rng, 4, 128)
+        m = min(_log(rng, 1, 8192), _NORM_MOST // k)
+        x = rng.choice((x, x, x, "fp32"))
+        residual = "fp32" if x == "fp32" else rng.choice((x, x, "fp32"))
+        gate = rng.choice(("none", "columns", "rows"))
+        return _norm(m if gate != "rows" else max(1, m // 2), k, x=x, residual=residual, gate=gate,
+                     quant=rng.choice(("none", "int8", "fp8", "fp8_block")), residual_scale=rng.choice((1.0, 0.5, 1.4)))
+    if op == "sample":
+        vocab = _log(rng, 1000, 200000)
+        rows = min(_log(rng, 1, 512), _SAMPLE_MOST // vocab)
+        return _sample(rows, vocab, x=rng.choice((x, "fp32")), mixed=rng.random() < 0.3, temperature=rng.choice((0.5, 0.8, 1.0, 1.3)),
+                       top_k=rng.choice((0, 0, 20, 50, _log(rng, 1, 1000))), top_p=rng.choice((1.0, 0.5, 0.9, 0.95, 0.99)),
+                       min_p=rng.choice((0.0, 0.0, 0.05, 0.001)))
+    kv_heads, group = rng.choice((1, 2, 4, 8)), rng.choice((1, 2, 3, 4, 4, 6, 8))
+    dim = rng.choice((32, 64, 96, 128, 128, 128, 160, 256))
+    kw = {"page": rng.choice((16, 16, 32, 48, 64, 256)), "x": x, "cache": rng.choice(("mxfp4", "mxfp4", "mxfp8"))}
+    heads = kv_heads * group
+    if op == "append":
+        tokens = min(_log(rng, 1, 8192), _APPEND_MOST // ((heads + 2 * kv_heads) * dim))
+        padded = rng.choice((0, 0, min(3, tokens // 4)))
+        return _append(tokens, heads, kv_heads, dim, rot=rng.choice((dim, dim, dim // 2)), axes=rng.choice((1, 1, 2, 3)),
+                       interleaved=rng.random() < 0.3, padded=padded, **kw)
+    batch = _log(rng, 1, 256)
+    query = 1 if rng.random() < 0.7 else min(_log(rng, 2, 512), max(2, 2048 // batch))
+    seq = max(query, _log(rng, 1, 32768))
+    # lengths that leave the padded 32-bit form its memory and its products
+    seq = max(query, min(seq, (1 << 29) // (batch * kv_heads * dim), (1 << 28) // (batch * query * heads)))
+    return _attention(batch, heads, kv_heads, dim, seq, query_max=query, lse=rng.random() < 0.3,
+                      softcap=rng.choice((0.0, 0.0, 20.0, 50.0)), window=rng.choice((0, 0, _log(rng, 1, 4096))), **kw)
+
+
+# ------------------------------------------------------------------------------------------------------------ inputs
+def _spread(n: int, lo: int, hi: int) -> list[int]:
+    """``n`` lengths between ``lo`` and ``hi``, both among them, evenly spread (which of a batch has which is drawn)."""
+    return [hi] if n == 1 else [lo + (hi - lo) * i // (n - 1) for i in range(n)]
+
+
+def _lengths(case: dict) -> tuple[list[int], list[int]]:
+    """Query tokens and cached tokens of each sequence (the queries' own included), in one order."""
+    b, q, s = case["batch"], case["query_max"], case["seq_max"]
+    queries = _spread(b, 1 if q == 1 else max(1, q // 4), q)
+    return queries, [max(a, c) for a, c in zip(queries, _spread(b, max(1, s // 8), s))]
+
+
+def _sections(case: dict) -> tuple[int, ...]:
+    """The pairs that turn by each axis of the positions."""
+    half, n = case["rot"] // 2, case["axes"]
+    first = half // 4
+    return {1: (half,), 2: (first, half - first), 3: (first, (half - first) // 2, half - first - (half - first) // 2)}[n]
+
+
+def _gen(seed: int) -> torch.Generator:
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def _rand(g, *shape):
+    return torch.rand(*shape, generator=g, device="cuda")
+
+
+class _State:
+    pass
+
+
+def _quantise(x: torch.Tensor, bits: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and block scales of fp32 ``x [..., dim]``.  The scale is 2^(byte - 127) with the smallest byte in 1 .. 254 for which
+    the block's largest magnitude is at most half a step past the largest code; a block with no finite largest magnitude has
+    byte 255 (NaN) and codes of zero.  Codes are the nearest ones, ties to even; 4-bit codes lie in pairs, the even column low."""
+    blocks = x.unflatten(-1, (-1, BLOCK))
+    amax = blocks.abs().amax(-1)
+    fine = torch.isfinite(amax)
+    mantissa, exponent = torch.frexp(torch.where(fine, amax, torch.ones_like(amax)))  # amax = mantissa 2^exponent, 0.5 <= mantissa < 1
+    top, room = (2, 0.875) if bits == 4 else (8, 0.90625)  # 7 / 8; 464 / 512
+    byte = exponent - 1 - top + (mantissa > room).int() + 127
+    byte = torch.where(amax > 0, byte, 1).clamp(1, 254)
+    y = blocks.double() * torch.exp2(127.0 - byte.double()).unsqueeze(-1)  # exact
+    y = torch.where(fine.unsqueeze(-1), y, 0.0)
+    byte = torch.where(fine, byte, 255).to(torch.uint8)
+    if bits == 8:
+        return y.clamp(-E4M3_MAX, E4M3_MAX).float().to(DTYPE["fp8"]).view(torch.uint8).flatten(-2), byte
+    # distances between neighbours: a half up to 2, one up to 4, two up to 6
+    a = y.abs()
+    a = torch.where(a < 2, torch.round(2 * a), torch.where(a < 4, torch.round(a) + 2, torch.round(a / 2) + 4)).clamp(max=7)
+    code = (a.to(torch.uint8) + 8 * torch.signbit(y).to(torch.uint8)).flatten(-2).unflatten(-1, (-1, 2))
+    return code[..., 0] + 16 * code[..., 1], byte
+
+
+def _values(codes: torch.Tensor, scales: torch.Tensor, bits: int) -> torch.Tensor:
+    """The values in 32 bits that codes and block scales stand for."""
+    if bits == 8:
+        v = codes.view(DTYPE["fp8"]).float()
+    else:
+        table = torch.tensor(E2M1 + tuple(-x for x in E2M1), device=codes.device)
+        v = table[torch.stack((codes & 15, codes >> 4), -1).flatten(-2).int()]
+    s = torch.where(scales == 255, math.nan, torch.exp2(scales.float() - 127.0))
+    return (v.unflatten(-1, (-1, BLOCK)) * s.unsqueeze(-1)).flatten(-2)
+
+
+def _cache_tensors(g, case: dict, pages: int) -> tuple:
+    """Codes and block scales of keys and values [pages, key heads, page, ..] as earlier tokens left them."""
+    bits, hk, ps, d = BITS[case["cache"]], case["kv_heads"], case["page"], case["dim"]
+    step = max(1, (1 << 26) // (hk * ps * d))
+    out = []
+    for _ in range(2):
+        codes = torch.empty(pages, hk, ps, d * bits // 8, dtype=torch.uint8, device="cuda")
+        scales = torch.empty(pages, hk, ps, d // BLOCK, dtype=torch.uint8, device="cuda")
+        for i in range(0, pages, step):
+            n = min(step, pages - i)
+            codes[i:i + n], scales[i:i + n] = _quantise(_randn(g, n, hk, ps, d), bits)
+        out += [codes, scales]
+    return out[0], out[2], out[1], out[3]
+
+
+def _inputs(case: dict, seed: int) -> _State:
+    g, st = _gen(seed), _State()
+    st.case = case
+    dt = DTYPE[case["x"]]
+    if case["op"] == "norm":
+        m, k = case["m"], case["k"]
+        st.x = (3 * _randn(g, m, k)).to(dt)
+        # a residual stream: a few columns much larger than the others
+        st.residual = (_randn(g, m, k) * (1 + 20 * (_rand(g, k) < 0.002))).to(DTYPE[case["residual"]])
+        st.post_weight = (0.5 + 0.1 * _randn(g, k)).to(dt)
+        st.weight = (1 + 0.1 * _randn(g, k)).to(dt)
+        st.gate = None if case["gate"] == "none" else (0.5 + 0.2 * _randn(g, *((m, k) if case["gate"] == "rows" else (k,)))).to(dt)
+        return st
+    if case["op"] == "sample":
+        b, v = case["rows"], case["vocab"]
+        # a broad bulk and some tokens far above it
+        logits = 2.5 * _randn(g, b, v)
+        st.logits = (logits - 3 * torch.log(_rand(g, b, v).clamp_min(1e-30)) * (_rand(g, b, v) < 0.0005)).to(dt)
+        st.uniform = _rand(g, b)
+        if case["mixed"]:  # requests with settings of their own; temperature 0 takes the most probable token
+            st.temperature = torch.where(_rand(g, b) < 0.15, 0.0, 0.3 + 1.2 * _rand(g, b))
+            st.top_k = torch.where(_rand(g, b) < 0.4, 0, torch.exp(7 * _rand(g, b)).int()).to(torch.int32)
+            st.top_p = torch.where(_rand(g, b) < 0.3, 1.0, 0.3 + 0.69 * _rand(g, b))
+            st.min_p = torch.where(_rand(g, b) < 0.7, 0.0, 0.1 * _rand(g, b))
+        else:
+            st.temperature, st.top_k, st.top_p, st.min_p = case["temperature"], case["top_k"], case["top_p"], case["min_p"]
+        return st
+    if case["op"] == "append":
+        t, h, hk, d = case["tokens"], case["heads"], case["kv_heads"], case["dim"]
+        need = -(-t // case["page"])
+        pages = need + 2 + need // 8  # other sequences' pages lie around; the last page is nobody's
+        st.qkv = _randn(g, t, (h + 2 * hk) * d).to(dt)
+        st.k, st.v, st.k_scale, st.v_scale = _cache_tensors(g, case, pages)
+        page = torch.randperm(pages - 1, generator=g, device="cuda")
+        i = torch.arange(t, device="cuda")
+        if t <= 64:  # a decode batch: one token for each of many sequences, anywhere in its page
+            slots = torch.randperm((pages - 1) * case["page"], generator=g, device="cuda")[:t]
+            st.positions = torch.randint(0, 8192, (t,), generator=g, device="cuda")
+        else:  # a prompt: its tokens fill pages of its own
+            slots = page[i // case["page"]] * case["page"] + i % case["page"]
+            st.positions = i.clone()
+        if case["axes"] > 1:  # an image's rows and columns count by themselves
+            st.positions = torch.stack([st.positions] + [(st.positions // 7 ** a) % 100 for a in range(case["axes"] - 1)])
+        if case["padded"]:
+            slots[t - case["padded"]:] = -1
+        st.slots = slots
+        st.all_slots = torch.arange(pages * case["page"], device="cuda")
+        angle = torch.arange(8192, device="cuda").view(-1, 1) * torch.pow(
+            torch.tensor(500000.0, device="cuda"), -torch.arange(0, case["rot"], 2, device="cuda") / case["rot"])
+        st.cos_sin = torch.cat((angle.cos(), angle.sin()), 1).contiguous()
+        return st
+    b, h, hk, d, ps = case["batch"], case["heads"], case["kv_heads"], case["dim"], case["page"]
+    queries, lens = _lengths(case)
+    order = torch.randperm(b, generator=torch.Generator().manual_seed(seed)).tolist()
+    queries, lens = [queries[i] for i in order], [lens[i] for i in order]
+    width = -(-case["seq_max"] // ps)
+    counts = [-(-n // ps) for n in lens]
+    pages = sum(counts) + 3
+    st.q = ((4 if case["softcap"] else 2) * _randn(g, sum(queries), h, d)).to(dt)
+    st.k, st.v, st.k_scale, st.v_scale = _cache_tensors(g, case, pages)
+    perm = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    first = torch.tensor([0, *counts], device="cuda").cumsum(0)[:-1].view(-1, 1)
+    column = torch.arange(width, device="cuda")
+    own_page = column < torch.tensor(counts, device="cuda").view(-1, 1)
+    st.page_table = torch.where(own_page, perm[(first + column).clamp(max=pages - 1)], 0).contiguous()
+    st.seq_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    starts = [0]
+    for n in queries:
+        starts.append(starts[-1] + n)
+    st.query_start = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    return st
+
+
+def prepare(case: dict, seed: int) -> _State:
+    st = _inputs(case, seed)
+    if own and case["op"] in ("append", "attention"):  # the handle that a program makes of its cache's tensors
+        st.cache = _package("ops_mx").MXKVCache(st.k, st.v, st.k_scale, st.v_scale)
+    return st
+
+
+# -------------------------------------------------------------------------------------------------------- plain forms
+def _plain_norm(st: _State):
+    case = st.case
+    x = st.x.float()
+    b = x / torch.sqrt((x * x).mean(-1, keepdim=True) + EPS) * st.post_weight.float() * case["residual_scale"]
+    b = b if st.gate is None else b * st.gate.float()
+    res = (st.residual.float() + b).to(st.residual.dtype)
+    h = res.float()
+    y = h / torch.sqrt((h * h).mean(-1, keepdim=True) + EPS) * st.weight.float()
+    if case["quant"] == "none":
+        return {"y": y.to(st.x.dtype), "residual": res}
+    m, k = y.shape
+    block = 128 if case["quant"] == "fp8_block" else k
+    blocks = torch.nn.functional.pad(y, (0, -k % block)).view(m, -1, block)
+    amax = blocks.abs().amax(-1)
+    top = 127.0 if case["quant"] == "int8" else E4M3_MAX
+    scale = torch.where(amax > 0, amax / top, torch.ones_like(amax))
+    q = (blocks / scale.unsqueeze(-1)).clamp(-top, top).view(m, -1)[:, :k]
+    if case["quant"] == "int8":
+        return {"y": (torch.round(q) * scale).to(DTYPE["bf16"]), "residual": res}
+    return {"y": q.to(DTYPE["fp8"]), "scale": scale.view(m) if block == k else scale, "residual": res}
+
+
+def _split_qkv(st: _State):
+    case = st.case
+    h, hk, d = case["heads"], case["kv_heads"], case["dim"]
+    q, k, v = st.qkv.split((h * d, hk * d, hk * d), dim=1)
+    return q.view(-1, h, d), k.view(-1, hk, d), v.view(-1, hk, d)
+
+
+def _angles(st: _State) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cosines and sines [tokens, 1, pairs]: each pair's angle is at its own axis's position."""
+    case, half = st.case, st.case["rot"] // 2
+    if case["axes"] == 1:
+        return st.cos_sin[st.positions].unsqueeze(1).chunk(2, -1)
+    axis = torch.repeat_interleave(torch.arange(case["axes"], device="cuda"), torch.tensor(_sections(case), device="cuda"))
+    position, pair = st.positions[axis].t(), torch.arange(half, device="cuda")
+    return st.cos_sin[position, pair].unsqueeze(1), st.cos_sin[position, half + pair].unsqueeze(1)
+
+
+def _plain_rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool) -> torch.Tensor:
+    # in 64 bits: what is a rounding off may get the other code, or the other scale
+    x, cos, sin = x.double(), cos.double(), sin.double()
+    rot = 2 * cos.shape[-1]
+    r = x[..., :rot]
+    a, b = (r[..., 0::2], r[..., 1::2]) if interleaved else (r[..., :rot // 2], r[..., rot // 2:])
+    u, w = a * cos - b * sin, b * cos + a * sin
+    r = torch.stack((u, w), -1).flatten(-2) if interleaved else torch.cat((u, w), -1)
+    return torch.cat((r, x[..., rot:]), -1).float()
+
+
+def _plain_append(st: _State):
+    case = st.case
+    bits = BITS[case["cache"]]
+    q, k, v = _split_qkv(st)
+    cos, sin = _angles(st)
+    q_rot = _plain_rotate(q, cos, sin, case["interleaved"]).to(q.dtype)
+    # padding writes nobody's page, and what already stands there
+    page, ps = st.k.shape[0] - 1, case["page"]
+    real = st.slots >= 0
+    where = torch.where(real, st.slots // ps, page), torch.where(real, st.slots % ps, 0)
+    new = _quantise(_plain_rotate(k, cos, sin, case["interleaved"]), bits) + _quantise(v.float(), bits)
+    for cache, x in zip((st.k, st.k_scale, st.v, st.v_scale), new):
+        cache[where[0], :, where[1]] = torch.where(real.view(-1, 1, 1), x, cache[page, :, 0])
+    back = [_values(c, s, bits).transpose(1, 2).flatten(0, 1).to(q.dtype) for c, s in ((st.k, st.k_scale), (st.v, st.v_scale))]
+    return {"q": q_rot, "k": back[0], "v": back[1]}
+
+
+def _plain_rows(codes: torch.Tensor, scales: torch.Tensor, pages: torch.Tensor, bits: int) -> torch.Tensor:
+    """[sequences, key heads, tokens, dim] in 32 bits of the pages in ``pages [sequences, n]``."""
+    return _values(codes[pages.long()], scales[pages.long()], bits).transpose(1, 2).flatten(2, 3)
+
+
+def _plain_attention(st: _State):
+    case = st.case
+    b, h, hk, d = case["batch"], case["heads"], case["kv_heads"], case["dim"]
+    g, n, s, bits = h // hk, case["query_max"], case["seq_max"], BITS[case["cache"]]
+    t = st.q.shape[0]
+    # the queries of each sequence in a row of their own, padded to the longest
+    start, count = st.query_start[:-1].long(), (st.query_start[1:] - st.query_start[:-1]).long()
+    i = torch.arange(n, device="cuda")
+    source = (start.view(-1, 1) + i).clamp(max=t - 1)
+    q = st.q.float()[source].view(b, n, hk, g, d).permute(0, 2, 1, 3, 4).reshape(b, hk, n * g, d) / math.sqrt(d)
+    ks = _plain_rows(st.k, st.k_scale, st.page_table, bits)[:, :, :s]
+    last = (st.seq_lens.long() - count).view(-1, 1) + i  # the last token that each query sees
+    key = torch.arange(s, device="cuda")
+    seen = key <= last.view(b, n, 1)
+    if case["window"]:
+        seen = seen & (key > last.view(b, n, 1) - case["window"])
+    seen = seen.view(b, 1, n, 1, s).expand(b, 1, n, g, s).reshape(b, 1, n * g, s)
+    scores = torch.matmul(q, ks.transpose(-1, -2))
+    del ks
+    if case["softcap"]:
+        scores = torch.tanh(scores / case["softcap"]) * case["softcap"]
+    scores = scores.masked_fill(~seen, -math.inf)
+    top = scores.amax(-1, keepdim=True)
+    weights = torch.exp(scores - top)
+    vs = _plain_rows(st.v, st.v_scale, st.page_table, bits)[:, :, :s]
+    total, out = weights.sum(-1, keepdim=True), torch.matmul(weights, vs)
+    out = (out / total).view(b, hk, n, g, d).permute(0, 2, 1, 3, 4).reshape(b, n, h, d)
+    lse = (top + torch.log(total)).view(b, hk, n, g).permute(0, 2, 1, 3).reshape(b, n, h)
+    row = torch.searchsorted(st.query_start[1:].long(), torch.arange(t, device="cuda"), right=True)
+    column = torch.arange(t, device="cuda") - start[row]
+    result = {"out": out[row, column].to(st.q.dtype)}
+    return {**result, "lse": lse[row, column]} if case["lse"] else result
+
+
+def _settings(st: _State) -> tuple[torch.Tensor, ...]:
+    """Temperature, top-k, top-p and min-p of each row; 0 tokens are all."""
+    b, v = st.logits.shape
+    t, k, p, m = (x if isinstance(x, torch.Tensor) else torch.full((b,), x, dtype=torch.int32 if i == 1 else torch.float32, device="cuda")
+                  for i, x in enumerate((st.temperature, st.top_k, st.top_p, st.min_p)))
+    return t.double(), torch.where(k <= 0, v, k.long()), p.double(), m.double()
+
+
+def _plain_sample(st: _State):
+    # in 64 bits: a random number may lie next to the border of two tokens
+    temperature, top_k, top_p, min_p = (x.view(-1, 1) for x in _settings(st))
+    logits = st.logits.double()
+    b, v = logits.shape
+    above = logits - logits.amax(-1, keepdim=True)
+    greedy = temperature <= 0
+    w = torch.exp(above / torch.where(greedy, 1.0, temperature))
+    order = torch.sort(st.logits, dim=-1, descending=True, stable=True)[1]  # equal ones in the order of their indexes
+    ws = w.gather(1, order) * (torch.arange(v, device="cuda") < top_k)
+    before = torch.cat((torch.zeros(b, 1, dtype=torch.float64, device="cuda"), ws.cumsum(-1)), 1)
+    kept = (ws > 0) & ((before[:, :-1] < top_p * before[:, -1:]) | (top_p >= 1)) & (ws >= min_p)
+    w = torch.zeros_like(w).scatter_(1, order, torch.where(kept, ws, 0.0))
+    w = torch.where(greedy, (torch.arange(v, device="cuda") == order[:, :1]).double(), w)
+    sums = w.cumsum(-1)
+    token = (sums <= st.uniform.double().view(-1, 1) * sums[:, -1:]).sum(-1, keepdim=True)
+    logprob = above.gather(1, token) - torch.log(torch.exp(above).sum(-1, keepdim=True))
+    return {"token": token.view(-1), "logprob": logprob.view(-1).float()}
+
+
+# ------------------------------------------------------------------------------------------------------------ the call
+def run(st: _State):
+    case = st.case
+    if not own:
+        return {"norm": _plain_norm, "append": _plain_append, "attention": _plain_attention, "sample": _plain_sample}[case["op"]](st)
+    if case["op"] == "norm":
+        y, scale, res = _package("ops_decoder").postnorm_add_rmsnorm(
+            st.x, st.post_weight, st.residual, st.weight, gate=st.gate, residual_scale=case["residual_scale"], eps=EPS,
+            quant=None if case["quant"] == "none" else case["quant"])
+        if case["quant"] == "none":
+            return {"y": y, "residual": res}
+        if case["quant"] == "int8":  # the values that the codes stand for, as 16-bit numbers
+            values = torch.empty(y.shape, dtype=DTYPE["bf16"], device=y.device)
+            return {"y": torch.mul(y, scale.view(-1, 1), out=values), "residual": res}
+        return {"y": y, "scale": scale, "residual": res}
+    if case["op"] == "sample":
+        token, logprob = _package("ops_sampling").sample_tokens(
+            st.logits, st.uniform, temperature=st.temperature, top_k=st.top_k, top_p=st.top_p, min_p=st.min_p, return_logprobs=True)
+        return {"token": token, "logprob": logprob}
+    ops = _package("ops_mx")
+    if case["op"] == "append":
+        q, k, v = _split_qkv(st)
+        q_rot = ops.mx_append(q, k, v, st.positions, st.cos_sin, st.cache, st.slots, interleaved=case["interleaved"],
+                              sections=_sections(case) if case["axes"] > 1 else None)
+        k, v = ops.mx_read(st.cache, st.all_slots, dtype=q.dtype)
+        return {"q": q_rot, "k": k, "v": v}
+    several = case["query_max"] > 1
+    got = ops.mx_attention(st.q, st.cache, st.page_table, st.seq_lens, query_start=st.query_start if several else None,
+                           max_query_len=case["query_max"], max_seq_len=case["seq_max"], softcap=case["softcap"] or None,
+                           window=case["window"] or None, return_lse=case["lse"])
+    return {"out": got[0], "lse": got[1]} if case["lse"] else {"out": got}
+
+
+# ------------------------------------------------------------------------------------------------ work, exact values
+def work(case: dict) -> dict:
+    item = ITEM[case["x"]]
+    if case["op"] == "norm":
+        m, k = case["m"], case["k"]
+        out = {"none": item, "int8": 1, "fp8": 1, "fp8_block": 1}[case["quant"]]
+        scales = {"none": 0, "int8": 1, "fp8": 1, "fp8_block": -(-k // 128)}[case["quant"]]
+        gate = {"none": 0, "columns": k, "rows": m * k}[case["gate"]]
+        return {"bytes": m * k * (item + 2 * ITEM[case["residual"]] + out) + 4 * m * scales + item * (2 * k + gate), "flops": 14 * m * k}
+    if case["op"] == "sample":
+        b, v = case["rows"], case["vocab"]
+        return {"bytes": b * (v * item + 16 + (16 if case["mixed"] else 0)), "flops": 8 * b * v}
+    h, hk, d, bits = case["heads"], case["kv_heads"], case["dim"], BITS[case["cache"]]
+    row = d * bits // 8 + d // BLOCK
+    if case["op"] == "append":
+        t = case["tokens"]
+        need = -(-t // case["page"])
+        slots = (need + 2 + need // 8) * case["page"]
+        written = (t - case["padded"]) * 2 * hk * row
+        back = slots * (2 * hk * (row + d * item) + 8)
+        return {"bytes": t * ((2 * h + 2 * hk) * d * item + 4 * case["rot"] + 8 * (1 + case["axes"])) + written + back,
+                "flops": 3 * t * (h + hk) * case["rot"] + 4 * t * hk * d}
+    queries, lens = _lengths(case)
+    w = case["window"] or case["seq_max"]
+    cached = sum(min(c, w + a - 1) for a, c in zip(queries, lens))  # what some query token of a sequence sees
+    products = sum(sum(min(c - a + 1 + i, w) for i in range(a)) for a, c in zip(queries, lens))
+    total = 2 * cached * hk * row + 2 * sum(queries) * h * d * item + (4 * sum(queries) * h if case["lse"] else 0)
+    return {"bytes": total + 4 * (-(-cached // case["page"])) + 4 * case["batch"], "flops": 4 * products * h * d}
+
+
+def _exact_codes(x: torch.Tensor, bits: int) -> torch.Tensor:
+    """The values that the nearest codes of ``x`` stand for, by comparison with all of them."""
+    if bits == 4:
+        grid = torch.tensor(E2M1, dtype=torch.float64, device="cuda")
+    else:
+        grid = torch.arange(127, dtype=torch.uint8, device="cuda").view(DTYPE["fp8"]).to(torch.float64)
+    blocks = x.unflatten(-1, (-1, BLOCK))
+    amax = blocks.abs().amax(-1, keepdim=True)
+    most = grid[-1] + (grid[-1] - grid[-2]) / 2
+    e = torch.ceil(torch.log2(amax / most)).clamp_min(-126)  # the smallest power of two that brings amax to `most`
+    e = torch.where(amax > 0, e, -126.0)
+    y = blocks * torch.exp2(-e)
+    middle = (grid[1:] + grid[:-1]) / 2
+    up, down = torch.searchsorted(middle, y.abs(), right=True), torch.searchsorted(middle, y.abs(), right=False)
+    index = torch.where(up % 2 == 0, up, down)  # on a middle, the even code
+    return (torch.sign(y) * grid[index] * torch.exp2(e)).flatten(-2)
+
+
+def exact(case: dict, seed: int):
+    st = _inputs(case, seed)
+    if case["op"] == "norm":
+        x = st.x.double()
+        block = x * torch.rsqrt(x.pow(2).sum(-1, keepdim=True) / case["k"] + EPS) * (st.post_weight.double() * case["residual_scale"])
+        if st.gate is not None:
+            block *= st.gate.double()
+        # the residual is kept, and normed, as its type holds it
+        res = (st.residual.double() + block).to(st.residual.dtype).double()
+        y = res * torch.rsqrt(res.pow(2).sum(-1, keepdim=True) / case["k"] + EPS) * st.weight.double()
+        if case["quant"] == "none":
+            return {"y": y, "residual": res}
+        k, top = case["k"], 127.0 if case["quant"] == "int8" else E4M3_MAX
+        width = 128 if case["quant"] == "fp8_block" else k
+        owner = torch.arange(k, device="cuda") // width
+        amax = torch.zeros(case["m"], -(-k // width), dtype=torch.float64, device="cuda")
+        amax = amax.index_reduce(1, owner, y.abs(), "amax")
+        scale = amax.masked_fill(amax == 0, top) / top
+        q = torch.minimum(torch.maximum(y / scale[:, owner], torch.tensor(-top, device="cuda")), torch.tensor(top, device="cuda"))
+        if case["quant"] == "int8":
+            return {"y": q.round() * scale[:, owner], "residual": res}
+        return {"y": q.float().to(DTYPE["fp8"]).double(), "scale": scale[:, 0] if width == k else scale, "residual": res}
+    if case["op"] == "sample":
+        settings = [x.tolist() for x in _settings(st)]
+        logprob = []
+        for i, row in enumerate(st.logits.double()):  # request by request, over its tokens from the most probable on
+            t, k, p, m = (x[i] for x in settings)
+            values, index = torch.sort(row, descending=True, stable=True)
+            n = 1
+            if t > 0:
+                q = torch.softmax(values[:k] / t, 0)
+                n = min(int((q >= m * q[0]).sum()), q.numel() if p >= 1 else 1 + int((q.cumsum(0)[:-1] < p).sum()))
+                chosen, at = torch.sort(index[:n])
+                q = q[at] / q[:n].sum()
+                n = int((q.cumsum(0) <= float(st.uniform[i].double())).sum())
+                token = chosen[min(n, chosen.numel() - 1)]
+            else:
+                token = index[0]
+            logprob.append(row[token] - torch.logsumexp(row, 0))
+        return {"token": None, "logprob": torch.stack(logprob)}
+    hk, d, ps, bits = case["kv_heads"], case["dim"], case["page"], BITS[case["cache"]]
+    g = case["heads"] // hk
+    if case["op"] == "append":
+        q, k, v = (x.double() for x in _split_qkv(st))
+        half = case["rot"] // 2
+        positions = st.positions.view(case["axes"], -1)
+        table = st.cos_sin.double()
+        turn, at = [], 0
+        for axis, n in enumerate(_sections(case)):  # each pair as a complex number
+            rows = table[positions[axis]]
+            turn.append(torch.complex(rows[:, at:at + n], rows[:, half + at:half + at + n]))
+            at += n
+        turn = torch.cat(turn, 1).unsqueeze(1)
+
+        def rotated(x):
+            r, rest = x[..., :2 * half], x[..., 2 * half:]
+            pair = r.unflatten(-1, (half, 2)) if case["interleaved"] else r.unflatten(-1, (2, half)).transpose(-1, -2)
+            z = torch.view_as_real(torch.view_as_complex(pair.contiguous()) * turn)
+            z = z if case["interleaved"] else z.transpose(-1, -2)
+            return torch.cat((z.flatten(-2), rest), -1)
+
+        out = {"q": rotated(q)}
+        rows = torch.nonzero(st.slots >= 0).flatten()
+        for name, new in (("k", rotated(k)), ("v", v)):
+            cache = _values(getattr(st, name), getattr(st, name + "_scale"), bits).double()
+            flat = cache.permute(0, 2, 1, 3).reshape(-1, hk, d)
+            flat[st.slots[rows]] = _exact_codes(new, bits)[rows]
+            out[name] = flat
+        return out
+    out = torch.empty(st.q.shape, dtype=torch.float64, device="cuda")
+    lse = torch.empty(st.q.shape[:2], dtype=torch.float64, device="cuda")
+    starts, lens = st.query_start.tolist(), st.seq_lens.tolist()
+    for i, n in enumerate(lens):  # sequence by sequence
+        a, c = starts[i], starts[i + 1]
+        pages = st.page_table[i, :-(-n // ps)].long()
+        k, v = (_values(x[pages], s[pages], bits).double().permute(1, 0, 2, 3).reshape(hk, -1, d)[:, :n]
+                for x, s in ((st.k, st.k_scale), (st.v, st.v_scale)))
+        q = st.q[a:c].double().view(c - a, hk, g, d).permute(1, 2, 0, 3).reshape(hk, g * (c - a), d)
+        s = (q @ k.transpose(1, 2)) * d ** -0.5
+        if case["softcap"]:
+            s = case["softcap"] * (1 - 2 / (torch.exp(2 * s / case["softcap"]) + 1))
+        at = n - (c - a) + torch.arange(c - a, device="cuda").view(-1, 1)  # each query's own token
+        j = torch.arange(n, device="cuda").view(1, -1)
+        hidden = (j > at) | ((at - j >= case["window"]) if case["window"] else (j < 0))
+        s = s.view(hk, g, c - a, n).masked_fill(hidden, -math.inf).view(hk, -1, n)
+        z = torch.logsumexp(s, -1)
+        o = torch.exp(s - z.unsqueeze(-1)) @ v
+        out[a:c] = o.view(hk, g, c - a, d).permute(2, 0, 1, 3).reshape(c - a, hk * g, d)
+        lse[a:c] = z.view(hk, g, c - a).permute(2, 0, 1).reshape(c - a, hk * g)
+    return {"out": out, "lse": lse} if case["lse"] else {"out": out}
