@@ -68,30 +68,30 @@ def _sample(rows: int, vocab: int, **kw) -> dict:
 def listed() -> list[dict]:
     cases = [
         # one token of one sequence between an attention and an INT8 gate+up projection: latency
-        ("norms int8, 1 token", _norm(1, 4096, quant="int8", gate="columns")),
+        ("norms int8 1 token", _norm(1, 4096, quant="int8", gate="columns")),
         # a prompt of no round length, a hidden size off every tile, a gate for each token, 16-bit out
-        ("norms 16-bit, ragged prompt", _norm(1111, 5001, x="fp16", residual="fp32", gate="rows", residual_scale=0.22)),
+        ("norms 16-bit ragged prompt", _norm(1111, 5001, x="fp16", residual="fp32", gate="rows", residual_scale=0.22)),
         # a long prompt in front of an FP8 linear with 128 x 128 weight blocks
-        ("norms fp8 blocks, long prompt", _norm(8192, 4096, quant="fp8_block")),
+        ("norms fp8 blocks long prompt", _norm(8192, 4096, quant="fp8_block")),
         # a decode batch of 61 sequences padded to a graph's 64 rows, 70B heads
-        ("append fp4, decode batch", _append(64, 64, 8, 128, padded=3)),
+        ("append fp4 decode batch", _append(64, 64, 8, 128, padded=3)),
         # a long prompt written into its pages and read back, as for a copy into another pool
-        ("append fp4, long prompt", _append(8192, 32, 8, 128)),
+        ("append fp4 long prompt", _append(8192, 32, 8, 128)),
         # an image between texts: positions of time, height and width, heads of 96, interleaved pairs, fp16
-        ("append fp8, three axes", _append(777, 12, 4, 96, rot=64, page=48, x="fp16", cache="mxfp8", interleaved=True, axes=3)),
+        ("append fp8 three axes", _append(777, 12, 4, 96, rot=64, page=48, x="fp16", cache="mxfp8", interleaved=True, axes=3)),
         # one user's chat of some thousand tokens: latency, the cache's length is what there is to split
-        ("attention fp4, 1 sequence", _attention(1, 32, 8, 128, 5000)),
+        ("attention fp4 1 sequence", _attention(1, 32, 8, 128, 5000)),
         # prompts of several hundred tokens, each of its own length, capped scores and a window, fp16
-        ("attention fp8, capped prompts", _attention(4, 16, 8, 256, 3001, query_max=300, x="fp16", cache="mxfp8", softcap=30.0,
+        ("attention fp8 capped prompts", _attention(4, 16, 8, 256, 3001, query_max=300, x="fp16", cache="mxfp8", softcap=30.0,
                                                      window=1024, lse=True)),
         # a decode batch over long contexts: the largest
-        ("attention fp4, 64 sequences", _attention(64, 64, 8, 128, 16384, page=64)),
+        ("attention fp4 64 sequences", _attention(64, 64, 8, 128, 16384, page=64)),
         # one row, usual settings: latency
-        ("sample, 1 row", _sample(1, 32000, top_k=50, top_p=0.9, temperature=0.8)),
+        ("sample 1 row", _sample(1, 32000, top_k=50, top_p=0.9, temperature=0.8)),
         # a batch of requests of one kind: a nucleus without a bound on its tokens
-        ("sample, 32 rows, nucleus", _sample(32, 128000, x="fp32", top_p=0.95)),
+        ("sample 32 rows nucleus", _sample(32, 128000, x="fp32", top_p=0.95)),
         # a large batch of requests with settings of their own, greedy ones among them, a vocabulary of odd size
-        ("sample, 256 rows, mixed", _sample(256, 150001, x="fp32", mixed=True)),
+        ("sample 256 rows mixed", _sample(256, 150001, x="fp32", mixed=True)),
     ]
     return [dict(c, name=name) for name, c in cases]
 
