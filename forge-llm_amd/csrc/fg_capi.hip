@@ -1202,29 +1202,25 @@ int check_cache(const fg_kv_cache* c, int dtype, const char* op) {
   return FG_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual, int64_t ldr, void* residual_out,
-                   int64_t ldro, int residual_dtype, const void* weight, int weight_dtype, float eps, void* y,
-                   int64_t ldy, int y_dtype, float* s, int64_t s_row, int64_t s_block, int32_t block, int64_t M,
-                   int64_t K, fg_stream_t stream) {
-  if (M < 0 || K <= 0 || M >= kMaxDim) return fail(FG_EINVAL, "fg_add_rmsnorm: bad sizes");
-  if (K > fg::kNormMaxK) return fail(FG_EUNSUPPORTED, "fg_add_rmsnorm: rows of more than %d columns", fg::kNormMaxK);
+// The row's part of a norm's arguments into `a`, or a refusal.  M = 0 is no error and leaves `a` as it is.
+int norm_args(const char* op, const void* x, int64_t ldx, int x_dtype, const void* residual, int64_t ldr, void* residual_out,
+              int64_t ldro, int residual_dtype, const void* weight, int weight_dtype, float eps, void* y, int64_t ldy, int y_dtype,
+              float* s, int64_t s_row, int64_t s_block, int32_t block, int64_t M, int64_t K, fg::NormArgs* a) {
+  if (M < 0 || K <= 0 || M >= kMaxDim) return fail(FG_EINVAL, "%s: bad sizes", op);
+  if (K > fg::kNormMaxK) return fail(FG_EUNSUPPORTED, "%s: rows of more than %d columns", op, fg::kNormMaxK);
   if (M == 0) return FG_OK;
   const bool codes = y_dtype == FG_I8 || y_dtype == FG_E4M3;
-  if (!x || !y || (codes && !s) || (residual && !residual_out)) return fail(FG_EINVAL, "fg_add_rmsnorm: null tensor");
-  if (!is_float_dt(x_dtype) || (weight && !is_float_dt(weight_dtype))) return fail(FG_EINVAL, "fg_add_rmsnorm: bad dtype");
+  if (!x || !y || (codes && !s) || (residual && !residual_out)) return fail(FG_EINVAL, "%s: null tensor", op);
+  if (!is_float_dt(x_dtype) || (weight && !is_float_dt(weight_dtype))) return fail(FG_EINVAL, "%s: bad dtype", op);
   if (residual && residual_dtype != x_dtype && residual_dtype != FG_F32)
-    return fail(FG_EINVAL, "fg_add_rmsnorm: the residual is of x's type or fp32");
-  if (!codes && y_dtype != x_dtype) return fail(FG_EINVAL, "fg_add_rmsnorm: y is of x's type, int8 or e4m3");
+    return fail(FG_EINVAL, "%s: the residual is of x's type or fp32", op);
+  if (!codes && y_dtype != x_dtype) return fail(FG_EINVAL, "%s: y is of x's type, int8 or e4m3", op);
   if (block != 0 && (!codes || block < 8 || block > 512 || (block & (block - 1))))
-    return fail(FG_EINVAL, "fg_add_rmsnorm: a block of scales is a power of two from 8 to 512 columns of codes");
+    return fail(FG_EINVAL, "%s: a block of scales is a power of two from 8 to 512 columns of codes", op);
   if (ldx < K || ldy < K || (residual && (ldr < K || ldro < K)))
-    return fail(FG_EINVAL, "fg_add_rmsnorm: leading dimensions too small");
-  if (codes && (s_row < 0 || s_block < 0)) return fail(FG_EINVAL, "fg_add_rmsnorm: bad scale strides");
-  if (!fg::norm_fits(M, K)) return hip_status(hipErrorInvalidConfiguration, "fg_add_rmsnorm launch");
+    return fail(FG_EINVAL, "%s: leading dimensions too small", op);
+  if (codes && (s_row < 0 || s_block < 0)) return fail(FG_EINVAL, "%s: bad scale strides", op);
+  if (!fg::norm_fits(M, K)) return hip_status(hipErrorInvalidConfiguration, op);
   // an output may stand in an input's place where each element is written by the thread that has read it; y, whose row is written
   // behind all reads of it, also where that is the only row
   struct Rows {
@@ -1238,16 +1234,50 @@ int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual
   const Rows xr = {x, ldx, x_dtype}, rr = {residual, ldr, residual_dtype}, yr = {y, ldy, y_dtype};
   const Rows ror = {residual ? residual_out : nullptr, ldro, residual_dtype};
   if ((M > 1 && (misplaced(yr, xr) || misplaced(yr, rr))) || y == ror.p)
-    return fail(FG_EINVAL, "fg_add_rmsnorm: y in the place of rows of another type or stride, or of residual_out");
+    return fail(FG_EINVAL, "%s: y in the place of rows of another type or stride, or of residual_out", op);
   if (misplaced(ror, rr) || misplaced(ror, xr))
-    return fail(FG_EINVAL, "fg_add_rmsnorm: residual_out in the place of rows of another type or stride");
+    return fail(FG_EINVAL, "%s: residual_out in the place of rows of another type or stride", op);
+  a->x = x; a->ldx = ldx; a->r = residual; a->ldr = ldr; a->ro = residual_out; a->ldro = ldro;
+  a->w = weight; a->wdt = weight_dtype; a->eps = eps; a->y = y; a->ldy = ldy; a->ydt = y_dtype;
+  a->s = s; a->s_row = s_row; a->s_block = s_block; a->log_l = block ? __builtin_ctz((unsigned)block) - 3 : -1;
+  a->K = (int)K;
+  return FG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual, int64_t ldr, void* residual_out,
+                   int64_t ldro, int residual_dtype, const void* weight, int weight_dtype, float eps, void* y,
+                   int64_t ldy, int y_dtype, float* s, int64_t s_row, int64_t s_block, int32_t block, int64_t M,
+                   int64_t K, fg_stream_t stream) {
   fg::NormArgs a;
-  a.x = x; a.ldx = ldx; a.r = residual; a.ldr = ldr; a.ro = residual_out; a.ldro = ldro;
-  a.w = weight; a.wdt = weight_dtype; a.eps = eps; a.y = y; a.ldy = ldy; a.ydt = y_dtype;
-  a.s = s; a.s_row = s_row; a.s_block = s_block; a.log_l = block ? __builtin_ctz((unsigned)block) - 3 : -1;
-  a.K = (int)K;
+  const int bad = norm_args("fg_add_rmsnorm", x, ldx, x_dtype, residual, ldr, residual_out, ldro, residual_dtype, weight, weight_dtype,
+                            eps, y, ldy, y_dtype, s, s_row, s_block, block, M, K, &a);
+  if (bad || M == 0) return bad;
   return hip_status(fg::launch_add_rmsnorm(a, x_dtype, residual_dtype, M, static_cast<hipStream_t>(stream)),
                     "fg_add_rmsnorm launch");
+}
+
+int fg_postnorm_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* post_weight, int post_weight_dtype,
+                            const void* gate, int64_t ldg, int gate_dtype, float residual_scale, float post_eps,
+                            const void* residual, int64_t ldr, void* residual_out, int64_t ldro, int residual_dtype,
+                            const void* weight, int weight_dtype, float eps, void* y, int64_t ldy, int y_dtype, float* s,
+                            int64_t s_row, int64_t s_block, int32_t block, int64_t M, int64_t K, fg_stream_t stream) {
+  static const char* const op = "fg_postnorm_add_rmsnorm";
+  fg::PostNormArgs p;
+  const int bad = norm_args(op, x, ldx, x_dtype, residual, ldr, residual_out, ldro, residual_dtype, weight, weight_dtype, eps, y, ldy,
+                            y_dtype, s, s_row, s_block, block, M, K, &p.norm);
+  if (bad || M == 0) return bad;
+  if (!residual) return fail(FG_EINVAL, "%s: null tensor", op);
+  if ((post_weight && !is_float_dt(post_weight_dtype)) || (gate && !is_float_dt(gate_dtype))) return fail(FG_EINVAL, "%s: bad dtype", op);
+  if (gate && ldg != 0 && ldg < K) return fail(FG_EINVAL, "%s: leading dimensions too small", op);
+  if (gate && (gate == y || gate == residual_out)) return fail(FG_EINVAL, "%s: an output in the gate's place", op);
+  p.pw = post_weight; p.pwdt = post_weight_dtype; p.gate = gate; p.ldg = ldg; p.gdt = gate_dtype;
+  p.scale = residual_scale; p.eps_post = post_eps;
+  return hip_status(fg::launch_postnorm_add_rmsnorm(p, x_dtype, residual_dtype, M, static_cast<hipStream_t>(stream)),
+                    "fg_postnorm_add_rmsnorm launch");
 }
 
 int fg_rope_append(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,

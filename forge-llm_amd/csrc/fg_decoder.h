@@ -29,6 +29,16 @@ struct NormArgs {
   int K;
 };
 
+struct PostNormArgs {
+  NormArgs norm;   // of the residual's sum; x is the block's output
+  const void* pw;  // the weight of the block's norm
+  int pwdt;
+  const void* gate;  // a row for each row of x (ldg) or, with ldg = 0, one for all
+  int64_t ldg;
+  int gdt;
+  float scale, eps_post;
+};
+
 struct RopeAppendArgs {
   const uint16_t *q, *k, *v;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h;  // element strides of tokens and heads
@@ -48,7 +58,9 @@ struct RopeAppendArgs {
   int Hq, Hk, D, rot;
 };
 
+int norm_plan(int64_t M, int64_t K, int* C);  // threads per row; units of 8 columns per thread
 bool norm_fits(int64_t M, int64_t K);  // whether one launch takes M rows of K columns
+hipError_t launch_postnorm_add_rmsnorm(const PostNormArgs& p, int xdt, int rdt, int64_t M, hipStream_t st);
 hipError_t launch_add_rmsnorm(const NormArgs& a, int xdt, int rdt, int64_t M, hipStream_t st);
 hipError_t launch_rope_append(const RopeAppendArgs& a, int64_t T, bool bf16, bool fp8, bool inter, hipStream_t st);
 

@@ -90,6 +90,8 @@ SIGNATURES = {
     # a cache goes as the address of a KVCache
     "fg_add_rmsnorm": ([P, I64, INT, P, I64, P, I64, INT, P, INT, F32_, P, I64, INT, P, I64, I64, I32_, I64, I64, P],
                        INT),
+    "fg_postnorm_add_rmsnorm": ([P, I64, INT, P, INT, P, I64, INT, F32_, F32_, P, I64, P, I64, INT, P, INT, F32_, P, I64, INT,
+                                 P, I64, I64, I32_, I64, I64, P], INT),
     "fg_rope_append": ([P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, INT, P, I32_, P, I64, I64, I32_, I32_, P,
                         I32_, P, I64, I32_, P], INT),
     "fg_prefix_attention_workspace_bytes": ([I64, I64, I32_, I32_, I32_, INT, I64, I64, I64, I32_], SZ),

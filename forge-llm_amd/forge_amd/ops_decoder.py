@@ -2,6 +2,7 @@
 
 * :func:`add_rmsnorm`: the residual's addition, the RMSNorm and, if asked for, the 8-bit codes and scales that
   ``ops_gemm.int8_linear`` / ``fp8_linear`` take;
+* :func:`postnorm_add_rmsnorm`: the same behind a norm of the block's output, its gate and its residual scale;
 * :func:`rope_append`: the rotation of a projection's queries and keys by their positions, and the keys' and values' way
   into a :class:`PagedKVCache`;
 * :func:`prefix_attention`: the attention that reads this cache, for a batch whose sequences share a prefix.
@@ -125,6 +126,86 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Te
             _check(status, "fg_add_rmsnorm")
     _done("add_rmsnorm")
     return NormOutput(y if x2 is x else y.view(shape), scale, x if residual is None else residual_out)
+
+
+def _factor(op: str, name: str, t: torch.Tensor | None, k: int) -> tuple[torch.Tensor | None, int]:
+    """A row of ``k`` factors in any float type, and its type's code."""
+    if t is None:
+        return None, 0
+    if t.shape != (k,) or t.dtype not in _FLOATS:
+        raise ConfigError(f"{op}: {name} must be an fp32, fp16 or bf16 tensor of [{k}]")
+    return t if t.is_contiguous() else t.contiguous(), _CODE[t.dtype]
+
+
+def postnorm_add_rmsnorm(x: torch.Tensor, post_weight: torch.Tensor | None, residual: torch.Tensor, weight: torch.Tensor | None, *,
+                         gate: torch.Tensor | None = None, residual_scale: float = 1.0, eps: float = 1e-5,
+                         post_eps: float | None = None, quant: str | None = None, block: int = 128,
+                         residual_out: torch.Tensor | None = None) -> NormOutput:
+    """The step between two blocks of a decoder that norms a block's output ``x`` as well as the next block's input, in one pass:
+    ``h = residual + x / sqrt(mean(x^2) + post_eps) * post_weight * residual_scale * gate``, then :func:`add_rmsnorm`'s ``y`` (and
+    codes) of ``h`` with ``weight`` and ``eps``.
+
+    ``gate``: ``[K]``, or one for each row in ``x``'s shape (expanded from fewer, if need be), in any float type; ``post_eps``
+    defaults to ``eps``.  ``residual`` (``x``'s shape, ``x``'s type or fp32), ``residual_out``, ``quant``, ``block`` and the result
+    are those of :func:`add_rmsnorm`.  What is added is fp32, ``h`` is rounded once.  A row whose squares overflow fp32 norms to
+    zeros.
+    """
+    op = "postnorm_add_rmsnorm"
+    _on_gpu(x, op)
+    if quant not in _QUANT:
+        raise ConfigError(f"{op}: unknown quant {quant!r}: use None, int8, fp8 or fp8_block")
+    xdt, shape = x.dtype, x.shape
+    if xdt not in _FLOATS:
+        raise ConfigError(f"{op}: x must be an fp32, fp16 or bf16 tensor")
+    if not shape:
+        raise ConfigError(f"{op}: x needs a last dimension to norm")
+    k = shape[-1]
+    _elsewhere(op, x, post_weight, residual, weight, gate, residual_out)
+    (post_weight, pdt), (weight, wdt) = _factor(op, "post_weight", post_weight, k), _factor(op, "weight", weight, k)
+    x2, ldx = _rows(x, k)
+    m = x2.shape[0]
+    rdt = residual.dtype
+    if residual.shape != shape or (rdt is not xdt and rdt is not torch.float32):
+        raise ConfigError(f"{op}: residual must have x's shape and x's type or fp32")
+    r2, ldr = _rows(residual, k)
+    g2, ldg, gdt = None, 0, 0
+    if gate is not None:
+        if gate.dtype not in _FLOATS or (gate.shape != shape and gate.shape != (k,)):
+            raise ConfigError(f"{op}: gate must be an fp32, fp16 or bf16 tensor of [{k}] or of x's shape")
+        gdt = _CODE[gate.dtype]
+        if gate.shape != shape or (gate.dim() == 2 and gate.stride() == (0, 1)):
+            g2 = gate if gate.stride(-1) == 1 else gate.contiguous()
+        else:
+            g2, ldg = _rows(gate, k)
+    if residual_out is None:
+        residual_out = ro2 = residual.new_empty(shape)
+        ldro = k
+    elif residual_out.shape != shape or residual_out.dtype is not rdt:
+        raise ConfigError(f"{op}: residual_out must be like residual")
+    else:
+        ro2, ldro = _rows(residual_out, k)
+        if m and ro2.data_ptr() != residual_out.data_ptr():
+            raise ConfigError(f"{op}: residual_out must be rows of adjacent columns that do not overlap")
+    ydt = _QUANT[quant] or xdt
+    y = x.new_empty((m, k), dtype=ydt)
+    scale, s_row, s_block = None, 0, 0
+    if quant == "fp8_block":
+        if block < 8 or block > 512 or block & (block - 1):
+            raise ConfigError(f"{op}: block is a power of two from 8 to 512")
+        scale = x.new_empty((-(-k // block), m), dtype=torch.float32).t()
+        s_row, s_block = 1, max(m, 1)
+    elif quant is not None:
+        scale, s_row = x.new_empty((m,), dtype=torch.float32), 1
+    if m and k:
+        status = _lib.lib().fg_postnorm_add_rmsnorm(
+            x2.data_ptr(), ldx, _CODE[xdt], _lib.ptr(post_weight), pdt, _lib.ptr(g2), ldg, gdt, residual_scale,
+            eps if post_eps is None else post_eps, r2.data_ptr(), ldr, ro2.data_ptr(), ldro, _CODE[rdt], _lib.ptr(weight), wdt, eps,
+            y.data_ptr(), k, _CODE[ydt], _lib.ptr(scale), s_row, s_block, block if quant == "fp8_block" else 0, m, k,
+            _lib.stream_of(x2))
+        if status:
+            _check(status, "fg_postnorm_add_rmsnorm")
+    _done(op)
+    return NormOutput(y if x2 is x else y.view(shape), scale, residual_out)
 
 
 # ================================================================================================ paged cache

@@ -293,6 +293,18 @@ int fg_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* residual
                    int64_t ldy, int y_dtype, float* s, int64_t s_row, int64_t s_block, int32_t block, int64_t M,
                    int64_t K, fg_stream_t stream);
 
+/* The step between two blocks whose outputs are normed too, in one pass:
+ *   b = x / sqrt(mean(x^2) + post_eps) * post_weight * residual_scale * gate in fp32 (in this order),
+ *   h = residual + b, rounded to residual_dtype and written to residual_out, y of h as in fg_add_rmsnorm.
+ * post_weight, gate and weight may be NULL (ones); gate has a row of K columns for each row of x at gate + row * ldg, or with
+ * ldg = 0 one for all, and is no output's place.  A row whose squares pass fp32's range norms to zeros.  The other arguments are
+ * those of fg_add_rmsnorm; residual is not NULL. */
+int fg_postnorm_add_rmsnorm(const void* x, int64_t ldx, int x_dtype, const void* post_weight, int post_weight_dtype,
+                            const void* gate, int64_t ldg, int gate_dtype, float residual_scale, float post_eps,
+                            const void* residual, int64_t ldr, void* residual_out, int64_t ldro, int residual_dtype,
+                            const void* weight, int weight_dtype, float eps, void* y, int64_t ldy, int y_dtype, float* s,
+                            int64_t s_row, int64_t s_block, int32_t block, int64_t M, int64_t K, fg_stream_t stream);
+
 /* Rotary embedding and cache append of T tokens: q [T][q_heads][head_dim], k and v [T][kv_heads][head_dim] (dtype
  * FG_F16 | FG_BF16, element strides of tokens and heads, columns adjacent).  Columns (i, i + rot / 2), or (2 i, 2 i + 1)
  * with interleaved, i < rot / 2, turn by the angle whose cosine is table[pos * ld_table + i] and sine
