@@ -13,6 +13,7 @@
 #include "../../include/forge_mi355x.h"
 #include "fg_attn.h"
 #include "fg_decoder.h"
+#include "fg_mx.h"
 #include "fg_device.h"
 
 namespace fg {
@@ -1391,6 +1392,97 @@ int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtyp
   return hip_status(fg::launch_attn(a, dtype == FG_BF16, cache->dtype == FG_E4M3, workspace, need,
                                     static_cast<hipStream_t>(stream)),
                     "fg_prefix_attention launch");
+}
+
+}  // extern "C"
+
+namespace {
+
+// `cache` as the kernels take it, or a refusal.
+int check_mx(const fg_mx_cache* c, const char* op, fg::MxCache* to) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return fail(FG_EINVAL, "%s: null cache", op);
+  if (c->num_pages <= 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->head_dim <= 0 || c->num_pages >= kMaxDim)
+    return fail(FG_EINVAL, "%s: bad cache sizes", op);
+  if (c->bits != 4 && c->bits != 8) return fail(FG_EINVAL, "%s: a block-scaled cache has 4 or 8 bits", op);
+  if (c->head_dim > 256 || c->head_dim % fg::kMxBlock)
+    return fail(FG_EUNSUPPORTED, "%s: head_dim %d is not a multiple of %d up to 256", op, c->head_dim, fg::kMxBlock);
+  const int64_t strides[3] = {c->page_stride, c->head_stride, c->token_stride}, row = (int64_t)c->head_dim * c->bits / 8;
+  for (int64_t s : strides)
+    if (s < 0 || s % (4 * c->bits)) return fail(FG_EINVAL, "%s: cache strides are no whole blocks", op);
+  if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
+    return fail(FG_EINVAL, "%s: the cache is not 16-byte aligned", op);
+  // rows are 32-bit numbers of 16-byte units
+  const double span = ((double)(c->num_pages - 1) * c->page_stride + (double)(c->page_size - 1) * c->token_stride) / 16;
+  if (span >= 4294967295.0) return fail(FG_EUNSUPPORTED, "%s: the pages of one head span 64 GiB or more", op);
+  if (rows_overlap({c->page_stride, c->num_pages}, {c->head_stride, c->kv_heads}, {c->token_stride, c->page_size}, row))
+    return fail(FG_EINVAL, "%s: the cache's rows overlap", op);
+  to->k = static_cast<uint8_t*>(c->k); to->v = static_cast<uint8_t*>(c->v);
+  to->ks = static_cast<uint8_t*>(c->k_scale); to->vs = static_cast<uint8_t*>(c->v_scale);
+  to->page = c->page_stride; to->head = c->head_stride; to->token = c->token_stride;
+  to->n_slots = c->num_pages * c->page_size; to->page_size = c->page_size; to->Hk = c->kv_heads; to->D = c->head_dim;
+  return FG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fg_mx_append(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                 const void* v, int64_t v_token, int64_t v_head, void* q_out, int64_t qo_token, int64_t qo_head, int dtype,
+                 const void* positions, int32_t positions_int64, int64_t ld_positions, int32_t axes, const int32_t* sections,
+                 const float* table, int64_t ld_table, int64_t max_pos, int32_t rot, int32_t interleaved,
+                 const void* slots, int32_t slots_int64, const fg_mx_cache* cache, int64_t T, int32_t q_heads,
+                 fg_stream_t stream) {
+  static const char* const op = "fg_mx_append";
+  if (T < 0 || T >= kMaxDim || q_heads <= 0 || q_heads >= kMaxDim / 2 || max_pos < 0) return fail(FG_EINVAL, "%s: bad sizes", op);
+  if (T == 0) return FG_OK;
+  if (dtype != FG_F16 && dtype != FG_BF16) return fail(FG_EINVAL, "%s: q, k and v are fp16 or bf16", op);
+  fg::MxAppendArgs a = {};
+  const int bad = check_mx(cache, op, &a.cache);
+  if (bad) return bad;
+  if (cache->kv_heads >= kMaxDim / 4) return fail(FG_EINVAL, "%s: bad sizes", op);
+  if (rows_overlap({qo_token, T}, {qo_head, q_heads}, {0, 1}, cache->head_dim))
+    return fail(FG_EINVAL, "%s: q_out's rows overlap", op);
+  if (q_out == q && ((T > 1 && qo_token != q_token) || (q_heads > 1 && qo_head != q_head)))
+    return fail(FG_EINVAL, "%s: q_out in the place of q's rows with other strides", op);
+  if (!q || !k || !v || !q_out || !positions || !table || !slots) return fail(FG_EINVAL, "%s: null tensor", op);
+  if (rot < 2 || rot % 2 || rot > cache->head_dim || ld_table < rot)
+    return fail(FG_EINVAL, "%s: rot is even, at most head_dim and at most the table's columns", op);
+  if (axes < 1 || axes > fg::kMxAxes || (axes > 1 && (!sections || ld_positions < T)))
+    return fail(FG_EINVAL, "%s: positions have 1 to %d axes, several with their sections", op, fg::kMxAxes);
+  int64_t pairs = 0;
+  for (int i = 0; i < axes; ++i) {
+    const int64_t n = sections ? sections[i] : rot / 2;
+    if (n < 0) return fail(FG_EINVAL, "%s: a section of less than no pairs", op);
+    pairs += n;
+    a.ends[i] = (int)std::min<int64_t>(pairs, rot);
+  }
+  if (pairs != rot / 2) return fail(FG_EINVAL, "%s: the sections have %lld of %d pairs", op, (long long)pairs, rot / 2);
+  a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k); a.v = static_cast<const uint16_t*>(v);
+  a.q_t = q_token; a.q_h = q_head; a.k_t = k_token; a.k_h = k_head; a.v_t = v_token; a.v_h = v_head;
+  a.qo = static_cast<uint16_t*>(q_out); a.qo_t = qo_token; a.qo_h = qo_head;
+  a.pos = positions; a.pos64 = positions_int64; a.ld_pos = ld_positions; a.axes = axes;
+  a.table = table; a.ld_table = ld_table; a.max_pos = max_pos; a.slots = slots; a.slots64 = slots_int64;
+  a.Hq = q_heads; a.rot = rot;
+  return hip_status(fg::launch_mx_append(a, T, dtype == FG_BF16, cache->bits, interleaved != 0, static_cast<hipStream_t>(stream)),
+                    "fg_mx_append launch");
+}
+
+int fg_mx_read(const fg_mx_cache* cache, const void* slots, int32_t slots_int64, void* k_out, void* v_out, int dtype,
+               int64_t n, fg_stream_t stream) {
+  static const char* const op = "fg_mx_read";
+  if (n < 0 || n >= kMaxDim) return fail(FG_EINVAL, "%s: bad sizes", op);
+  if (n == 0) return FG_OK;
+  fg::MxReadArgs a = {};
+  const int bad = check_mx(cache, op, &a.cache);
+  if (bad) return bad;
+  if (dtype != FG_F16 && dtype != FG_BF16) return fail(FG_EINVAL, "%s: the values are fp16 or bf16", op);
+  if (!slots || !k_out || !v_out) return fail(FG_EINVAL, "%s: null tensor", op);
+  if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16)
+    return fail(FG_EINVAL, "%s: the results are not 16-byte aligned", op);
+  if (cache->kv_heads >= kMaxDim / 64) return fail(FG_EINVAL, "%s: bad sizes", op);
+  a.slots = slots; a.slots64 = slots_int64; a.ko = static_cast<uint16_t*>(k_out); a.vo = static_cast<uint16_t*>(v_out); a.n = n;
+  return hip_status(fg::launch_mx_read(a, dtype == FG_BF16, cache->bits, static_cast<hipStream_t>(stream)), "fg_mx_read launch");
 }
 
 }  // extern "C"

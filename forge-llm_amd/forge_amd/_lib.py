@@ -62,6 +62,13 @@ class KVCache(ctypes.Structure):
                 ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
 
 
+class MXCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64), ("num_pages", ctypes.c_int64), ("bits", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
 P, I64, I32_, INT, SZ, F32_ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 
 SIGNATURES = {
@@ -97,6 +104,10 @@ SIGNATURES = {
     "fg_prefix_attention_workspace_bytes": ([I64, I64, I32_, I32_, I32_, INT, I64, I64, I64, I32_], SZ),
     "fg_prefix_attention": ([P, I64, I64, INT, P, P, I64, P, I64, P, P, I64, I64, I32_, I64, I64, F32_, P, I64, I64, P,
                              P, SZ, P], INT),
+    # a block-scaled cache goes as the address of an MXCache
+    "fg_mx_append": ([P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, INT, P, I32_, I64, I32_, P, P, I64, I64, I32_, I32_,
+                      P, I32_, P, I64, I32_, P], INT),
+    "fg_mx_read": ([P, P, I32_, P, P, INT, I64, P], INT),
     "fg_version": ([], ctypes.c_char_p),
     "fg_last_error": ([], ctypes.c_char_p),
     "fg_last_kernel": ([], ctypes.c_char_p),

@@ -339,6 +339,44 @@ int fg_prefix_attention(const void* q, int64_t q_token, int64_t q_head, int dtyp
                         int64_t o_head, float* lse, void* workspace, size_t workspace_bytes, fg_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
+ * A paged cache in 4 or 8 bits with a power-of-two scale for each 32 columns (OCP microscaling formats: e2m1 or e4m3
+ * elements, e8m0 scales), the way into it and back out of it.  bits is 4 or 8; head_dim a multiple of 32 up to 256.
+ * The codes of (page, head, token) are the head_dim * bits / 8 bytes at page * page_stride + head * head_stride +
+ * token * token_stride of k and of v (bytes; 4-bit codes in pairs, the even column low), their head_dim / 32 scale
+ * bytes at the same place divided by 4 * bits of k_scale and v_scale: byte b stands for 2^(b - 127), 255 for NaN.
+ * k and v are 16-byte aligned, strides are multiples of 4 * bits bytes, and the rows lie apart.
+ *
+ * A block's scale is the smallest power of two from 2^-126 on that brings its largest magnitude to half a step past the
+ * largest code at most (7 in e2m1, 464 in e4m3); codes are the nearest ones, ties to even.  A block with a NaN or an
+ * infinity has byte 255 and codes of zero.
+ * ------------------------------------------------------------------------------------------------------------- */
+typedef struct fg_mx_cache {
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  int64_t page_stride, head_stride, token_stride;
+  int64_t num_pages;
+  int32_t bits, kv_heads, page_size, head_dim;
+} fg_mx_cache;
+
+/* Rotary embedding and cache append of T tokens, as fg_rope_append, with positions of several axes: pair i turns by
+ * positions[a * ld_positions + token], where axis a has the sections[a] pairs behind those of the axes before it (host
+ * memory; sections[0] + .. = rot / 2, each 0 or more; axes from 1 to 4; with one axis sections may be NULL).  Queries
+ * are rotated in fp32; keys with one rounding to fp32, from which their codes are made, as the values' are from them. */
+int fg_mx_append(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                 const void* v, int64_t v_token, int64_t v_head, void* q_out, int64_t qo_token, int64_t qo_head, int dtype,
+                 const void* positions, int32_t positions_int64, int64_t ld_positions, int32_t axes, const int32_t* sections,
+                 const float* table, int64_t ld_table, int64_t max_pos, int32_t rot, int32_t interleaved,
+                 const void* slots, int32_t slots_int64, const fg_mx_cache* cache, int64_t T, int32_t q_heads,
+                 fg_stream_t stream);
+
+/* The keys and values of n slots (page * page_size + token; int32 or int64) as k_out and v_out [n][kv_heads][head_dim], adjacent,
+ * 16-byte aligned, in dtype FG_F16 | FG_BF16: exact where the type can hold the value.  A slot outside the cache gives zeros. */
+int fg_mx_read(const fg_mx_cache* cache, const void* slots, int32_t slots_int64, void* k_out, void* v_out, int dtype,
+               int64_t n, fg_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
  * Library information.  fg_device_ok replaces the capability gate triton_usable (forge/kernels/ops_gemm.py:159-175):
  * returns 1 when `device` is a gfx950 GPU this build can run on, else 0 (message in fg_last_error).
  * ------------------------------------------------------------------------------------------------------------- */
