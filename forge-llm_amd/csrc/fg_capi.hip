@@ -13,8 +13,8 @@
 #include "../../include/forge_mi355x.h"
 #include "fg_attn.h"
 #include "fg_decoder.h"
-#include "fg_mx.h"
 #include "fg_device.h"
+#include "fg_mx_attn.h"
 
 namespace fg {
 hipError_t launch_w4_gemv(int mt, int R, bool xbf16, const void* x, int64_t ldx, const int32_t* qw, int64_t ldq,
@@ -1483,6 +1483,72 @@ int fg_mx_read(const fg_mx_cache* cache, const void* slots, int32_t slots_int64,
   if (cache->kv_heads >= kMaxDim / 64) return fail(FG_EINVAL, "%s: bad sizes", op);
   a.slots = slots; a.slots64 = slots_int64; a.ko = static_cast<uint16_t*>(k_out); a.vo = static_cast<uint16_t*>(v_out); a.n = n;
   return hip_status(fg::launch_mx_read(a, dtype == FG_BF16, cache->bits, static_cast<hipStream_t>(stream)), "fg_mx_read launch");
+}
+
+}  // extern "C"
+
+namespace {
+
+// The sizes of an attention call over a block-scaled cache into `m`; a message for sizes that no plan is made for.
+const char* mx_attn_sizes(fg::MxAttnArgs& m, int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t bits,
+                          int64_t max_seq_len, int64_t max_query_len, int64_t window, bool ragged) {
+  if (const char* why = attn_sizes(m.a, T, B, q_heads, kv_heads, head_dim, 0, max_seq_len, max_query_len, ragged, 1)) return why;
+  if (window < 0) return "bad sizes";
+  if (T * q_heads >= fg::kNoWindow) return "sizes past 32 bits";
+  m.bits = bits;
+  m.window = window == 0 || window >= fg::kNoWindow ? fg::kNoWindow : (int)window;
+  return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fg_mx_attention_workspace_bytes(int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t bits,
+                                       int64_t max_seq_len, int64_t max_query_len, int64_t window, int32_t ragged) {
+  fg::MxAttnArgs m = {};
+  if (mx_attn_sizes(m, T, B, q_heads, kv_heads, head_dim, bits, max_seq_len, max_query_len, window, ragged != 0)) return 0;
+  if (T == 0) return 0;
+  const size_t need = fg::mx_attn_plan(m);
+  return m.a.items < 0 ? 0 : need;  // a plan that the call refuses takes no memory
+}
+
+int fg_mx_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const fg_mx_cache* cache,
+                    const int32_t* page_table, int64_t ld_pages, const int32_t* seq_lens, const int32_t* query_start,
+                    int64_t T, int64_t B, int32_t q_heads, int64_t max_seq_len, int64_t max_query_len, float scale,
+                    float softcap, int64_t window, void* out, int64_t o_token, int64_t o_head, float* lse, void* workspace,
+                    size_t workspace_bytes, fg_stream_t stream) {
+  static const char* const op = "fg_mx_attention";
+  fg::MxCache c;
+  const int bad = check_mx(cache, op, &c);
+  if (bad) return bad;
+  fg::MxAttnArgs m = {};
+  if (const char* why = mx_attn_sizes(m, T, B, q_heads, cache->kv_heads, cache->head_dim, cache->bits, max_seq_len, max_query_len,
+                                      window, query_start != nullptr))
+    return fail(FG_EINVAL, "%s: %s", op, why);
+  if (T == 0) return FG_OK;
+  if (dtype != FG_F16 && dtype != FG_BF16) return fail(FG_EINVAL, "%s: q is fp16 or bf16", op);
+  if (!(softcap >= 0.f)) return fail(FG_EINVAL, "%s: softcap is positive, or 0 for none", op);
+  if (!q || !out || (B > 0 && !seq_lens) || (max_seq_len > 0 && B > 0 && !page_table)) return fail(FG_EINVAL, "%s: null tensor", op);
+  if (rows_overlap({o_token, T}, {o_head, q_heads}, {0, 1}, cache->head_dim))
+    return fail(FG_EINVAL, "%s: out's rows overlap", op);
+  if (B > 0 && ld_pages * cache->page_size < max_seq_len)
+    return fail(FG_EINVAL, "%s: max_seq_len is past the page table's columns", op);
+  const size_t need = fg::mx_attn_plan(m);
+  if (m.a.items < 0) return fail(FG_EINVAL, "%s: more work items or rows than a launch takes", op);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return fail(FG_EINVAL, "%s: the workspace needs %zu bytes, 16-byte aligned", op, need);
+  fg::AttnArgs& a = m.a;
+  a.q = static_cast<const uint16_t*>(q); a.q_t = q_token; a.q_h = q_head;
+  a.out = static_cast<uint16_t*>(out); a.o_t = o_token; a.o_h = o_head; a.lse = lse;
+  a.k = c.k; a.v = c.v; a.c_head = c.head; a.c_page = (uint32_t)(c.page / 16); a.c_token = (uint32_t)(c.token / 16);
+  m.ks = c.ks; m.vs = c.vs; m.s_head = c.head / (4 * cache->bits);
+  a.pages = page_table; a.ld_pages = ld_pages; a.lens = seq_lens; a.starts = query_start;
+  a.page = cache->page_size; a.n_pages = (int)cache->num_pages;
+  const float log2e = 1.4426950408889634f;
+  m.cap_in = softcap > 0.f ? scale / softcap : 0.f;  // 0 where the cap is past all scores
+  m.factor = (m.cap_in != 0.f ? softcap : scale) * log2e;
+  return hip_status(fg::launch_mx_attn(m, dtype == FG_BF16, workspace, need, static_cast<hipStream_t>(stream)), "fg_mx_attention launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,99 @@
+// Attention over a block-scaled cache: o = softmax(s) V over the keys in a query token's window, s = scale q k or, capped,
+// cap tanh(scale q k / cap).  Keys are cut into parts, an item (row tile, key head, part) makes one pass over its keys with a running
+// maximum and sum (mx_rows, mx_tile), and the parts of a row are joined as in attention over 16-bit pages.  Here: the join and the
+// plan.
+#include <algorithm>
+
+#include "fg_attn_join.h"
+#include "fg_mx_attn.h"
+
+namespace fg {
+
+template <bool BF16, int L, int W>
+__global__ void __launch_bounds__(256) mx_join_kernel(const MxAttnArgs m) {
+  const AttnArgs& a = m.a;
+  const JoinRow<L, W> r;
+  if (r.id >= (int64_t)a.T * a.Hq) return;
+  const int t = (int)(r.id / a.Hq), h = (int)(r.id - (int64_t)t * a.Hq);
+  int seq = t, tok = 0, count = 1;
+  bool inside = true;
+  if (a.starts) {
+    seq = attn_sequence(a, t);
+    inside = a.B > 0 && a.starts[seq] <= t && t < a.starts[seq + 1];
+    if (inside) {
+      const int first = attn_start(a, seq);
+      tok = t - first;
+      count = attn_start(a, seq + 1) - first;
+    }
+  }
+  const bool served = !inside || tok < a.max_q;
+  int n = 0;
+  if (inside && served) {  // the parts of the row's tile
+    const int len = max(min(a.lens[seq], a.max_len), 0), rows = min(count, a.max_q) * a.G, tile = m.tile ? kTileRows : 16;
+    const int row0 = (tok * a.G + h % a.G) / tile * tile;
+    const MxRange all = mx_range(m, len, len - count + 1, row0 / a.G, min(rows - 1, row0 + tile - 1) / a.G);
+    n = max((all.end - all.begin + a.part_s - 1) / a.part_s, 1);
+  }
+  attn_join<BF16, L, W>(a, r, t, h, n, served);
+}
+
+static int join_waves(const MxAttnArgs& m) { return m.a.parts_s >= 8 ? 4 : 1; }
+
+// Fills in the plan; returns the partial sums' bytes.  items is -1 where the threads of a launch would pass 32 bits.
+size_t mx_attn_plan(MxAttnArgs& m) {
+  AttnArgs& a = m.a;
+  const int64_t rows = (int64_t)a.max_q * a.G, cus = device_cus();
+  m.tile = rows > 16;
+  const int64_t tile = m.tile ? kTileRows : 16, tokens = std::min<int64_t>(a.max_q, tile / a.G + 2);
+  const int64_t span = std::min<int64_t>(a.max_len, (int64_t)m.window + tokens - 1);  // keys that a tile's rows see at most
+  a.tiles_s = (int)((rows + tile - 1) / tile);
+  const int64_t sets = (int64_t)a.Hk * a.B, items = std::max<int64_t>(sets * a.tiles_s, 1), unit = m.tile ? 64 : kRowsTile * kRowsWaves;
+  // about two workgroups per CU
+  int64_t parts = std::max<int64_t>(1, 2 * cus / items);
+  if (!m.tile) parts = std::max<int64_t>(parts, (span + kMaxPart - 1) / kMaxPart);
+  const int64_t part = std::max<int64_t>(unit, ((span + parts - 1) / parts + unit - 1) / unit * unit);
+  a.part_s = (int)part;
+  a.parts_s = (int)std::max<int64_t>(1, (span + part - 1) / part);
+  const int64_t all = attn_count(a.parts_s * sets, a.tiles_s);
+  a.items = all < (1LL << 24) - 64 ? (int)all : -1;
+  if (a.parts_s == 1 && a.B > 0) return 0;  // nothing to join
+  if ((int64_t)a.T * a.Hq * join_waves(m) >= 1LL << 26) a.items = -1;
+  return (size_t)a.parts_s * a.T * a.Hq * ((size_t)a.D * 4 + sizeof(float2));
+}
+
+hipError_t launch_mx_attn_bf16(const MxAttnArgs& m, hipStream_t st);
+hipError_t launch_mx_attn_fp16(const MxAttnArgs& m, hipStream_t st);
+
+// A planned call; `bytes`: what mx_attn_plan returned for it.
+hipError_t launch_mx_attn(MxAttnArgs& m, bool bf16, void* ws, size_t bytes, hipStream_t st) {
+  AttnArgs& a = m.a;
+  a.acc = nullptr;
+  a.ml = nullptr;
+  if (bytes) {
+    a.acc = static_cast<float*>(ws);
+    a.ml = reinterpret_cast<float2*>(a.acc + (size_t)a.parts_s * a.T * a.Hq * a.D);
+  }
+  if (a.items) {
+    const hipError_t e = bf16 ? launch_mx_attn_bf16(m, st) : launch_mx_attn_fp16(m, st);
+    if (e != hipSuccess) return e;
+  }
+  note_kernel("%s<%d> parts=%d%s", m.tile ? "mx_tile_kernel" : "mx_rows_kernel", m.bits, a.parts_s, bytes ? " + mx_join_kernel" : "");
+  if (!bytes) return hipSuccess;
+  const int many = join_waves(m);
+  auto join = [&](auto b_tag, auto l_tag) {
+    constexpr bool B = decltype(b_tag)::value;
+    constexpr int L = decltype(l_tag)::value;
+    const dim3 grid((unsigned)(((int64_t)a.T * a.Hq * many + 3) / 4));
+    if (many == 1) hipLaunchKernelGGL((mx_join_kernel<B, L, 1>), grid, dim3(256), 0, st, m);
+    else hipLaunchKernelGGL((mx_join_kernel<B, L, 4>), grid, dim3(256), 0, st, m);
+    return hipGetLastError();
+  };
+  auto by_d = [&](auto b_tag) {
+    if (a.D <= 64) return join(b_tag, std::integral_constant<int, 16>{});
+    if (a.D <= 128) return join(b_tag, std::integral_constant<int, 32>{});
+    return join(b_tag, std::integral_constant<int, 64>{});
+  };
+  return bf16 ? by_d(std::true_type{}) : by_d(std::false_type{});
+}
+
+}  // namespace fg

@@ -1,0 +1,7 @@
+#include "fg_mx_kernels.h"
+
+namespace fg {
+
+hipError_t launch_mx_attn_bf16(const MxAttnArgs& m, hipStream_t st) { return launch_mx_items<true>(m, st); }
+
+}  // namespace fg

@@ -1,0 +1,250 @@
+// mx_rows: work items of up to 16 rows (decoding) over block-scaled keys and values.  The products are those of attn_rows: a
+// wavefront by itself on tiles of 32 keys, S^T = K Q^T, then O^T += V^T P^T with P^T straight from the registers of the first.
+// A lane reads one run of DP / 4 adjacent columns of a key, which is whole blocks of 32 or a part of one, so its codes become 16-bit
+// floats by the conversions that take the scale along (two values an instruction, exact); the first product's columns are
+// numbered as the runs lie.  Values are converted on the way to LDS and come back through the transposing read.
+#pragma once
+
+#include "fg_attn_rows.h"
+#include "fg_mx_attn.h"
+
+namespace fg {
+
+template <int DP>
+struct MxRowsLds {
+  static constexpr int kV = kRowsTile * DP * 2, kO = 16 * DP * 4;
+  static constexpr int kTab = kRowsWaves * (kV > kO ? kV : kO), kRed = kTab + kMaxPart * 4;
+  static constexpr int kBytes = kRed + 2 * kRowsWaves * 16 * 4;
+};
+
+template <bool BF16, int BITS, bool CAP, int DP>
+__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) mx_rows_kernel(const MxAttnArgs m_) {
+  constexpr int U = DP / 8, C = DP / 32, DB = DP / 16;
+  constexpr int RUN = DP / 4, W = RUN * BITS / 32, WC = BITS / 4;  // columns of a lane's run, their words, words of 8 columns
+  constexpr int SB = RUN > kMxBlock ? RUN / kMxBlock : 1;          // scales of a run
+  using L = MxRowsLds<DP>;
+  __shared__ __align__(16) uint8_t lds[L::kBytes];
+  uint32_t* tab = reinterpret_cast<uint32_t*>(lds + L::kTab);
+  float* red = reinterpret_cast<float*>(lds + L::kRed);
+  const AttnArgs& a = m_.a;
+
+  AttnItem it;
+  if (!mx_item<16>(m_, blockIdx.x, it)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, grp = lane >> 4;
+  attn_row_table(a, it, tab, kRowsTile);
+
+  // this lane's row: the fragment of Q, and the keys it sees
+  const int row = it.row0 + l16, tok = row / a.G, g = row - tok * a.G;
+  const uint16_t* qp = a.q + (int64_t)(it.token0 + tok) * a.q_t + (int64_t)(it.head * a.G + g) * a.q_h;
+  const AttnFactor factor = attn_factor(m_.factor, 1.f);
+  const uint32_t sign = CAP ? 0 : factor.sign;
+  s16x8 qf[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int d = RUN * grp + 8 * c;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (row < it.rows && d < a.D) __builtin_memcpy(&u, __builtin_assume_aligned(qp + d, 2), 16);
+    u.x ^= sign; u.y ^= sign; u.z ^= sign; u.w ^= sign;
+    qf[c] = __builtin_bit_cast(s16x8, u);
+  }
+  const int seen = it.seen0 + tok, low = seen - m_.window;                              // keys low .. seen - 1
+  const int min_seen = it.seen0 + it.row0 / a.G;                                        // of the tile's first row
+  const int max_low = it.seen0 + min(it.rows - 1, it.row0 + 15) / a.G - m_.window;      // of its last
+  const float sc = CAP ? m_.factor : factor.value, cap_in = m_.cap_in;
+  const bool there = RUN * grp < a.D;  // this lane's run, or its first block
+  const uint8_t *kb = a.k + it.head * a.c_head + grp * (RUN * BITS / 8), *vb = a.v + it.head * a.c_head + grp * (RUN * BITS / 8);
+  const uint8_t *ksb = m_.ks + it.head * m_.s_head + RUN * grp / kMxBlock, *vsb = m_.vs + it.head * m_.s_head + RUN * grp / kMxBlock;
+
+  f32x4 o[DB];
+  float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  __syncthreads();
+
+  const int n = max(it.end - it.begin, 0), step = kRowsTile * kRowsWaves;
+  uint8_t* vl = lds + wave * L::kV;
+  // NB tiles in registers: while one is computed the others are on their way (a run of 64 bytes leaves room for one: the next is
+  // loaded behind the products that used it)
+  constexpr int NB = W >= 16 ? 1 : 2;
+  uint32_t kr[NB][2][W], vr[NB][2][W], kse[NB][2][SB], vse[NB][2][SB];
+  uint32_t ok[NB];  // bit t: key t of the tile is there
+  auto words = [](uint32_t(&to)[W], const uint8_t* p) __attribute__((always_inline)) {
+    if constexpr (W == 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      to[0] = u.x;
+      to[1] = u.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p + 4 * i);
+        to[i] = u.x;
+        to[i + 1] = u.y;
+        to[i + 2] = u.z;
+        to[i + 3] = u.w;
+      }
+    }
+  };
+  auto fetch = [&](int b, int t0) __attribute__((always_inline)) {
+    const uint32_t rows[2] = {tab[t0 + l16], tab[t0 + 16 + l16]};
+    ok[b] = (uint32_t)(__ballot(rows[0] != kNoRow) & 0xffff) | (uint32_t)(__ballot(rows[1] != kNoRow) & 0xffff) << 16;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint64_t at = (uint64_t)rows[h] * 16, sat = BITS == 4 ? rows[h] : rows[h] >> 1;
+      if (ok[b] == 0xffffffffu && a.D == DP) {
+        words(kr[b][h], kb + at);
+        words(vr[b][h], vb + at);
+#pragma unroll
+        for (int i = 0; i < SB; ++i) {
+          kse[b][h][i] = ksb[sat + i];
+          vse[b][h][i] = vsb[sat + i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) kr[b][h][i] = vr[b][h][i] = 0;
+#pragma unroll
+        for (int i = 0; i < SB; ++i) kse[b][h][i] = vse[b][h][i] = 1;
+        if (rows[h] != kNoRow && there) {
+#pragma unroll
+          for (int i = 0; i < SB; ++i) {  // blocks of the run that the head has
+            if (RUN * grp + kMxBlock * i >= a.D) continue;
+            constexpr int n = W / SB;
+            kse[b][h][i] = ksb[sat + i];
+            vse[b][h][i] = vsb[sat + i];
+#pragma unroll
+            for (int j = 0; j < n; j += 2) {
+              const uint2 x = *reinterpret_cast<const uint2*>(kb + at + 4 * (n * i + j));
+              const uint2 y = *reinterpret_cast<const uint2*>(vb + at + 4 * (n * i + j));
+              kr[b][h][n * i + j] = x.x;
+              kr[b][h][n * i + j + 1] = x.y;
+              vr[b][h][n * i + j] = y.x;
+              vr[b][h][n * i + j + 1] = y.y;
+            }
+          }
+        }
+      }
+    }
+  };
+  auto turn = [&](int b, int t0) __attribute__((always_inline)) {
+    const uint32_t here = ok[b];
+    auto scale = [](uint32_t byte) { return __uint_as_float(byte << 23); };  // 255: the conversion gives NaN
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int t = 16 * h + l16;
+        *reinterpret_cast<uint4*>(vl + (t * U + rows_unit<U>(t, C * grp + c)) * 16) =
+            mx_eight<BF16, BITS>(vr[b][h][c * WC], vr[b][h][c * WC + WC - 1], scale(vse[b][h][c * 8 / kMxBlock]));
+      }
+    f32x4 s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const uint4 k8 = mx_eight<BF16, BITS>(kr[b][h][c * WC], kr[b][h][c * WC + WC - 1], scale(kse[b][h][c * 8 / kMxBlock]));
+        s[h] = mfma16<BF16>(__builtin_bit_cast(s16x8, k8), qf[c], c ? s[h] : (f32x4)(0.f));
+      }
+    if (t0 + NB * step < n) fetch(b, t0 + NB * step);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = CAP ? mx_tanh(s[j / 4][j % 4] * cap_in) : s[j / 4][j % 4];
+    const int first = it.begin + t0;
+    if (here != 0xffffffffu || first + kRowsTile > min_seen || first < max_low) {
+      asm volatile("");  // a branch, so that whole tiles skip it
+      const int left = seen - first, skip = low - first;  // keys of the tile that this lane's row sees: skip .. left - 1
+      uint32_t mask = left >= 32 ? here : (left > 0 ? here & ((1u << left) - 1) : 0u);
+      if (skip > 0) mask = skip >= 32 ? 0u : mask & ~((1u << skip) - 1);
+      mask >>= 4 * grp;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (!(mask >> (16 * (j / 4) + j % 4) & 1)) x[j] = -__builtin_inff();
+    }
+    float top = x[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+    top = attn_top<BF16>(top, sc);
+    if (__any(top > m + kSlack)) {
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - attn_base(mn));
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= f;
+    }
+    const float base = attn_base(m);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], sc, -base));
+    l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = pack2<BF16>(x[2 * j], x[2 * j + 1]);
+    const s16x8 p = __builtin_bit_cast(s16x8, make_uint4(w[0], w[1], w[2], w[3]));
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      s16x4 half[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // 16 lanes read 4 keys x 16 columns
+        const int t = 16 * h + 4 * grp + l16 / 4;
+        half[h] = lds_tr16(vl + (t * U + rows_unit<U>(t, 2 * d + (l16 % 4) / 2)) * 16 + 8 * (l16 % 2));
+      }
+      o[d] = mfma16<BF16>(__builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7), p, o[d]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  };
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    if (wave * kRowsTile + b * step < n) fetch(b, wave * kRowsTile + b * step);
+  for (int t0 = wave * kRowsTile; t0 < n; t0 += NB * step) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (t0 + b * step < n) turn(b, t0 + b * step);
+  }
+
+  // join the wavefronts: maxima and sums first, then each adds up a quarter of the columns
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
+  if (grp == 0) {
+    red[wave * 16 + l16] = m;
+    red[(kRowsWaves + wave) * 16 + l16] = l;
+  }
+  __syncthreads();
+  float top = red[l16], sum = 0.f;
+#pragma unroll
+  for (int w = 1; w < kRowsWaves; ++w) top = fmaxf(top, red[w * 16 + l16]);
+  const float base = attn_base(top);
+#pragma unroll
+  for (int w = 0; w < kRowsWaves; ++w)
+    sum += red[(kRowsWaves + w) * 16 + l16] * __builtin_amdgcn_exp2f(red[w * 16 + l16] - base);
+  const float f = __builtin_amdgcn_exp2f(m - base);
+  f32x4* ol = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+  for (int d = 0; d < DB; ++d) ol[(wave * DB + d) * 64 + lane] = o[d] * f;
+  __syncthreads();
+  if (row >= it.rows) return;
+  const int64_t t = it.token0 + tok;
+  const int h = it.head * a.G + g;
+  const int64_t at = ((int64_t)it.slot * a.T + t) * a.Hq + h;
+  const float inv = a.acc ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);  // a row that saw no key gives zeros
+#pragma unroll
+  for (int e = 0; e < DB / kRowsWaves; ++e) {
+    const int d = e * kRowsWaves + wave, col = 16 * d + 4 * grp;
+    if (col >= a.D) continue;
+    f32x4 r = ol[d * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < kRowsWaves; ++w) r += ol[(w * DB + d) * 64 + lane];
+    r *= inv;
+    if (a.acc) {
+      *reinterpret_cast<f32x4*>(a.acc + at * a.D + col) = r;
+    } else {
+      const uint2 w = make_uint2(pack2<BF16>(r[0], r[1]), pack2<BF16>(r[2], r[3]));
+      __builtin_memcpy(__builtin_assume_aligned(a.out + t * a.o_t + h * a.o_h + col, 2), &w, 8);
+    }
+  }
+  if (wave == 0 && grp == 0) {
+    if (a.acc) a.ml[at] = make_float2(top, sum);
+    else if (a.lse) a.lse[t * a.Hq + h] = (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+  }
+}
+
+}  // namespace fg

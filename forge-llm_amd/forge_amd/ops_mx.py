@@ -3,7 +3,8 @@ that reads it, computed by libforge_mi355x.so only.
 
 * :class:`MXKVCache`: keys and values in the OCP microscaling formats, e2m1 (4 bits) or e4m3 (8 bits) codes with e8m0 scales;
 * :func:`mx_append`: rotation by positions of one or several axes, and the new tokens' codes and scales;
-* :func:`mx_read`: tokens of the cache as 16-bit values.
+* :func:`mx_read`: tokens of the cache as 16-bit values;
+* :func:`mx_attention`: attention over this cache, with a tanh cap on the scores and a window.
 
 Beside :class:`ops_decoder.PagedKVCache`, whose e4m3 form has one given scale per head, this cache takes its scales from the values
 as they are written.  As in ``ops_decoder`` every op is one call into the C ABI (``include/forge_mi355x.h``) on the current
@@ -12,6 +13,7 @@ torch's caching allocator, so a layer can be captured in a HIP graph.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -197,3 +199,84 @@ def mx_read(cache: MXKVCache, slots: torch.Tensor, *, dtype: torch.dtype = torch
             _check(status, "fg_mx_read")
     _done(op)
     return k, v
+
+
+# ================================================================================================ attention
+def mx_attention(q: torch.Tensor, cache: MXKVCache, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                 query_start: torch.Tensor | None = None, max_query_len: int = 1, max_seq_len: int | None = None,
+                 scale: float | None = None, softcap: float | None = None, window: int | None = None, return_lse: bool = False,
+                 out: torch.Tensor | None = None) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Attention of ``q [T, heads, dim]`` over the cache, for B sequences: each query token sees its sequence's tokens up to itself,
+    with ``window`` the last ``window`` of them (its own included).  Scores are ``scale * q.k`` or, with ``softcap``,
+    ``softcap * tanh(scale * q.k / softcap)``.  Returns ``[T, heads, dim]`` in ``q``'s type, with ``return_lse`` also the logarithm of
+    each row's softmax sum, fp32 ``[T, heads]``.
+
+    ``page_table``, ``seq_lens``, ``query_start``, ``max_query_len``, ``max_seq_len``, ``scale`` and ``out`` are those of
+    :func:`ops_decoder.prefix_attention`, as is what tokens of no sequence, rows that see no token (zeros, lse -inf), query tokens
+    past ``max_query_len`` (NaN) and page ids outside the cache (no tokens) give.
+
+    Codes become ``q``'s type exactly, but for fp16 queries over values past 65504 (infinite) or below 2^-24.  Scores, softmax and
+    sums are fp32, a capped score within ``2^-20 * softcap``; the probabilities are rounded to ``q``'s type for the product with the
+    values.  A NaN block that some query token of a sequence sees can show in that sequence's earlier query tokens too.
+    """
+    op = "mx_attention"
+    _on_gpu(q, op)
+    handle, hk, page, dim, bits = cache._handle()
+    _elsewhere(op, q, page_table, seq_lens, query_start, cache.k, out)
+    q = _heads(op, "q", q, dim)
+    shape = q.shape
+    t, h, _ = shape
+    if h % hk or h == 0:
+        raise ConfigError(f"{op}: {h} query heads are no multiple of {hk} key heads")
+    pages = page_table.shape
+    if len(pages) != 2 or page_table.dtype is not torch.int32:
+        raise ConfigError(f"{op}: page_table must be int32 [sequences, pages]")
+    b, width = pages
+    if seq_lens.shape != (b,) or seq_lens.dtype is not torch.int32:
+        raise ConfigError(f"{op}: seq_lens must be int32 [{b}]")
+    ragged = query_start is not None
+    if ragged and (query_start.shape != (b + 1,) or query_start.dtype is not torch.int32):
+        raise ConfigError(f"{op}: query_start must be int32 [{b + 1}]")
+    if not ragged and (t != b or max_query_len != 1):
+        raise ConfigError(f"{op}: without query_start each of the {b} sequences has one query token, got {t}")
+    if max_query_len < 1:
+        raise ConfigError(f"{op}: max_query_len must be positive")
+    if max_seq_len is None:
+        max_seq_len = width * page
+    elif not 0 <= max_seq_len <= width * page:
+        raise ConfigError(f"{op}: max_seq_len {max_seq_len} is past the page table's {width} pages of {page}")
+    if window is None:
+        window = 0
+    elif window < 1:
+        raise ConfigError(f"{op}: window must be positive (None: all tokens)")
+    if softcap is None:
+        softcap = 0.0
+    elif not softcap > 0:
+        raise ConfigError(f"{op}: softcap must be positive (None: no cap)")
+    out, o0, o1 = _result(op, "out", out, q, shape)
+    lse = q.new_empty((t, h), dtype=torch.float32) if return_lse else None
+    if t:
+        q0, q1, _ = q.stride()
+        ld, column = page_table.stride()
+        if column != 1 or b <= 1 or ld < width:
+            page_table, ld = page_table.contiguous(), width
+        if not seq_lens.is_contiguous():
+            seq_lens = seq_lens.contiguous()
+        query_start = query_start.contiguous() if ragged else None
+        need = _attention_workspace(q.get_device(), t, b, h, hk, dim, bits, max_seq_len, max_query_len, window, ragged)
+        ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+        status = _lib.lib().fg_mx_attention(
+            q.data_ptr(), q0, q1, _CODE[q.dtype], handle, page_table.data_ptr(), ld, seq_lens.data_ptr(), _lib.ptr(query_start), t, b, h,
+            max_seq_len, max_query_len, dim ** -0.5 if scale is None else scale, softcap, window, out.data_ptr(), o0, o1, _lib.ptr(lse),
+            _lib.ptr(ws), need, _lib.stream_of(q))
+        if status:
+            _check(status, "fg_mx_attention")
+    _done(op)
+    return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(_device: int, t: int, b: int, h: int, hk: int, dim: int, bits: int, max_seq_len: int, max_query_len: int,
+                         window: int, ragged: bool) -> int:
+    """Bytes of a call's partial sums, which follow from its sizes (and the GPU's CUs) alone."""
+    return _lib.lib().fg_mx_attention_workspace_bytes(t, b, h, hk, dim, bits, max_seq_len, max_query_len, window, ragged)

@@ -376,6 +376,21 @@ int fg_mx_append(const void* q, int64_t q_token, int64_t q_head, const void* k, 
 int fg_mx_read(const fg_mx_cache* cache, const void* slots, int32_t slots_int64, void* k_out, void* v_out, int dtype,
                int64_t n, fg_stream_t stream);
 
+/* Attention of T query tokens over the cache, for B sequences: o = softmax(s) V over the keys that a query token sees,
+ * s = scale q.k or, with softcap > 0, softcap * tanh(scale q.k / softcap).  page_table, seq_lens, query_start, max_seq_len,
+ * max_query_len, lse and what happens to rows that see nothing, tokens of no sequence and ids outside are those of
+ * fg_prefix_attention (without a prefix).  window > 0: a query token sees the last `window` of the tokens up to itself (its own
+ * included); 0: all of them.
+ *   workspace: fg_mx_attention_workspace_bytes bytes, 16-byte aligned; 0 also for sizes that the call refuses. */
+size_t fg_mx_attention_workspace_bytes(int64_t T, int64_t B, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                       int32_t bits, int64_t max_seq_len, int64_t max_query_len, int64_t window,
+                                       int32_t ragged);
+int fg_mx_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const fg_mx_cache* cache,
+                    const int32_t* page_table, int64_t ld_pages, const int32_t* seq_lens, const int32_t* query_start,
+                    int64_t T, int64_t B, int32_t q_heads, int64_t max_seq_len, int64_t max_query_len, float scale,
+                    float softcap, int64_t window, void* out, int64_t o_token, int64_t o_head, float* lse, void* workspace,
+                    size_t workspace_bytes, fg_stream_t stream);
+
 /* ---------------------------------------------------------------------------------------------------------------
  * Library information.  fg_device_ok replaces the capability gate triton_usable (forge/kernels/ops_gemm.py:159-175):
  * returns 1 when `device` is a gfx950 GPU this build can run on, else 0 (message in fg_last_error).

@@ -56,3 +56,32 @@ def rotate_axes_ref(x, positions, table, sections, interleaved):
         u, w = x[:, :, a].clone(), x[:, :, b].clone()
         x[:, :, a], x[:, :, b] = u * c - w * s, w * c + u * s
     return x
+
+
+def capped_attention_ref(q, k, v, present, seq_lens, starts, scale, softcap, window):
+    """(out, lse, sum of p |v|) in fp64 of ``q [T, heads, dim]`` over ``k``, ``v`` (fp64, a [key heads, n, dim] for each sequence) and
+    ``present`` (which of the n tokens are there): a token sees the last ``window`` of its sequence's up to itself."""
+    q = q.cpu().double()
+    t, h, d = q.shape
+    out, mag = torch.zeros(t, h, d, dtype=torch.float64), torch.zeros(t, h, d, dtype=torch.float64)
+    lse = torch.full((t, h), -float("inf"), dtype=torch.float64)
+    for b, n in enumerate(seq_lens):
+        a, c = starts[b], starts[b + 1]
+        if n == 0 or a == c:
+            continue
+        at = n - (c - a) + torch.arange(c - a).view(-1, 1)
+        j = torch.arange(n)
+        sees = (j <= at) & (j > at - window) if window else j <= at
+        sees = sees & present[b]
+        some = sees.any(1)
+        group = h // k[b].shape[0]
+        for head in range(h):
+            kk, vv = (torch.where(present[b].view(-1, 1), x[b][head // group], 0.0) for x in (k, v))
+            s = q[a:c, head] @ kk.t() * scale
+            s = softcap * torch.tanh(s / softcap) if softcap else s
+            s = s.masked_fill(~sees, -float("inf"))[some]
+            z = torch.logsumexp(s, 1)
+            p = torch.exp(s - z.view(-1, 1))
+            rows = torch.nonzero(some).flatten() + a
+            lse[rows, head], out[rows, head], mag[rows, head] = z, p @ vv, p @ vv.abs()
+    return out, lse, mag
