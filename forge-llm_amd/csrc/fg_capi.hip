@@ -15,6 +15,7 @@
 #include "fg_decoder.h"
 #include "fg_device.h"
 #include "fg_mx_attn.h"
+#include "fg_sample.h"
 
 namespace fg {
 hipError_t launch_w4_gemv(int mt, int R, bool xbf16, const void* x, int64_t ldx, const int32_t* qw, int64_t ldq,
@@ -1549,6 +1550,49 @@ int fg_mx_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, c
   m.cap_in = softcap > 0.f ? scale / softcap : 0.f;  // 0 where the cap is past all scores
   m.factor = (m.cap_in != 0.f ? softcap : scale) * log2e;
   return hip_status(fg::launch_mx_attn(m, dtype == FG_BF16, workspace, need, static_cast<hipStream_t>(stream)), "fg_mx_attention launch");
+}
+
+}  // extern "C"
+
+namespace {
+
+const char* sample_sizes(fg::SampleArgs& a, int64_t B, int64_t V) {
+  // a workgroup of 1024 threads for each chunk of a row
+  if (B < 0 || V <= 0 || V >= kMaxDim / 2 || B >= 1 << 16) return "bad sizes";
+  a.B = (int)B; a.V = (int)V;
+  return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fg_sample_workspace_bytes(int64_t B, int64_t V) {
+  fg::SampleArgs a = {};
+  return sample_sizes(a, B, V) || B == 0 ? 0 : fg::sample_plan(a);
+}
+
+int fg_sample_tokens(const void* logits, int64_t ld, int dtype, const float* u, const float* temperature,
+                     float temperature_all, const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+                     const float* min_p, float min_p_all, int64_t* token, float* logprob, int64_t B, int64_t V,
+                     void* workspace, size_t workspace_bytes, fg_stream_t stream) {
+  static const char* const op = "fg_sample_tokens";
+  fg::SampleArgs a = {};
+  if (const char* why = sample_sizes(a, B, V)) return fail(FG_EINVAL, "%s: %s", op, why);
+  if (B == 0) return FG_OK;
+  if (!logits || !u || !token) return fail(FG_EINVAL, "%s: null tensor", op);
+  if (!is_float_dt(dtype)) return fail(FG_EINVAL, "%s: bad dtype", op);
+  if (ld < 0) return fail(FG_EINVAL, "%s: bad row stride", op);
+  const size_t need = fg::sample_plan(a);
+  if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(FG_EINVAL, "%s: the workspace needs %zu bytes, 16-byte aligned", op, need);
+  a.x = logits; a.ld = ld; a.u = u;
+  a.temperature = temperature; a.temperature_all = temperature_all; a.top_k = top_k; a.top_k_all = top_k_all;
+  a.top_p = top_p; a.top_p_all = top_p_all; a.min_p = min_p; a.min_p_all = min_p_all;
+  a.token = token; a.logprob = logprob; a.ws = static_cast<uint8_t*>(workspace);
+  const bool drawn = temperature || temperature_all > 0.f;
+  a.cuts = drawn && (top_k || (top_k_all > 0 && top_k_all < V) || top_p || top_p_all < 1.f);
+  return hip_status(fg::launch_sample(a, dtype, static_cast<hipStream_t>(stream)), "fg_sample_tokens launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,737 @@
+// Tokens from their logits and given random numbers u.  With M the row's largest logit and T its temperature the weights are
+//   w_i = 2^((l_i - M) log2(e) / T),
+// kept are the first k tokens in the order of their logits (equal ones by their index), of these the shortest beginning whose weight
+// reaches p times the k tokens', and of these the ones with w_i >= min_p; the token is the first, by index, at which the kept
+// weights' sum passes u times their total.
+//
+// Weights are computed in fp64 and summed as whole numbers of 2^-bits (a bits of 44 for 2^17 tokens or so): sums do not hang on their
+// order, so they go through atomics, and a token of less than half a unit is one that nobody draws.
+//
+// Nothing is sorted.  A histogram of the row over (M - l) log2(e) / T, with the weight and the number of the tokens in each
+// bin, says in which bin the k-th token and the nucleus's last one lie.  Where all bins up to there hold few tokens (kList), these are
+// collected and settle the row by themselves; else the border bins' tokens settle the border, and one more pass over the row sums
+// up the weights in front of it, in the order of the indexes.  The border within a list is found by histograms again, each over a
+// 2048th of the one before.
+//
+// One launch for each pass (extremes, histogram, collection, sums); a row is cut into chunks of a workgroup each while rows are few,
+// and what follows a pass is done by the workgroup that ends last.  Bound by HBM for the first pass, for the others by
+// the L2 and Infinity caches and the arithmetic of the weights; for one row by the launches.
+#include <algorithm>
+
+#include "fg_sample.h"
+
+namespace fg {
+
+namespace {
+
+constexpr int kBins = 2048, kList = 4096, kThreads = 1024, kWaves = kThreads / 64, kMaxChunks = 64;
+
+struct ChunkSum {
+  float max, min;  // of the finite or infinite logits above -inf; min of those
+  int arg;         // the largest one's first index, -1: none
+  float sum;       // of exp(l - max)
+};
+
+struct RowState {
+  uint64_t mass[kBins];
+  uint32_t count[kBins];
+  uint64_t list[kList];  // key << 32 | index, in any order
+  uint64_t wave_mass[kMaxChunks * kWaves];
+  ChunkSum part[kMaxChunks];
+  uint32_t listed, ticket[2];
+  uint32_t done;         // the row has its token
+  uint32_t cut_key, cut_index;  // kept: a larger key, or this one up to this index
+};
+
+// A row's settings and extremes.
+struct Row {
+  float t, p, minp;
+  int k;
+  bool greedy, by_k, by_p;
+  float max, min;
+  int arg;
+  double scale;  // log2(e) / T
+};
+
+// A logit's place in the order as an unsigned number: NaN counts as -inf, -0 as 0.
+__device__ __forceinline__ uint32_t key_of(float l) {
+  const uint32_t b = __float_as_uint(l + 0.f);
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(uint32_t key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
+
+template <int DT>
+__device__ __forceinline__ float one(const void* row, int i) {
+  const float l = load_f(row, DT, i);
+  return __builtin_isnan(l) ? -__builtin_inff() : l;
+}
+
+typedef uint32_t u32x4_by4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_by2 __attribute__((ext_vector_type(2), aligned(2)));
+
+// Four neighbouring logits, as many as there are up to `end`; the others are -inf.
+template <int DT>
+__device__ __forceinline__ void four(const void* row, int i, int end, float (&l)[4]) {
+  if (i + 4 <= end) {
+    if constexpr (DT == FG_F32) {
+      const u32x4_by4 w = *reinterpret_cast<const u32x4_by4*>(static_cast<const float*>(row) + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l[j] = __uint_as_float(w[j]);
+    } else {
+      const u32x2_by2 w = *reinterpret_cast<const u32x2_by2*>(static_cast<const uint16_t*>(row) + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint16_t b = (uint16_t)(w[j / 2] >> (16 * (j % 2)));
+        l[j] = DT == FG_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) l[j] = __builtin_isnan(l[j]) ? -__builtin_inff() : l[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) l[j] = i + j < end ? one<DT>(row, i + j) : -__builtin_inff();
+  }
+}
+
+// 2^-y for the weights: 2^-(k / 64) from a table and the exponential series of the rest, |x| <= ln 2 / 128, to x^5 (the next term is
+// below 2^-54).
+struct Powers {
+  double at[64];
+  __device__ __forceinline__ void fill() {
+    if (threadIdx.x < 64) at[threadIdx.x] = exp2(-(double)threadIdx.x / 64);
+  }
+};
+__device__ __forceinline__ double weight(const Powers& t, double y, int bits) {
+  const int k = (int)(y * 64 + 0.5);
+  const double x = ((double)k * 0.015625 - y) * 0.6931471805599453;
+  double e = __builtin_fma(x, 1.0 / 120, 1.0 / 24);
+  e = __builtin_fma(x, e, 1.0 / 6);
+  e = __builtin_fma(x, e, 0.5);
+  e = __builtin_fma(x, e, 1.0);
+  e = __builtin_fma(x, e, 1.0);
+  return __builtin_amdgcn_ldexp(t.at[k & 63] * e, bits - (k >> 6));
+}
+__device__ __forceinline__ uint64_t whole(double v) {  // to the nearest whole number, of less than 2^52
+  return __builtin_bit_cast(uint64_t, v + 0x1p52) & 0xfffffffffffffull;
+}
+
+// The exponent y >= 0 of logit l (infinite for one that weighs nothing).
+__device__ __forceinline__ double exponent(const Row& r, float l) {
+  if (l == r.max) return 0;
+  return ((double)r.max - (double)l) * r.scale;
+}
+__device__ __forceinline__ double most(int bits) { return bits + 1; }  // from here on a weight is no unit
+
+__device__ __forceinline__ double bin_scale(const Row& r, int bits) {
+  const double range = fmin(((double)r.max - (double)r.min) * r.scale, most(bits));
+  return range > 0 ? kBins / range : 0;
+}
+__device__ __forceinline__ int bin_of(double y, double scale) { return min((int)(y * scale), kBins - 1); }
+
+__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
+  return (uint64_t)(uint32_t)__shfl_up((int)(v >> 32), d, kWave) << 32 | (uint32_t)__shfl_up((int)v, d, kWave);
+}
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
+  return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), d, kWave) << 32 | (uint32_t)__shfl_xor((int)v, d, kWave);
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) v += shfl_xor64(v, d);
+  return v;
+}
+
+// Sum of the threads' values in front of this one; `all`: of all.  Two barriers.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* part, uint64_t* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint64_t o = shfl_up64(s, d);
+    if (lane >= d) s += o;
+  }
+  __syncthreads();  // the last call's sums have been read
+  if (lane == 63) part[wave] = s;
+  __syncthreads();
+  uint64_t before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    before += w < wave ? part[w] : 0;
+    sum += part[w];
+  }
+  *all = sum;
+  return before + s - v;
+}
+
+__device__ __forceinline__ void row_settings(const SampleArgs& a, int b, Row& r) {
+  r.t = a.temperature ? a.temperature[b] : a.temperature_all;
+  r.p = a.top_p ? a.top_p[b] : a.top_p_all;
+  r.minp = a.min_p ? a.min_p[b] : a.min_p_all;
+  r.k = a.top_k ? a.top_k[b] : a.top_k_all;
+  r.greedy = !(r.t > 0.f);
+  r.by_k = r.k > 0 && r.k < a.V;
+  r.by_p = r.p < 1.f;
+  r.minp = r.minp > 0.f ? fminf(r.minp, 1.f) : 0.f;
+  r.scale = 1.4426950408889634 / (double)r.t;
+}
+
+// The row's extremes from its chunks'; every thread has them.
+__device__ __forceinline__ void row_extremes(const SampleArgs& a, const RowState& s, Row& r) {
+  r.max = -__builtin_inff();
+  r.min = __builtin_inff();
+  r.arg = -1;
+  for (int c = 0; c < a.chunks; ++c) {
+    const ChunkSum p = s.part[c];
+    if (p.arg >= 0 && (r.arg < 0 || p.max > r.max)) {
+      r.max = p.max;
+      r.arg = p.arg;
+    }
+    r.min = fminf(r.min, p.min);
+  }
+}
+
+// Token i of logit l for row b.
+__device__ __forceinline__ void give(const SampleArgs& a, const RowState& s, int b, const Row& r, int i, float l) {
+  a.token[b] = i;
+  if (!a.logprob) return;
+  if (i < 0) {
+    a.logprob[b] = -__builtin_inff();
+    return;
+  }
+  if (r.max == __builtin_inff()) {  // the infinite ones share the row
+    a.logprob[b] = __builtin_nanf("");
+    return;
+  }
+  float sum = 0.f;
+  for (int c = 0; c < a.chunks; ++c)
+    if (s.part[c].arg >= 0) sum += s.part[c].sum * __builtin_amdgcn_exp2f((s.part[c].max - r.max) * 1.4426950408889634f);
+  a.logprob[b] = (l - r.max) - __builtin_amdgcn_logf(sum) * 0.69314718055994531f;
+}
+
+__device__ __forceinline__ const void* row_of(const SampleArgs& a, int b, int dt) {
+  return static_cast<const char*>(a.x) + (int64_t)b * a.ld * (dt == FG_F32 ? 4 : 2);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------------------------------------ extremes
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_extremes_kernel(const SampleArgs a) {
+  __shared__ ChunkSum part[kWaves];
+  const int b = blockIdx.x / a.chunks, c = blockIdx.x - b * a.chunks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  RowState& s = reinterpret_cast<RowState*>(a.ws)[b];
+  if (a.cuts) {
+    for (int i = c * kThreads + threadIdx.x; i < kBins; i += a.chunks * kThreads) {
+      s.mass[i] = 0;
+      s.count[i] = 0;
+    }
+  }
+  if (c == 0 && threadIdx.x == 0) s.listed = s.ticket[0] = s.ticket[1] = s.done = 0;
+  const void* row = row_of(a, b, DT);
+  const int end = min(a.V, (c + 1) * a.chunk);
+  const float inf = __builtin_inff(), log2e = 1.4426950408889634f;
+  float mx = -inf, mn = inf, sum = 0.f;
+  int arg = -1;
+#pragma unroll 2
+  for (int i = c * a.chunk + 4 * threadIdx.x; i < end; i += 4 * kThreads) {
+    float l[4];
+    four<DT>(row, i, end, l);
+    const float was = mx;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (l[j] > mx) {
+        mx = l[j];
+        arg = i + j;
+      }
+      mn = l[j] > -inf ? fminf(mn, l[j]) : mn;
+    }
+    if (a.logprob && mx > -inf) {
+      sum *= __builtin_amdgcn_exp2f((was - mx) * log2e);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += __builtin_amdgcn_exp2f((l[j] - mx) * log2e);
+    }
+  }
+  auto join = [&](float m2, float n2, int a2, float s2) {
+    if (a2 < 0) return;
+    if (arg < 0 || m2 > mx || (m2 == mx && a2 < arg)) {
+      sum = s2 + (arg < 0 ? 0.f : sum * __builtin_amdgcn_exp2f((mx - m2) * log2e));
+      mx = m2;
+      arg = a2;
+    } else {
+      sum += s2 * __builtin_amdgcn_exp2f((m2 - mx) * log2e);
+    }
+    mn = fminf(mn, n2);
+  };
+  for (int d = 1; d < 64; d *= 2) {
+    const float m2 = __shfl_xor(mx, d, kWave), n2 = __shfl_xor(mn, d, kWave), s2 = __shfl_xor(sum, d, kWave);
+    const int a2 = __shfl_xor(arg, d, kWave);
+    join(m2, n2, a2, s2);
+  }
+  if (lane == 0) part[wave] = {mx, mn, arg, sum};
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kWaves; ++w) join(part[w].max, part[w].min, part[w].arg, part[w].sum);
+    s.part[c] = {mx, mn, arg, sum};
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ histogram
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_histogram_kernel(const SampleArgs a) {
+  __shared__ uint64_t mass[kBins];
+  __shared__ uint32_t count[kBins];
+  __shared__ Powers powers;
+  const int b = blockIdx.x / a.chunks, c = blockIdx.x - b * a.chunks;
+  RowState& s = reinterpret_cast<RowState*>(a.ws)[b];
+  Row r;
+  row_settings(a, b, r);
+  if (r.greedy || !(r.by_k || r.by_p)) return;
+  row_extremes(a, s, r);
+  if (r.arg < 0) return;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    mass[i] = 0;
+    count[i] = 0;
+  }
+  powers.fill();
+  __syncthreads();
+  const void* row = row_of(a, b, DT);
+  const int end = min(a.V, (c + 1) * a.chunk);
+  const double scale = bin_scale(r, a.bits), top = most(a.bits);
+#pragma unroll 2
+  for (int i = c * a.chunk + 4 * threadIdx.x; i < end; i += 4 * kThreads) {
+    float l[4];
+    four<DT>(row, i, end, l);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double y = exponent(r, l[j]);
+      if (!(y < top)) continue;
+      const int bin = bin_of(y, scale);
+      atomicAdd(reinterpret_cast<unsigned long long*>(&mass[bin]), (unsigned long long)whole(weight(powers, y, a.bits)));
+      atomicAdd(&count[bin], 1u);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    if (a.chunks == 1) {
+      s.mass[i] = mass[i];
+      s.count[i] = count[i];
+    } else if (count[i]) {
+      atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[i]), (unsigned long long)mass[i]);
+      atomicAdd(&s.count[i], count[i]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ borders
+namespace {
+
+struct Shared {
+  uint64_t mass[kBins];
+  uint64_t list[kList];
+  uint64_t part[kWaves];
+  Powers powers;
+  uint64_t found[4];
+  uint32_t lo, hi;
+  int last;
+};
+
+// The smallest coordinate at which the sum of the values of the elements up to there reaches `target`, and the sum in front of
+// it.  each(f) calls f(coordinate, value) for the elements; false: the sum of all of them does not reach it.
+template <class Each>
+__device__ __forceinline__ bool border(Shared& m, uint64_t target, const Each& each, uint32_t* at, uint64_t* before) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    m.lo = 0xffffffffu;
+    m.hi = 0;
+  }
+  __syncthreads();
+  uint32_t lo = 0xffffffffu, hi = 0;
+  each([&](uint32_t c, uint64_t) {
+    lo = min(lo, c);
+    hi = max(hi, c);
+  });
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    lo = min(lo, (uint32_t)__shfl_xor((int)lo, d, kWave));
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, d, kWave));
+  }
+  if ((threadIdx.x & 63) == 0 && lo <= hi) {
+    atomicMin(&m.lo, lo);
+    atomicMax(&m.hi, hi);
+  }
+  __syncthreads();
+  lo = m.lo;
+  hi = m.hi;
+  uint64_t base = 0;
+  if (lo > hi) return false;
+  for (;;) {
+    const int width = 32 - __clz((int)(hi - lo)), shift = width > 11 ? width - 11 : 0;  // (hi - lo) >> shift < 2048
+    for (int i = threadIdx.x; i < kBins; i += kThreads) m.mass[i] = 0;
+    if (threadIdx.x == 0) m.found[0] = ~0ull;
+    __syncthreads();
+    each([&](uint32_t c, uint64_t v) {
+      if (c >= lo && c <= hi) atomicAdd(reinterpret_cast<unsigned long long*>(&m.mass[(c - lo) >> shift]), (unsigned long long)v);
+    });
+    __syncthreads();
+    uint64_t v[2], all;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = m.mass[2 * threadIdx.x + j];
+    uint64_t sum = base + block_scan(v[0] + v[1], m.part, &all);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (sum < target && target <= sum + v[j]) {
+        m.found[0] = 2 * threadIdx.x + j;
+        m.found[1] = sum;
+      }
+      sum += v[j];
+    }
+    __syncthreads();
+    const uint64_t bin = m.found[0];
+    if (bin == ~0ull) return false;
+    base = m.found[1];
+    lo += (uint32_t)bin << shift;
+    if (shift == 0) {
+      *at = lo;
+      *before = base;
+      return true;
+    }
+    hi = (uint32_t)min((uint64_t)hi, (uint64_t)lo + ((1u << shift) - 1));
+    __syncthreads();
+  }
+}
+
+// The smallest whole number that is p times s or more, and not less than one.
+__device__ __forceinline__ uint64_t share(float p, uint64_t s) {
+  const double v = ceil((double)p * (double)s);
+  return v > 1 ? min((uint64_t)v, s) : 1;
+}
+// What the kept weights' sum has to reach: the first whole number past u times the total.
+__device__ __forceinline__ uint64_t drawn(float u, uint64_t total) {
+  const double v = floor((double)u * (double)total);
+  return v > 0 ? min((uint64_t)v, total - 1) + 1 : 1;  // NaN counts as 0
+}
+
+}  // namespace
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_borders_kernel(const SampleArgs a) {
+  __shared__ Shared m;
+  const int b = blockIdx.x / a.chunks, c = blockIdx.x - b * a.chunks;
+  RowState& s = reinterpret_cast<RowState*>(a.ws)[b];
+  Row r;
+  row_settings(a, b, r);
+  if (r.greedy || !(r.by_k || r.by_p)) return;
+  row_extremes(a, s, r);
+  if (r.arg < 0) return;
+  const void* row = row_of(a, b, DT);
+  const double scale = bin_scale(r, a.bits), top = most(a.bits);
+  m.powers.fill();
+
+  // Where the borders are: sums in front of each bin.
+  uint64_t v[2], n[2], mass = 0, tokens = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    v[j] = s.mass[2 * threadIdx.x + j];
+    n[j] = s.count[2 * threadIdx.x + j];
+  }
+  const uint64_t v0 = block_scan(v[0] + v[1], m.part, &mass), n0 = block_scan(n[0] + n[1], m.part, &tokens);
+  __syncthreads();
+  __shared__ int bin_k, bin_lo, bin_hi;
+  __shared__ uint64_t k_mass, k_count, lo_mass, listed[2];
+  const bool by_k = r.by_k && (uint64_t)r.k < tokens;
+  auto find = [&](auto reaches) {  // calls reaches(bin, mass in front, tokens in front, mass, tokens) for this thread's bins
+    uint64_t vs = v0, ns = n0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      reaches(2 * (int)threadIdx.x + j, vs, ns, v[j], n[j]);
+      vs += v[j];
+      ns += n[j];
+    }
+  };
+  if (threadIdx.x == 0) bin_k = kBins;
+  __syncthreads();
+  if (by_k)
+    find([&](int bin, uint64_t vs, uint64_t ns, uint64_t vb, uint64_t nb) {
+      if (ns < (uint64_t)r.k && (uint64_t)r.k <= ns + nb) {
+        bin_k = bin;
+        k_mass = vs;
+        k_count = ns;
+        listed[0] = vs + vb;
+      }
+    });
+  __syncthreads();
+  const uint64_t least = by_k ? k_mass : mass, full = by_k ? listed[0] : mass;  // the k tokens weigh this much at least, at most
+  if (threadIdx.x == 0) {
+    bin_lo = by_k ? bin_k : kBins - 1;
+    bin_hi = bin_lo;
+    lo_mass = least;
+  }
+  __syncthreads();
+  if (r.by_p) {
+    const uint64_t t0 = share(r.p, least), t1 = share(r.p, full);
+    __syncthreads();
+    find([&](int bin, uint64_t vs, uint64_t, uint64_t vb, uint64_t) {
+      if (vs < t0 && t0 <= vs + vb && bin <= bin_k) {
+        bin_lo = bin;
+        lo_mass = vs;
+      }
+      if (vs < t1 && t1 <= vs + vb && bin <= bin_k) bin_hi = bin;
+    });
+    __syncthreads();
+  }
+  // All tokens up to the last border, where they are few; else the border bins' own.
+  const int last = by_k ? bin_k : bin_hi;
+  find([&](int bin, uint64_t, uint64_t ns, uint64_t, uint64_t nb) {
+    if (bin == last) listed[1] = ns + nb;
+  });
+  __syncthreads();
+  const bool whole_row = listed[1] <= kList;
+  auto border_bin = [&](int bin) { return (by_k && bin == bin_k) || (r.by_p && bin >= bin_lo && bin <= bin_hi); };
+  uint64_t borders = 0, border_tokens = 0;
+  find([&](int bin, uint64_t, uint64_t, uint64_t, uint64_t nb) { borders += border_bin(bin) ? nb : 0; });
+  block_scan(borders, m.part, &border_tokens);
+  if (!whole_row && !by_k && !r.by_p) {  // fewer than k tokens weigh anything
+    if (c == 0 && threadIdx.x == 0) {
+      s.cut_key = 0;
+      s.cut_index = 0;
+    }
+    return;
+  }
+  const bool fits = whole_row || border_tokens <= kList;
+  if (fits) {
+    const int end = min(a.V, (c + 1) * a.chunk);
+#pragma unroll 2
+    for (int i = c * a.chunk + 4 * threadIdx.x; i < end; i += 4 * kThreads) {
+      float l[4];
+      four<DT>(row, i, end, l);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double y = exponent(r, l[j]);
+        if (!(y < top)) continue;
+        const int bin = bin_of(y, scale);
+        if (whole_row ? bin <= last : border_bin(bin)) {
+          const uint32_t at = atomicAdd(&s.listed, 1u);  // the histogram has counted them: below kList
+          if (at < kList) s.list[at] = (uint64_t)key_of(l[j]) << 32 | (uint32_t)(i + j);
+        }
+      }
+    }
+  }
+  if (a.chunks > 1) {  // the workgroup that ends last goes on
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) m.last = atomicAdd(&s.ticket[0], 1u) == (uint32_t)a.chunks - 1;
+    __syncthreads();
+    if (!m.last) return;
+    __threadfence();
+  } else {
+    __syncthreads();
+  }
+  const int count = fits ? (int)(whole_row ? listed[1] : border_tokens) : 0;
+  for (int i = threadIdx.x; i < count; i += kThreads) m.list[i] = s.list[i];
+  __syncthreads();
+
+  // Calls f(key, index, weight, bin) for the collected tokens or, where they are too many for the list, for the border bins'.
+  auto each = [&](auto f) {
+    if (fits) {
+      for (int i = threadIdx.x; i < count; i += kThreads) {
+        const uint32_t key = (uint32_t)(m.list[i] >> 32);
+        const double y = exponent(r, of_key(key));
+        f(key, (uint32_t)m.list[i], weight(m.powers, y, a.bits), bin_of(y, scale));
+      }
+    } else {
+      for (int i = threadIdx.x; i < a.V; i += kThreads) {
+        const float l = one<DT>(row, i);
+        const double y = exponent(r, l);
+        if (!(y < top)) continue;
+        const int bin = bin_of(y, scale);
+        if (border_bin(bin)) f(key_of(l), (uint32_t)i, weight(m.powers, y, a.bits), bin);
+      }
+    }
+  };
+  auto mass_of = [&](uint32_t key) { return whole(weight(m.powers, exponent(r, of_key(key)), a.bits)); };
+  // the k-th token's key, and how many of that key are among the k
+  uint32_t cut = 0, at = 0;
+  uint64_t ties = ~0ull, before = 0, kept = mass;
+  if (by_k) {
+    const uint64_t need = (uint64_t)r.k - k_count;
+    border(m, need, [&](auto f) {
+      each([&](uint32_t key, uint32_t, double, int bin) {
+        if (bin == bin_k) f(~key, 1);
+      });
+    }, &at, &before);
+    cut = ~at;
+    ties = need - before;
+    uint64_t above = 0;
+    each([&](uint32_t key, uint32_t, double w, int bin) {
+      if (bin == bin_k && key > cut) above += whole(w);
+    });
+    block_scan(above, m.part, &kept);
+    kept += k_mass + ties * mass_of(cut);
+  }
+  if (r.by_p) {
+    const uint64_t need = share(r.p, kept);
+    if (need > lo_mass && border(m, need - lo_mass, [&](auto f) {
+          each([&](uint32_t key, uint32_t, double w, int bin) {
+            if (bin >= bin_lo && bin <= bin_hi) f(~key, whole(w));
+          });
+        }, &at, &before)) {
+      const uint32_t key = ~at;
+      const uint64_t each_one = max(mass_of(key), (uint64_t)1), some = (need - lo_mass - before + each_one - 1) / each_one;
+      if (key > cut || (key == cut && some < ties)) {
+        cut = key;
+        ties = some;
+      }
+    }
+  }
+  // the last one of the border's equals that is kept, if not all are
+  uint32_t cut_index = 0xffffffffu;
+  if (border(m, ties, [&](auto f) {
+        each([&](uint32_t key, uint32_t i, double, int) {
+          if (key == cut) f(i, 1);
+        });
+      }, &at, &before))
+    cut_index = at;
+  if (!whole_row) {
+    if (threadIdx.x == 0) {
+      s.cut_key = cut;
+      s.cut_index = cut_index;
+    }
+    return;
+  }
+  auto keeps = [&](uint32_t key, uint32_t i, double w) {
+    return (key > cut || (key == cut && i <= cut_index)) && w >= (double)r.minp * (double)(1ull << a.bits);
+  };
+  uint64_t mine = 0, total = 0;
+  each([&](uint32_t key, uint32_t i, double w, int) { mine += keeps(key, i, w) ? whole(w) : 0; });
+  block_scan(mine, m.part, &total);
+  border(m, drawn(a.u[b], total), [&](auto f) {
+    each([&](uint32_t key, uint32_t i, double w, int) {
+      if (keeps(key, i, w)) f(i, whole(w));
+    });
+  }, &at, &before);
+  if (threadIdx.x == 0) {
+    give(a, s, b, r, (int)at, one<DT>(row, (int)at));
+    s.done = 1;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sums in the order of the indexes
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs a) {
+  __shared__ Powers powers;
+  __shared__ uint64_t part[kWaves];
+  __shared__ int is_last, found;
+  __shared__ uint64_t found_before;
+  const int b = blockIdx.x / a.chunks, c = blockIdx.x - b * a.chunks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  RowState& s = reinterpret_cast<RowState*>(a.ws)[b];
+  Row r;
+  row_settings(a, b, r);
+  const void* row = row_of(a, b, DT);
+  const bool cuts = r.by_k || r.by_p;
+  if (!r.greedy && cuts && s.done) return;
+  row_extremes(a, s, r);
+  if (r.greedy || r.arg < 0) {  // the first of the largest, or none
+    if (c == 0 && threadIdx.x == 0) give(a, s, b, r, r.arg, r.max);
+    return;
+  }
+  powers.fill();
+  __syncthreads();
+  const uint32_t cut = cuts ? s.cut_key : 0, cut_index = cuts ? s.cut_index : 0;
+  const double top = most(a.bits), least = (double)r.minp * (double)(1ull << a.bits);
+  auto value = [&](float l, int i) -> uint64_t {  // what token i adds to the sum
+    const uint32_t key = key_of(l);
+    if (key < cut || (key == cut && (uint32_t)i > cut_index)) return 0;
+    const double y = exponent(r, l);
+    if (!(y < top)) return 0;
+    const double w = weight(powers, y, a.bits);
+    return w >= least ? whole(w) : 0;
+  };
+  // a wavefront sums up a stretch of its own
+  const int stretch = a.chunk / kWaves;
+  auto first_of = [&](int piece) { return piece * stretch; };
+  const int begin = first_of(c * kWaves + wave), end = min(a.V, begin + stretch);
+  uint64_t sum = 0;
+#pragma unroll 2
+  for (int i = begin + 4 * lane; i < end; i += 256) {
+    float l[4];
+    four<DT>(row, i, end, l);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += value(l[j], i + j);
+  }
+  sum = wave_sum64(sum);
+  if (lane == 0) s.wave_mass[c * kWaves + wave] = sum;
+  __threadfence();
+  __syncthreads();
+  if (a.chunks > 1) {
+    if (threadIdx.x == 0) is_last = atomicAdd(&s.ticket[1], 1u) == (uint32_t)a.chunks - 1;
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+  }
+  // the stretch in which the sum passes its mark, then the token: a thread takes some neighbours each
+  auto pick = [&](uint64_t v, uint64_t base, uint64_t target, int id) {  // the thread whose values reach it
+    uint64_t all;
+    const uint64_t before = base + block_scan(v, part, &all);
+    if (before < target && target <= before + v) {
+      found = id;
+      found_before = before;
+    }
+    __syncthreads();
+  };
+  const int pieces = a.chunks * kWaves;  // 1024 at most
+  const uint64_t mine = (int)threadIdx.x < pieces ? s.wave_mass[threadIdx.x] : 0;
+  uint64_t total;
+  block_scan(mine, part, &total);
+  const uint64_t target = drawn(a.u[b], total);
+  pick(mine, 0, target, threadIdx.x);
+  const int from = first_of(found), to = min(a.V, from + stretch), per = (stretch + kThreads - 1) / kThreads;
+  const uint64_t base = found_before;
+  const int i0 = from + (int)threadIdx.x * per, i1 = min(to, i0 + per);
+  uint64_t few = 0;
+  for (int i = i0; i < i1; ++i) few += value(one<DT>(row, i), i);
+  __syncthreads();
+  pick(few, base, target, threadIdx.x);
+  if (found == (int)threadIdx.x) {
+    uint64_t at = found_before;
+    for (int i = i0; i < i1; ++i) {
+      const float l = one<DT>(row, i);
+      at += value(l, i);
+      if (at >= target) {
+        give(a, s, b, r, i, l);
+        break;
+      }
+    }
+  }
+}
+
+// Chunks of whole 4096 columns, so that the rows fill the CUs about twice.
+size_t sample_plan(SampleArgs& a) {
+  const int64_t unit = 4 * kThreads, most_chunks = std::min<int64_t>(kMaxChunks, (a.V + unit - 1) / unit);
+  const int64_t chunks = std::min<int64_t>(most_chunks, std::max<int64_t>(1, 2 * (int64_t)device_cus() / std::max(a.B, 1)));
+  a.chunk = (int)(((a.V + chunks - 1) / chunks + unit - 1) / unit * unit);
+  a.chunks = (a.V + a.chunk - 1) / a.chunk;
+  int log = 0;
+  while ((1LL << log) < a.V) ++log;
+  a.bits = std::min(46, 62 - log);  // the sum of all weights stays below 2^63
+  return (size_t)a.B * sizeof(RowState);
+}
+
+hipError_t launch_sample(const SampleArgs& a, int dt, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.B * a.chunks)), block(kThreads);
+  auto go = [&](auto dt_tag) {
+    constexpr int DT = decltype(dt_tag)::value;
+    hipLaunchKernelGGL((sample_extremes_kernel<DT>), grid, block, 0, st, a);
+    if (a.cuts) {
+      hipLaunchKernelGGL((sample_histogram_kernel<DT>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((sample_borders_kernel<DT>), grid, block, 0, st, a);
+    }
+    hipLaunchKernelGGL((sample_sums_kernel<DT>), grid, block, 0, st, a);
+    note_kernel("sample_extremes_kernel%s + sample_sums_kernel chunks=%d",
+                a.cuts ? " + sample_histogram_kernel + sample_borders_kernel" : "", a.chunks);
+    return hipGetLastError();
+  };
+  if (dt == FG_F32) return go(std::integral_constant<int, FG_F32>{});
+  if (dt == FG_BF16) return go(std::integral_constant<int, FG_BF16>{});
+  return go(std::integral_constant<int, FG_F16>{});
+}
+
+}  // namespace fg

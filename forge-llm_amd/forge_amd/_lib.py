@@ -110,6 +110,8 @@ SIGNATURES = {
     "fg_mx_read": ([P, P, I32_, P, P, INT, I64, P], INT),
     "fg_mx_attention_workspace_bytes": ([I64, I64, I32_, I32_, I32_, I32_, I64, I64, I64, I32_], SZ),
     "fg_mx_attention": ([P, I64, I64, INT, P, P, I64, P, P, I64, I64, I32_, I64, I64, F32_, F32_, I64, P, I64, I64, P, P, SZ, P], INT),
+    "fg_sample_workspace_bytes": ([I64, I64], SZ),
+    "fg_sample_tokens": ([P, I64, INT, P, P, F32_, P, I32_, P, F32_, P, F32_, P, P, I64, I64, P, SZ, P], INT),
     "fg_version": ([], ctypes.c_char_p),
     "fg_last_error": ([], ctypes.c_char_p),
     "fg_last_kernel": ([], ctypes.c_char_p),

@@ -392,6 +392,25 @@ int fg_mx_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, c
                     size_t workspace_bytes, fg_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
+ * Tokens from their logits [B][V] (row stride ld; FG_F32 | FG_F16 | FG_BF16) and given random numbers u [B] in [0, 1).
+ * Row b's weights are exp((l_i - max l) / temperature).  Kept are the first top_k tokens in the order of their logits (equal ones by
+ * their index; top_k <= 0: all), of these the shortest beginning whose weight reaches top_p times theirs (top_p >= 1 or NaN: all, <= 0:
+ * one) and of these the ones that weigh min_p times the largest at least.  token[b] is the first, by index, at which
+ * the kept weights' sum passes u[b] times their total (u below 0 or NaN counts as 0, from 1 on gives the last).  A temperature
+ * of 0 or less (or NaN) gives the first of the largest logits.
+ * Logits of -inf and NaN weigh nothing; a row of nothing else gives -1.  Tokens that weigh less than 2^-47 (2^-31 at the
+ * least, for more than 2^16 tokens by as many powers of two less) of the largest are not drawn.
+ * logprob (may be NULL): float [B], the logarithm of softmax(l) at the token (temperature 1, all tokens); -inf for token -1, NaN
+ * in rows with a logit of +inf.
+ * temperature, top_k, top_p, min_p: device arrays of B, or NULL for the value that follows for all rows.
+ *   workspace: fg_sample_workspace_bytes bytes, 16-byte aligned. */
+size_t fg_sample_workspace_bytes(int64_t B, int64_t V);
+int fg_sample_tokens(const void* logits, int64_t ld, int dtype, const float* u, const float* temperature,
+                     float temperature_all, const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+                     const float* min_p, float min_p_all, int64_t* token, float* logprob, int64_t B, int64_t V,
+                     void* workspace, size_t workspace_bytes, fg_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
  * Library information.  fg_device_ok replaces the capability gate triton_usable (forge/kernels/ops_gemm.py:159-175):
  * returns 1 when `device` is a gfx950 GPU this build can run on, else 0 (message in fg_last_error).
  * ------------------------------------------------------------------------------------------------------------- */
