@@ -41,50 +41,46 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
   }
 }
 
-// Codes of 8 values as they lie in memory.  `fast`: div_by applies (finite values, a scale in its range).
+// Codes of 4 values as they lie in memory.  `fast`: div_by applies (finite values, a scale in its range).
 template <bool FP8>
-__device__ __forceinline__ uint2 encode8(const float (&v)[8], float scale, float y, bool fast) {
-  float c[8];
+__device__ __forceinline__ uint32_t encode4(const float* v, float scale, float y, bool fast) {
+  float d[4];
   if (fast) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const float q = div_by(v[i], scale, y);
       // the corrections turn -0 into +0; an e4m3 code keeps the sign of a zero
-      c[i] = FP8 ? __builtin_copysignf(fminf(fmaxf(q, -448.f), 448.f), v[i]) : fminf(fmaxf(q, -127.f), 127.f);
+      d[i] = FP8 ? __builtin_copysignf(fminf(fmaxf(q, -448.f), 448.f), v[i]) : fminf(fmaxf(q, -127.f), 127.f);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const float q = __fdiv_rn(v[i], scale);
       if (FP8)
-        c[i] = __builtin_isnan(q) ? q : fminf(fmaxf(q, -448.f), 448.f);
+        d[i] = __builtin_isnan(q) ? q : fminf(fmaxf(q, -448.f), 448.f);
       else
-        c[i] = __builtin_isnan(q) ? 0.f : fminf(fmaxf(q, -127.f), 127.f);
+        d[i] = __builtin_isnan(q) ? 0.f : fminf(fmaxf(q, -127.f), 127.f);
     }
   }
-  uint32_t w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float* d = c + 4 * h;
-    if (FP8) {
-      if (fast) {
-        int p = __builtin_amdgcn_cvt_pk_fp8_f32(d[0], d[1], 0, false);
-        p = __builtin_amdgcn_cvt_pk_fp8_f32(d[2], d[3], p, true);
-        w[h] = (uint32_t)p;
-      } else {
-        w[h] = (uint32_t)f32_to_e4m3(d[0]) | (uint32_t)f32_to_e4m3(d[1]) << 8 | (uint32_t)f32_to_e4m3(d[2]) << 16 |
-               (uint32_t)f32_to_e4m3(d[3]) << 24;
-      }
-    } else {
-      // |d| <= 127: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low byte
-      uint32_t b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(d[i] + 12582912.f);
-      w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u),
-                                   __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), 0x05040100u);
+  if (FP8) {
+    if (fast) {
+      const int p = __builtin_amdgcn_cvt_pk_fp8_f32(d[0], d[1], 0, false);
+      return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(d[2], d[3], p, true);
     }
+    return (uint32_t)f32_to_e4m3(d[0]) | (uint32_t)f32_to_e4m3(d[1]) << 8 | (uint32_t)f32_to_e4m3(d[2]) << 16 |
+           (uint32_t)f32_to_e4m3(d[3]) << 24;
   }
-  return make_uint2(w[0], w[1]);
+  // |d| <= 127: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low byte
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(d[i] + 12582912.f);
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u),
+                               __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), 0x05040100u);
+}
+
+template <bool FP8>
+__device__ __forceinline__ uint2 encode8(const float (&v)[8], float scale, float y, bool fast) {
+  return make_uint2(encode4<FP8>(v, scale, y, fast), encode4<FP8>(v + 4, scale, y, fast));
 }
 
 __device__ __forceinline__ void load8_f(const void* p, int dt, int64_t i, float (&f)[8]) {

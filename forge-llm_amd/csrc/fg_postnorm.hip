@@ -1,5 +1,6 @@
 // The step between two blocks of a decoder layer that norms a block's output as well as the next one's input, one row in one pass:
-//   b = x / sqrt(mean(x^2) + eps_post) * post_weight * residual_scale * gate      fp32, in this order
+//   b = x / sqrt(mean(x^2) + eps_post) * post_weight * residual_scale * gate      fp32, in this order, an IEEE quotient: a sum next
+//                                          to a border of the residual's type goes to the side that the same steps one by one give
 //   h = rnd(r + b)                         rounded to the residual's type; the new residual
 //   y = (h w) / sqrt(mean(h^2) + eps)      fp32, stored in x's type or as codes, as add_rmsnorm does
 //
@@ -10,9 +11,16 @@
 
 namespace fg {
 
-template <int XT, int RT, int C>
+constexpr int kStrides = 4096;  // columns of a row whose squares are added up by strides
+
+// STRIDES: the squares of x are added up in the order of a wavefront that reads four columns a lane, columns 256 apart one after the
+// other, then each four neighbours, then lanes, neighbours first.  It is the order in which the sum of such rows is taken where the
+// steps run one by one, so that rms, and with it every h next to a border of its type, comes out the same to the bit; x goes through
+// LDS for it (8192 x 4096 in bf16 to e4m3 blocks: 60 us either way).
+template <int XT, int RT, int C, bool STRIDES>
 __global__ void __launch_bounds__(1024) postnorm_add_rmsnorm_kernel(const PostNormArgs p) {
-  __shared__ float red_post[16];
+  __shared__ __align__(16) float red_post[STRIDES ? 256 : 16];
+  __shared__ __align__(16) uint8_t kept_x[STRIDES ? kStrides * (XT == FG_F32 ? 4 : 2) : 16];
   __shared__ NormRed red;
   const NormArgs& a = p.norm;
   const int64_t row = blockIdx.x;
@@ -42,22 +50,54 @@ __global__ void __launch_bounds__(1024) postnorm_add_rmsnorm_kernel(const PostNo
   };
   if (kEarly && K > at(0)) factors(0);
   float ss = 0.f;
+  if constexpr (STRIDES) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    if (K <= at(c)) continue;
-    float x[8];
-    widen8<XT>(xv[c], x);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(x[j], x[j], ss);
-  }
-  ss = wave_sum(ss);
-  if (waves > 1) {
-    if (lane == 0) red_post[wave] = ss;
+    for (int c = 0; c < C; ++c)
+      if (K > at(c)) {
+        uint4* to = reinterpret_cast<uint4*>(kept_x + at(c) * (XT == FG_F32 ? 4 : 2));  // a row's last unit ends in zeros
+        to[0] = make_uint4(xv[c].w[0][0], xv[c].w[0][1], xv[c].w[0][2], xv[c].w[0][3]);
+        if constexpr (XT == FG_F32) to[1] = make_uint4(xv[c].w[1][0], xv[c].w[1][1], xv[c].w[1][2], xv[c].w[1][3]);
+      }
     __syncthreads();
-    ss = red_post[0];
-    for (int i = 1; i < waves; ++i) ss += red_post[i];
+    for (int r = threadIdx.x; r < 256; r += T) {
+      float sum = 0.f;
+      for (int i = r; i < K; i += 1024) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = load_f(kept_x, XT, i + 256 * j);
+          sum += i + 256 * j < K ? x * x : 0.f;
+        }
+      }
+      red_post[r] = sum;
+    }
+    __syncthreads();
+    const float4 four = reinterpret_cast<const float4*>(red_post)[lane];
+    ss = ((four.x + four.y) + four.z) + four.w;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) ss += __shfl_xor(ss, off, kWave);
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (K <= at(c)) continue;
+      float x[8];
+      widen8<XT>(xv[c], x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(x[j], x[j], ss);
+    }
+    ss = wave_sum(ss);
+    if (waves > 1) {
+      if (lane == 0) red_post[wave] = ss;
+      __syncthreads();
+      ss = red_post[0];
+      for (int i = 1; i < waves; ++i) ss += red_post[i];
+    }
   }
-  const float rs = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)K) + p.eps_post));
+  // x / rms by multiply-adds: both by the power of two that brings rms into their range; one that is infinite gives zeros
+  float rms = __builtin_sqrtf(__fdiv_rn(ss, (float)K) + p.eps_post);
+  const float by = div_by_ok(rms) ? 1.f : (rms > 1.f ? 0x1p-64f : 0x1p64f);
+  rms *= by;
+  const float rs = __fdiv_rn(1.f, rms);
+  rms = rms == __builtin_inff() ? 0.f : rms;
   float t[C][8];
   uint32_t m[C];
   ss = 0.f;
@@ -75,7 +115,7 @@ __global__ void __launch_bounds__(1024) postnorm_add_rmsnorm_kernel(const PostNo
     widen8<XT>(xv[c], x);
     widen8<RT>(rv[c], h);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] += x[j] * rs * pw[j] * p.scale * g[j];
+    for (int j = 0; j < 8; ++j) h[j] += div_by(x[j] * by, rms, rs) * pw[j] * p.scale * g[j];
     const Raw8<RT> kept = narrow8<RT>(h);
     widen8<RT>(kept, h);
     store_raw8<RT>(hrow, at(c), n, kept);
@@ -96,7 +136,11 @@ hipError_t launch_postnorm_add_rmsnorm(const PostNormArgs& p, int xdt, int rdt, 
   auto go = [&](auto x_tag, auto r_tag, auto c_tag) {
     constexpr int XT = decltype(x_tag)::value, RT = decltype(r_tag)::value, CC = decltype(c_tag)::value;
     note_kernel("postnorm_add_rmsnorm_kernel<%d,%d,%d> T=%d", XT, RT, CC, T);
-    hipLaunchKernelGGL((postnorm_add_rmsnorm_kernel<XT, RT, CC>), dim3((unsigned)M), dim3(T), 0, st, p);
+    // two units a thread: the rows are many
+    if (CC == 2 && p.norm.K % 4 == 0 && p.norm.K <= kStrides)
+      hipLaunchKernelGGL((postnorm_add_rmsnorm_kernel<XT, RT, CC, CC == 2>), dim3((unsigned)M), dim3(T), 0, st, p);
+    else
+      hipLaunchKernelGGL((postnorm_add_rmsnorm_kernel<XT, RT, CC, false>), dim3((unsigned)M), dim3(T), 0, st, p);
     return hipGetLastError();
   };
   auto pick = [&](auto x_tag, auto r_tag) {

@@ -69,7 +69,8 @@ def _check(x, pw, r, w, gate, got, quant, scale=1.0, block=128, post_eps=EPS):
         assert bool(((got.y.cpu().float().double() - ratio).abs() <= ratio.abs() * (2.0 ** -4 + 4 * REL) + 2.0 ** -10).all())
 
 
-SHAPES = [(1, 1), (3, 7), (2, 8), (5, 9), (4, 511), (4, 512), (3, 520), (1, 4096), (2, 5001), (3, 8200), (1, 32768), (600, 1000)]
+SHAPES = [(1, 1), (3, 7), (2, 8), (5, 9), (4, 511), (4, 512), (3, 520), (1, 4096), (2, 5001), (3, 8200), (1, 32768), (600, 1000),
+          (601, 7), (515, 256), (520, 1028), (530, 2049), (514, 4096), (513, 4097)]  # many rows: their squares by strides up to 4096
 
 
 @pytest.mark.parametrize("quant", QUANTS)
@@ -83,7 +84,7 @@ def test_against_the_definition(dt, rdt, quant):
 
 @pytest.mark.parametrize("block", [8, 64, 512])
 def test_blocks_and_another_epsilon(block):
-    for m, k in ((3, 1000), (700, 640)):
+    for m, k in ((3, 1000), (700, 640), (700, 2500)):
         x, pw, r, w, gt = _data(m, k, BF, BF, "rows")
         got = _run(x, pw, r, w, gt, quant="fp8_block", block=block, post_eps=0.1)
         assert got.scale.shape == (m, -(-k // block))
@@ -175,3 +176,14 @@ def test_refusals():
     long = torch.zeros(1, 32769, dtype=BF, device=DEV)
     with pytest.raises(Exception, match="32768"):
         ops.postnorm_add_rmsnorm(long, None, long, None)
+
+
+@pytest.mark.parametrize("m,k", [(600, 1024), (600, 1000), (520, 4096)])
+def test_many_rows_as_the_steps_one_by_one(m, k):
+    """Up to 4096 columns the squares are added up in the order of torch's own sum: the same quotients, and the residual to the bit."""
+    x, pw, r, w, gt = (None if t is None else t.to(DEV) for t in _data(m, k, BF, BF, "columns"))
+    xf = x.float()
+    b = xf / torch.sqrt((xf * xf).mean(-1, keepdim=True) + EPS) * pw.float() * 0.5 * gt.float()
+    got = ops.postnorm_add_rmsnorm(x, pw, r, w, gate=gt, residual_scale=0.5, eps=EPS)
+    # fp32 sums that differ in their last place in some rows would show in one of 2^13 residuals or so
+    assert int((got.residual != (r.float() + b).to(BF)).sum()) <= m * k // 2 ** 13
