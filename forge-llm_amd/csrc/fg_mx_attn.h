@@ -17,6 +17,7 @@ struct MxAttnArgs {
   float cap_in;            // CAP: a score s becomes tanh(s cap_in), in units of the cap
   float factor;            // what makes that, or a score, an exponent of 2
   bool tile;               // whether mx_tile takes the rows, or mx_rows
+  int page_shift;          // log2 of the page size, -1: no power of two
 };
 
 constexpr int kNoWindow = 1 << 30;
@@ -24,18 +25,23 @@ constexpr int kNoWindow = 1 << 30;
 size_t mx_attn_plan(MxAttnArgs& m);
 hipError_t launch_mx_attn(MxAttnArgs& m, bool bf16, void* ws, size_t bytes, hipStream_t st);
 
-// The keys [begin, end) that some of a tile's rows see: the tokens a0 .. a1 of the sequence's, of which token i sees seen0 + i
-// keys from the front, but the last `window` of them.
+// The keys [low, end) that some of a tile's rows see: the tokens a0 .. a1 of the sequence's, of which token i sees seen0 + i keys from
+// the front, but the last `window` of them.  begin: low down to a whole tile, so that tiles do not cross the pages' sixteens.
 struct MxRange {
-  int begin, end;
+  int begin, low, end;
 };
 __device__ __forceinline__ MxRange mx_range(const MxAttnArgs& m, int len, int seen0, int a0, int a1) {
-  return {max(seen0 + a0 - m.window, 0), max(min(seen0 + a1, len), 0)};
+  const int low = max(seen0 + a0 - m.window, 0);
+  return {low & ~31, low, max(min(seen0 + a1, len), 0)};
 }
+
+struct MxItem : AttnItem {
+  int low;  // keys in front of it are nobody's
+};
 
 // Item `id` of the grid; false: nothing to do.  TILE rows per item.
 template <int TILE>
-__device__ __forceinline__ bool mx_item(const MxAttnArgs& m, int id, AttnItem& it) {
+__device__ __forceinline__ bool mx_item(const MxAttnArgs& m, int id, MxItem& it) {
   const AttnArgs& a = m.a;
   const int tiles = a.tiles_s, pairs = a.parts_s * a.Hk * a.B;
   int pair, tile;
@@ -47,7 +53,9 @@ __device__ __forceinline__ bool mx_item(const MxAttnArgs& m, int id, AttnItem& i
     pair = id / tiles;
     tile = id % tiles;
   }
-  const int rest = pair / a.Hk, seq = rest / a.parts_s, part = rest - seq * a.parts_s;
+  // Workgroups go to the shader engines in turn and wait for theirs: sequences begin with another part each, so that the parts that
+  // short ones lack do not always fall to the same engine (64 sequences of 2048 to 16384 tokens in 8 parts: 2 to 15 items per CU).
+  const int rest = pair / a.Hk, seq = rest / a.parts_s, part = (rest - seq * a.parts_s + seq) % a.parts_s;
   tile = tiles - 1 - tile;  // the tiles that see the most first
   int t0 = seq, n = 1;      // the sequence's query tokens
   if (a.starts) {
@@ -66,6 +74,7 @@ __device__ __forceinline__ bool mx_item(const MxAttnArgs& m, int id, AttnItem& i
   const MxRange all = mx_range(m, len, it.seen0, it.row0 / a.G, min(it.rows - 1, it.row0 + TILE - 1) / a.G);
   it.begin = all.begin + part * a.part_s;
   it.end = min(it.begin + a.part_s, all.end);
+  it.low = all.low;
   it.causal = true;
   it.table = a.pages + seq * a.ld_pages;
   it.slot = part;

@@ -45,13 +45,17 @@ size_t mx_attn_plan(MxAttnArgs& m) {
   const int64_t rows = (int64_t)a.max_q * a.G, cus = device_cus();
   m.tile = rows > 16;
   const int64_t tile = m.tile ? kTileRows : 16, tokens = std::min<int64_t>(a.max_q, tile / a.G + 2);
-  const int64_t span = std::min<int64_t>(a.max_len, (int64_t)m.window + tokens - 1);  // keys that a tile's rows see at most
+  // keys that a tile's rows see at most, from a whole tile of 32 on
+  const int64_t span = std::min<int64_t>(a.max_len, (int64_t)m.window + tokens + 30);
   a.tiles_s = (int)((rows + tile - 1) / tile);
   const int64_t sets = (int64_t)a.Hk * a.B, items = std::max<int64_t>(sets * a.tiles_s, 1), unit = m.tile ? 64 : kRowsTile * kRowsWaves;
-  // about two workgroups per CU
+  // About two workgroups per CU: us by keys per part, 32 + 2 x 8 heads of 128 in 4 bits, 1 sequence of 5000 128 / 256 / 512: 11.6 / 10.9 /
+  // 12.0, 4 of 16000 512 / 1024: 20.0 / 19.6, 16 of 4000 with 4 queries each 512 / 1024: 21.2 / 20.5.  Where the sequences fill the
+  // CUs by themselves, parts of up to 4096 keys, so that long ones do not outlast the others (64 of 2048 to 16384, 64 + 2 x 8 heads,
+  // 16384 / 4096 / 2048: 170 / 148 / 150; up to 4000 keys one part: 2 parts of 256 columns 129, one 108).
   int64_t parts = std::max<int64_t>(1, 2 * cus / items);
-  if (!m.tile) parts = std::max<int64_t>(parts, (span + kMaxPart - 1) / kMaxPart);
-  const int64_t part = std::max<int64_t>(unit, ((span + parts - 1) / parts + unit - 1) / unit * unit);
+  if (!m.tile) parts = std::max<int64_t>(parts, (span + 4095) / 4096);
+  const int64_t part = std::max<int64_t>(m.tile ? 64 : 256, ((span + parts - 1) / parts + unit - 1) / unit * unit);
   a.part_s = (int)part;
   a.parts_s = (int)std::max<int64_t>(1, (span + part - 1) / part);
   const int64_t all = attn_count(a.parts_s * sets, a.tiles_s);
@@ -67,6 +71,7 @@ hipError_t launch_mx_attn_fp16(const MxAttnArgs& m, hipStream_t st);
 // A planned call; `bytes`: what mx_attn_plan returned for it.
 hipError_t launch_mx_attn(MxAttnArgs& m, bool bf16, void* ws, size_t bytes, hipStream_t st) {
   AttnArgs& a = m.a;
+  m.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz((unsigned)a.page) : -1;
   a.acc = nullptr;
   a.ml = nullptr;
   if (bytes) {

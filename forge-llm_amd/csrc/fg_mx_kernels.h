@@ -13,7 +13,8 @@ static hipError_t launch_mx_items(const MxAttnArgs& m, hipStream_t st) {
     constexpr int BITS = decltype(bits_tag)::value, DP = decltype(d_tag)::value;
     constexpr bool CAP = decltype(c_tag)::value;
     if (m.tile) hipLaunchKernelGGL((mx_tile_kernel<BF16, BITS, CAP, DP>), grid, block, 0, st, m);
-    else hipLaunchKernelGGL((mx_rows_kernel<BF16, BITS, CAP, DP>), grid, block, 0, st, m);
+    else if (m.a.page % 16 == 0 && m.a.c_token < 1u << 24) hipLaunchKernelGGL((mx_rows_kernel<BF16, BITS, CAP, DP, true>), grid, block, 0, st, m);
+    else hipLaunchKernelGGL((mx_rows_kernel<BF16, BITS, CAP, DP, false>), grid, block, 0, st, m);
     return hipGetLastError();
   };
   auto by_d = [&](auto bits_tag, auto c_tag) {

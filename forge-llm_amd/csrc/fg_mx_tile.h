@@ -20,14 +20,14 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) mx_tile_kernel(const Mx
   uint32_t* tab = reinterpret_cast<uint32_t*>(lds + TileLds<DP>::kTab);
   const AttnArgs& a = m_.a;
 
-  AttnItem it;
+  MxItem it;
   if (!mx_item<kTileRows>(m_, blockIdx.x, it)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, l32 = lane & 31, half = lane >> 5;
   const int n = max(it.end - it.begin, 0), tiles = (n + KT - 1) / KT;
   auto fill = [&](int from) {  // kTabHalf entries of the row table
     for (int i = from + threadIdx.x; i < from + kTabHalf; i += 256) {
       if (i >= tiles * KT) break;
-      tab[i % (2 * kTabHalf)] = i < n ? attn_row(a, it, it.begin + i) : kNoRow;
+      tab[i % (2 * kTabHalf)] = i < n && it.begin + i >= it.low ? attn_row(a, it, it.begin + i) : kNoRow;
     }
   };
   fill(0);
