@@ -51,10 +51,11 @@ size_t mx_attn_plan(MxAttnArgs& m) {
   const int64_t sets = (int64_t)a.Hk * a.B, items = std::max<int64_t>(sets * a.tiles_s, 1), unit = m.tile ? 64 : kRowsTile * kRowsWaves;
   // About two workgroups per CU: us by keys per part, 32 + 2 x 8 heads of 128 in 4 bits, 1 sequence of 5000 128 / 256 / 512: 11.6 / 10.9 /
   // 12.0, 4 of 16000 512 / 1024: 20.0 / 19.6, 16 of 4000 with 4 queries each 512 / 1024: 21.2 / 20.5.  Where the sequences fill the
-  // CUs by themselves, parts of up to 4096 keys, so that long ones do not outlast the others (64 of 2048 to 16384, 64 + 2 x 8 heads,
-  // 16384 / 4096 / 2048: 170 / 148 / 150; up to 4000 keys one part: 2 parts of 256 columns 129, one 108).
+  // CUs by themselves one part does, but for long ones, which would outlast the others: parts of 2048 keys (64 of 2048 to 16384, 64 +
+  // 2 x 8 heads, 16384 / 4096 / 2048: 170 / 148 / 150; 64 of up to 8000 x 64 columns 8000 / 4096 / 2048: 58 / 66 / 56; 64 of up to
+  // 4000 x 256 columns 4000 / 2048: 108 / 129).
   int64_t parts = std::max<int64_t>(1, 2 * cus / items);
-  if (!m.tile) parts = std::max<int64_t>(parts, (span + 4095) / 4096);
+  if (!m.tile && span > 8192) parts = std::max<int64_t>(parts, (span + 2047) / 2048);
   const int64_t part = std::max<int64_t>(m.tile ? 64 : 256, ((span + parts - 1) / parts + unit - 1) / unit * unit);
   a.part_s = (int)part;
   a.parts_s = (int)std::max<int64_t>(1, (span + part - 1) / part);

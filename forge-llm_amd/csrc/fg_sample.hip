@@ -50,6 +50,7 @@ struct Row {
   bool greedy, by_k, by_p;
   float max, min;
   int arg;
+  float sum;     // of exp(l - max)
   double scale;  // log2(e) / T
 };
 
@@ -120,6 +121,12 @@ __device__ __forceinline__ double exponent(const Row& r, float l) {
   if (l == r.max) return 0;
   return ((double)r.max - (double)l) * r.scale;
 }
+// A logit that no logit of an exponent of y or less is below: what is, needs no fp64.
+__device__ __forceinline__ float floor_of(const Row& r, double y) {
+  const double l = (double)r.max - y / r.scale;  // infinite or no number: nothing is said
+  const float f = (float)(l - 1e-6 * (fabs(l) + fabs((double)r.max) + 1));
+  return f == f ? f : -__builtin_inff();
+}
 __device__ __forceinline__ double most(int bits) { return bits + 1; }  // from here on a weight is no unit
 
 __device__ __forceinline__ double bin_scale(const Row& r, int bits) {
@@ -140,17 +147,26 @@ __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
   return v;
 }
 
-// Sum of the threads' values in front of this one; `all`: of all.  Two barriers.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* part, uint64_t* all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// A wavefront's own: sum of the lanes' values in front of this one; `all`: of all.
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v, uint64_t* all) {
+  const int lane = threadIdx.x & 63;
   uint64_t s = v;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const uint64_t o = shfl_up64(s, d);
     if (lane >= d) s += o;
   }
+  *all = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(s >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)s, 63);
+  return s - v;
+}
+
+// Sum of the threads' values in front of this one; `all`: of all.  Two barriers.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* part, uint64_t* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t mine;
+  const uint64_t in_front = wave_scan(v, &mine);
   __syncthreads();  // the last call's sums have been read
-  if (lane == 63) part[wave] = s;
+  if (lane == 0) part[wave] = mine;
   __syncthreads();
   uint64_t before = 0, sum = 0;
 #pragma unroll
@@ -159,7 +175,7 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* part, uint6
     sum += part[w];
   }
   *all = sum;
-  return before + s - v;
+  return before + in_front;
 }
 
 __device__ __forceinline__ void row_settings(const SampleArgs& a, int b, Row& r) {
@@ -174,23 +190,54 @@ __device__ __forceinline__ void row_settings(const SampleArgs& a, int b, Row& r)
   r.scale = 1.4426950408889634 / (double)r.t;
 }
 
-// The row's extremes from its chunks'; every thread has them.
+// What a row's workgroups hand to the one that ends last goes past the XCDs' L2 caches both ways (a fence would write each whole
+// cache back, once for every workgroup: 32 rows of 128000 357 us, now 87), and is in memory when the wavefront's wait is over.
+template <class T>
+__device__ __forceinline__ void put_far(T* p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class T>
+__device__ __forceinline__ T get_far(const T* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Whether this workgroup is the last of its row's; what the others have put far can be got.  Every thread is there.
+__device__ __forceinline__ bool last_of_row(uint32_t* ticket, int chunks, int* shared) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    *shared = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)chunks - 1;
+  __syncthreads();
+  return *shared;
+}
+
+// The row's extremes from its chunks', a lane each; every thread has them.
+static_assert(kMaxChunks <= 64, "a lane for each chunk");
 __device__ __forceinline__ void row_extremes(const SampleArgs& a, const RowState& s, Row& r) {
-  r.max = -__builtin_inff();
-  r.min = __builtin_inff();
-  r.arg = -1;
-  for (int c = 0; c < a.chunks; ++c) {
-    const ChunkSum p = s.part[c];
-    if (p.arg >= 0 && (r.arg < 0 || p.max > r.max)) {
-      r.max = p.max;
-      r.arg = p.arg;
+  const int lane = threadIdx.x & 63;
+  ChunkSum p = {-__builtin_inff(), __builtin_inff(), -1, 0.f};
+  if (lane < a.chunks) p = s.part[lane];
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    if (d >= a.chunks) break;
+    const float mx = __shfl_xor(p.max, d, kWave), sum = __shfl_xor(p.sum, d, kWave);
+    const int arg = __shfl_xor(p.arg, d, kWave);
+    if (arg >= 0) {
+      const float most = fmaxf(p.max, mx), log2e = 1.4426950408889634f;
+      const float own = p.arg < 0 ? 0.f : p.sum * __builtin_amdgcn_exp2f((p.max - most) * log2e);
+      p.sum = own + sum * __builtin_amdgcn_exp2f((mx - most) * log2e);
+      if (p.arg < 0 || mx > p.max || (mx == p.max && arg < p.arg)) p.arg = arg;
+      p.max = most;
     }
-    r.min = fminf(r.min, p.min);
+    p.min = fminf(p.min, __shfl_xor(p.min, d, kWave));
   }
+  r.max = __shfl(p.max, 0, kWave);
+  r.min = __shfl(p.min, 0, kWave);
+  r.arg = __shfl(p.arg, 0, kWave);
+  r.sum = __shfl(p.sum, 0, kWave);
 }
 
 // Token i of logit l for row b.
-__device__ __forceinline__ void give(const SampleArgs& a, const RowState& s, int b, const Row& r, int i, float l) {
+__device__ __forceinline__ void give(const SampleArgs& a, int b, const Row& r, int i, float l) {
   a.token[b] = i;
   if (!a.logprob) return;
   if (i < 0) {
@@ -201,10 +248,7 @@ __device__ __forceinline__ void give(const SampleArgs& a, const RowState& s, int
     a.logprob[b] = __builtin_nanf("");
     return;
   }
-  float sum = 0.f;
-  for (int c = 0; c < a.chunks; ++c)
-    if (s.part[c].arg >= 0) sum += s.part[c].sum * __builtin_amdgcn_exp2f((s.part[c].max - r.max) * 1.4426950408889634f);
-  a.logprob[b] = (l - r.max) - __builtin_amdgcn_logf(sum) * 0.69314718055994531f;
+  a.logprob[b] = (l - r.max) - __builtin_amdgcn_logf(r.sum) * 0.69314718055994531f;
 }
 
 __device__ __forceinline__ const void* row_of(const SampleArgs& a, int b, int dt) {
@@ -305,7 +349,8 @@ __global__ void __launch_bounds__(kThreads) sample_histogram_kernel(const Sample
       const double y = exponent(r, l[j]);
       if (!(y < top)) continue;
       const int bin = bin_of(y, scale);
-      atomicAdd(reinterpret_cast<unsigned long long*>(&mass[bin]), (unsigned long long)whole(weight(powers, y, a.bits)));
+      // without top-p nobody asks what the bins weigh
+      if (r.by_p) atomicAdd(reinterpret_cast<unsigned long long*>(&mass[bin]), (unsigned long long)whole(weight(powers, y, a.bits)));
       atomicAdd(&count[bin], 1u);
     }
   }
@@ -329,21 +374,43 @@ struct Shared {
   uint64_t list[kList];
   uint64_t part[kWaves];
   Powers powers;
-  uint64_t found[4];
-  uint32_t lo, hi;
+  uint64_t found[3];
+  uint32_t lo[kWaves], hi[kWaves];
   int last;
+  // the borders' bins, the tokens and the weight in front of them and in them
+  int bin_k, bin_lo, bin_hi;
+  uint64_t k_mass, k_full, lo_mass;
+  uint32_t k_count, k_tokens, lo_count, hi_count;
+  uint32_t listed, place;
 };
 
-// The smallest coordinate at which the sum of the values of the elements up to there reaches `target`, and the sum in front of
-// it.  each(f) calls f(coordinate, value) for the elements; false: the sum of all of them does not reach it.
-template <class Each>
-__device__ __forceinline__ bool border(Shared& m, uint64_t target, const Each& each, uint32_t* at, uint64_t* before) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    m.lo = 0xffffffffu;
-    m.hi = 0;
+// Where a row is settled: by a workgroup, or by one wavefront, which needs no barrier, where its tokens are few.
+template <bool WAVE>
+__device__ __forceinline__ void together() {
+  if constexpr (WAVE) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
   }
-  __syncthreads();
+}
+template <bool WAVE>
+__device__ __forceinline__ uint64_t scan(uint64_t v, uint64_t* part, uint64_t* all) {
+  if constexpr (WAVE) return wave_scan(v, all);
+  else return block_scan(v, part, all);
+}
+
+// The smallest coordinate at which the sum of the values of the elements up to there reaches `target`; the sum in front of it, and what
+// it has itself: by histograms, each over a bin of the one before (2048 bins of a workgroup, 64 of a wavefront).  each(f) calls
+// f(coordinate, value) for the elements; false: the sum of all of them does not reach it.
+struct Border {
+  uint32_t at;
+  uint64_t before, here;
+};
+template <bool WAVE, class Each>
+__device__ __forceinline__ bool border(Shared& m, uint64_t target, const Each& each, Border* found) {
+  constexpr int kPer = WAVE ? 1 : kBins / kThreads, kLog = WAVE ? 6 : 11;  // bins of a thread, of all
+  const int me = WAVE ? threadIdx.x & 63 : threadIdx.x;
   uint32_t lo = 0xffffffffu, hi = 0;
   each([&](uint32_t c, uint64_t) {
     lo = min(lo, c);
@@ -354,48 +421,58 @@ __device__ __forceinline__ bool border(Shared& m, uint64_t target, const Each& e
     lo = min(lo, (uint32_t)__shfl_xor((int)lo, d, kWave));
     hi = max(hi, (uint32_t)__shfl_xor((int)hi, d, kWave));
   }
-  if ((threadIdx.x & 63) == 0 && lo <= hi) {
-    atomicMin(&m.lo, lo);
-    atomicMax(&m.hi, hi);
+  if constexpr (!WAVE) {
+    __syncthreads();  // what an earlier call left in m has been read
+    if ((threadIdx.x & 63) == 0) {
+      m.lo[threadIdx.x >> 6] = lo;
+      m.hi[threadIdx.x >> 6] = hi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      lo = min(lo, m.lo[w]);
+      hi = max(hi, m.hi[w]);
+    }
   }
-  __syncthreads();
-  lo = m.lo;
-  hi = m.hi;
   uint64_t base = 0;
   if (lo > hi) return false;
   for (;;) {
-    const int width = 32 - __clz((int)(hi - lo)), shift = width > 11 ? width - 11 : 0;  // (hi - lo) >> shift < 2048
-    for (int i = threadIdx.x; i < kBins; i += kThreads) m.mass[i] = 0;
-    if (threadIdx.x == 0) m.found[0] = ~0ull;
-    __syncthreads();
+    const int width = 32 - __clz((int)(hi - lo)), shift = width > kLog ? width - kLog : 0;  // (hi - lo) >> shift < 2^kLog
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) m.mass[me * kPer + j] = 0;
+    if (me == 0) m.found[0] = ~0ull;
+    together<WAVE>();
     each([&](uint32_t c, uint64_t v) {
       if (c >= lo && c <= hi) atomicAdd(reinterpret_cast<unsigned long long*>(&m.mass[(c - lo) >> shift]), (unsigned long long)v);
     });
-    __syncthreads();
-    uint64_t v[2], all;
+    together<WAVE>();
+    uint64_t v[kPer], sum = 0, all;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) v[j] = m.mass[2 * threadIdx.x + j];
-    uint64_t sum = base + block_scan(v[0] + v[1], m.part, &all);
+    for (int j = 0; j < kPer; ++j) {
+      v[j] = m.mass[me * kPer + j];
+      sum += v[j];
+    }
+    sum = base + scan<WAVE>(sum, m.part, &all);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < kPer; ++j) {
       if (sum < target && target <= sum + v[j]) {
-        m.found[0] = 2 * threadIdx.x + j;
+        m.found[0] = me * kPer + j;
         m.found[1] = sum;
+        m.found[2] = v[j];
       }
       sum += v[j];
     }
-    __syncthreads();
-    const uint64_t bin = m.found[0];
+    together<WAVE>();
+    const uint64_t bin = m.found[0], here = m.found[2];
     if (bin == ~0ull) return false;
     base = m.found[1];
     lo += (uint32_t)bin << shift;
     if (shift == 0) {
-      *at = lo;
-      *before = base;
+      *found = {lo, base, here};
       return true;
     }
     hi = (uint32_t)min((uint64_t)hi, (uint64_t)lo + ((1u << shift) - 1));
-    __syncthreads();
+    together<WAVE>();
   }
 }
 
@@ -404,10 +481,135 @@ __device__ __forceinline__ uint64_t share(float p, uint64_t s) {
   const double v = ceil((double)p * (double)s);
   return v > 1 ? min((uint64_t)v, s) : 1;
 }
+// Whether a token weighs min_p of the largest.
+__device__ __forceinline__ bool weighs(const Row& r, const Powers& t, double y, int bits) {
+  return !(r.minp > 0.f) || weight(t, y, bits) >= (double)r.minp * (double)(1ull << bits);
+}
 // What the kept weights' sum has to reach: the first whole number past u times the total.
 __device__ __forceinline__ uint64_t drawn(float u, uint64_t total) {
   const double v = floor((double)u * (double)total);
   return v > 0 ? min((uint64_t)v, total - 1) + 1 : 1;  // NaN counts as 0
+}
+
+constexpr int kFew = 512;  // tokens that a wavefront settles
+
+// What the histogram says of a row: its border bins (bin_lo .. bin_hi of top-p, bin_k of top-k) and what is collected.
+struct Edges {
+  bool by_k, by_p, whole_row, fits;
+  int bin_k, bin_lo, bin_hi;
+  uint64_t mass;  // of all tokens
+  double scale;
+  __device__ __forceinline__ bool border_bin(int bin) const { return (by_k && bin == bin_k) || (bin >= bin_lo && bin <= bin_hi); }
+};
+
+// The row's border from `count` collected tokens and, where these are the whole row that matters, its token.
+template <int DT, bool WAVE>
+__device__ __forceinline__ void settle(const SampleArgs& a, Shared& m, RowState& s, int b, const Row& r, const void* row, const Edges& q, int count) {
+  const double scale = q.scale, top = most(a.bits);
+  // This thread's tokens: key, index, whole weight, bin.
+  constexpr int kEach = WAVE ? kFew / 64 : kList / kThreads, kStep = WAVE ? 64 : kThreads;
+  const int me = WAVE ? threadIdx.x & 63 : threadIdx.x;
+  uint32_t keys[kEach], index[kEach];
+  uint64_t weights[kEach];
+  int bins[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = me + e * kStep;
+    bins[e] = -1;
+    if (i >= count) continue;
+    const uint64_t item = a.chunks > 1 ? get_far(&s.list[i]) : m.list[i];
+    keys[e] = (uint32_t)(item >> 32);
+    index[e] = (uint32_t)item;
+    const double y = exponent(r, of_key(keys[e])), w = weight(m.powers, y, a.bits);
+    weights[e] = whole(w);
+    bins[e] = bin_of(y, scale);
+  }
+  // Calls f(key, index, weight, bin) for the collected tokens or, where they are too many for the list, for the border bins'.
+  auto each = [&](auto f) {
+    if (WAVE || q.fits) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (bins[e] >= 0) f(keys[e], index[e], weights[e], bins[e]);
+    } else {
+      for (int i = threadIdx.x; i < a.V; i += kThreads) {
+        const float l = one<DT>(row, i);
+        const double y = exponent(r, l);
+        if (!(y < top)) continue;
+        const int bin = bin_of(y, scale);
+        if (q.border_bin(bin)) f(key_of(l), (uint32_t)i, whole(weight(m.powers, y, a.bits)), bin);
+      }
+    }
+  };
+  // the k-th token's key, and how many of that key are among the k
+  Border at;
+  uint32_t cut = 0;
+  uint64_t ties = ~0ull, equals = 0, kept = q.mass;
+  if (q.by_k) {
+    const uint64_t need = (uint64_t)r.k - m.k_count;
+    border<WAVE>(m, need, [&](auto f) {
+      each([&](uint32_t key, uint32_t, uint64_t, int bin) {
+        if (bin == q.bin_k) f(~key, 1);
+      });
+    }, &at);
+    cut = ~at.at;
+    ties = need - at.before;
+    equals = at.here;
+    if (r.by_p) {  // what the k tokens weigh
+      uint64_t above = 0;
+      each([&](uint32_t key, uint32_t, uint64_t w, int bin) {
+        if (bin == q.bin_k && key > cut) above += w;
+      });
+      scan<WAVE>(above, m.part, &kept);
+      kept += m.k_mass + ties * whole(weight(m.powers, exponent(r, of_key(cut)), a.bits));
+    }
+  }
+  if (r.by_p) {
+    const uint64_t need = share(r.p, kept), lo_mass = m.lo_mass;
+    if (need > lo_mass && border<WAVE>(m, need - lo_mass, [&](auto f) {
+          each([&](uint32_t key, uint32_t, uint64_t w, int bin) {
+            if (bin >= q.bin_lo && bin <= q.bin_hi) f(~key, w);
+          });
+        }, &at)) {
+      const uint32_t key = ~at.at;
+      const uint64_t one_of = max(whole(weight(m.powers, exponent(r, of_key(key)), a.bits)), (uint64_t)1);
+      const uint64_t some = (need - lo_mass - at.before + one_of - 1) / one_of;
+      if (key > cut || (key == cut && some < ties)) {
+        cut = key;
+        ties = some;
+        equals = at.here / one_of;
+      }
+    }
+  }
+  // the last one of the border's equals that is kept, if not all are
+  uint32_t cut_index = 0xffffffffu;
+  if (ties < equals && border<WAVE>(m, ties, [&](auto f) {
+        each([&](uint32_t key, uint32_t i, uint64_t, int) {
+          if (key == cut) f(i, 1);
+        });
+      }, &at))
+    cut_index = at.at;
+  if (!q.whole_row) {
+    if (me == 0) {
+      s.cut_key = cut;
+      s.cut_index = cut_index;
+    }
+    return;
+  }
+  auto keeps = [&](uint32_t key, uint32_t i) {
+    return (key > cut || (key == cut && i <= cut_index)) && weighs(r, m.powers, exponent(r, of_key(key)), a.bits);
+  };
+  uint64_t mine = 0, total = 0;
+  each([&](uint32_t key, uint32_t i, uint64_t w, int) { mine += keeps(key, i) ? w : 0; });
+  scan<WAVE>(mine, m.part, &total);
+  border<WAVE>(m, drawn(a.u[b], total), [&](auto f) {
+    each([&](uint32_t key, uint32_t i, uint64_t w, int) {
+      if (keeps(key, i)) f(i, w);
+    });
+  }, &at);
+  if (me == 0) {
+    give(a, b, r, (int)at.at, one<DT>(row, (int)at.at));
+    s.done = 1;
+  }
 }
 
 }  // namespace
@@ -420,197 +622,117 @@ __global__ void __launch_bounds__(kThreads) sample_borders_kernel(const SampleAr
   Row r;
   row_settings(a, b, r);
   if (r.greedy || !(r.by_k || r.by_p)) return;
+  uint64_t v[2], n[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    v[j] = r.by_p ? s.mass[2 * threadIdx.x + j] : 0;
+    n[j] = s.count[2 * threadIdx.x + j];
+  }
   row_extremes(a, s, r);
   if (r.arg < 0) return;
   const void* row = row_of(a, b, DT);
   const double scale = bin_scale(r, a.bits), top = most(a.bits);
   m.powers.fill();
-
-  // Where the borders are: sums in front of each bin.
-  uint64_t v[2], n[2], mass = 0, tokens = 0;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    v[j] = s.mass[2 * threadIdx.x + j];
-    n[j] = s.count[2 * threadIdx.x + j];
+  if (threadIdx.x == 0) {
+    m.bin_k = kBins;
+    m.k_mass = m.k_full = m.lo_mass = 0;
+    m.listed = 0;
   }
-  const uint64_t v0 = block_scan(v[0] + v[1], m.part, &mass), n0 = block_scan(n[0] + n[1], m.part, &tokens);
-  __syncthreads();
-  __shared__ int bin_k, bin_lo, bin_hi;
-  __shared__ uint64_t k_mass, k_count, lo_mass, listed[2];
-  const bool by_k = r.by_k && (uint64_t)r.k < tokens;
-  auto find = [&](auto reaches) {  // calls reaches(bin, mass in front, tokens in front, mass, tokens) for this thread's bins
+
+  // Where the borders are: sums in front of each thread's two bins.
+  uint64_t mass = 0, tokens = 0;
+  const uint64_t n0 = block_scan(n[0] + n[1], m.part, &tokens);
+  const uint64_t v0 = r.by_p ? block_scan(v[0] + v[1], m.part, &mass) : 0;
+  auto find = [&](auto f) {  // calls f(bin, weight in front, tokens in front, weight, tokens)
     uint64_t vs = v0, ns = n0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      reaches(2 * (int)threadIdx.x + j, vs, ns, v[j], n[j]);
+      f(2 * (int)threadIdx.x + j, vs, ns, v[j], n[j]);
       vs += v[j];
       ns += n[j];
     }
   };
-  if (threadIdx.x == 0) bin_k = kBins;
-  __syncthreads();
+  const bool by_k = r.by_k && (uint64_t)r.k < tokens;
   if (by_k)
     find([&](int bin, uint64_t vs, uint64_t ns, uint64_t vb, uint64_t nb) {
       if (ns < (uint64_t)r.k && (uint64_t)r.k <= ns + nb) {
-        bin_k = bin;
-        k_mass = vs;
-        k_count = ns;
-        listed[0] = vs + vb;
+        m.bin_k = bin;
+        m.k_mass = vs;
+        m.k_full = vs + vb;
+        m.k_count = (uint32_t)ns;
+        m.k_tokens = (uint32_t)nb;
       }
     });
   __syncthreads();
-  const uint64_t least = by_k ? k_mass : mass, full = by_k ? listed[0] : mass;  // the k tokens weigh this much at least, at most
-  if (threadIdx.x == 0) {
-    bin_lo = by_k ? bin_k : kBins - 1;
-    bin_hi = bin_lo;
-    lo_mass = least;
-  }
-  __syncthreads();
+  const int bin_k = m.bin_k;
   if (r.by_p) {
-    const uint64_t t0 = share(r.p, least), t1 = share(r.p, full);
-    __syncthreads();
-    find([&](int bin, uint64_t vs, uint64_t, uint64_t vb, uint64_t) {
-      if (vs < t0 && t0 <= vs + vb && bin <= bin_k) {
-        bin_lo = bin;
-        lo_mass = vs;
+    // the k tokens weigh k_mass at least and k_full at most
+    const uint64_t t0 = share(r.p, by_k ? m.k_mass : mass), t1 = share(r.p, by_k ? m.k_full : mass);
+    find([&](int bin, uint64_t vs, uint64_t ns, uint64_t vb, uint64_t nb) {
+      if (bin > bin_k) return;
+      if (vs < t0 && t0 <= vs + vb) {
+        m.bin_lo = bin;
+        m.lo_mass = vs;
+        m.lo_count = (uint32_t)ns;
       }
-      if (vs < t1 && t1 <= vs + vb && bin <= bin_k) bin_hi = bin;
+      if (vs < t1 && t1 <= vs + vb) {
+        m.bin_hi = bin;
+        m.hi_count = (uint32_t)(ns + nb);
+      }
     });
-    __syncthreads();
   }
-  // All tokens up to the last border, where they are few; else the border bins' own.
-  const int last = by_k ? bin_k : bin_hi;
-  find([&](int bin, uint64_t, uint64_t ns, uint64_t, uint64_t nb) {
-    if (bin == last) listed[1] = ns + nb;
-  });
   __syncthreads();
-  const bool whole_row = listed[1] <= kList;
-  auto border_bin = [&](int bin) { return (by_k && bin == bin_k) || (r.by_p && bin >= bin_lo && bin <= bin_hi); };
-  uint64_t borders = 0, border_tokens = 0;
-  find([&](int bin, uint64_t, uint64_t, uint64_t, uint64_t nb) { borders += border_bin(bin) ? nb : 0; });
-  block_scan(borders, m.part, &border_tokens);
+  // All tokens up to the last border, where they are few; else the border bins' own: from bin_lo to bin_hi, and bin_k.
+  const int bin_lo = r.by_p ? m.bin_lo : kBins, bin_hi = r.by_p ? m.bin_hi : -1;
+  const uint32_t upto = by_k ? m.k_count + m.k_tokens : (r.by_p ? m.hi_count : (uint32_t)tokens);
+  const bool whole_row = upto <= kList;
   if (!whole_row && !by_k && !r.by_p) {  // fewer than k tokens weigh anything
-    if (c == 0 && threadIdx.x == 0) {
-      s.cut_key = 0;
-      s.cut_index = 0;
-    }
+    if (c == 0 && threadIdx.x == 0) s.cut_key = s.cut_index = 0;
     return;
   }
-  const bool fits = whole_row || border_tokens <= kList;
+  const uint32_t edge = (r.by_p ? m.hi_count - m.lo_count : 0) + (by_k && bin_k > bin_hi ? m.k_tokens : 0);
+  const bool fits = whole_row || edge <= kList;
+  const int last = whole_row ? (by_k ? bin_k : (r.by_p ? bin_hi : kBins - 1)) : max(by_k ? bin_k : 0, bin_hi);
+  const Edges q = {by_k, r.by_p, whole_row, fits, bin_k, bin_lo, bin_hi, mass, scale};
   if (fits) {
     const int end = min(a.V, (c + 1) * a.chunk);
-#pragma unroll 2
-    for (int i = c * a.chunk + 4 * threadIdx.x; i < end; i += 4 * kThreads) {
-      float l[4];
-      four<DT>(row, i, end, l);
+    const float least = floor_of(r, (last + 1.0) / scale);
+    for (int i = c * a.chunk + 4 * threadIdx.x; i < end; i += 8 * kThreads) {
+      float l[2][4];
+      four<DT>(row, i, end, l[0]);
+      four<DT>(row, min(i + 4 * kThreads, end), end, l[1]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const double y = exponent(r, l[j]);
-        if (!(y < top)) continue;
-        const int bin = bin_of(y, scale);
-        if (whole_row ? bin <= last : border_bin(bin)) {
-          const uint32_t at = atomicAdd(&s.listed, 1u);  // the histogram has counted them: below kList
-          if (at < kList) s.list[at] = (uint64_t)key_of(l[j]) << 32 | (uint32_t)(i + j);
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (!(l[u][j] >= least)) continue;
+          const double y = exponent(r, l[u][j]);
+          if (!(y < top)) continue;
+          const int bin = bin_of(y, scale);
+          if (whole_row ? bin <= last : q.border_bin(bin)) {
+            const uint32_t at = atomicAdd(&m.listed, 1u);  // the histogram has counted them: below kList
+            if (at < kList) m.list[at] = (uint64_t)key_of(l[u][j]) << 32 | (uint32_t)(i + 4 * kThreads * u + j);
+          }
         }
-      }
     }
   }
-  if (a.chunks > 1) {  // the workgroup that ends last goes on
-    __threadfence();
+  if (a.chunks > 1) {
     __syncthreads();
-    if (threadIdx.x == 0) m.last = atomicAdd(&s.ticket[0], 1u) == (uint32_t)a.chunks - 1;
+    const uint32_t n = min(m.listed, (uint32_t)kList);
+    if (threadIdx.x == 0 && n) m.place = atomicAdd(&s.listed, n);
     __syncthreads();
-    if (!m.last) return;
-    __threadfence();
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads)
+      if (m.place + i < kList) put_far(&s.list[m.place + i], m.list[i]);
+    if (!last_of_row(&s.ticket[0], a.chunks, &m.last)) return;
   } else {
     __syncthreads();
   }
-  const int count = fits ? (int)(whole_row ? listed[1] : border_tokens) : 0;
-  for (int i = threadIdx.x; i < count; i += kThreads) m.list[i] = s.list[i];
-  __syncthreads();
 
-  // Calls f(key, index, weight, bin) for the collected tokens or, where they are too many for the list, for the border bins'.
-  auto each = [&](auto f) {
-    if (fits) {
-      for (int i = threadIdx.x; i < count; i += kThreads) {
-        const uint32_t key = (uint32_t)(m.list[i] >> 32);
-        const double y = exponent(r, of_key(key));
-        f(key, (uint32_t)m.list[i], weight(m.powers, y, a.bits), bin_of(y, scale));
-      }
-    } else {
-      for (int i = threadIdx.x; i < a.V; i += kThreads) {
-        const float l = one<DT>(row, i);
-        const double y = exponent(r, l);
-        if (!(y < top)) continue;
-        const int bin = bin_of(y, scale);
-        if (border_bin(bin)) f(key_of(l), (uint32_t)i, weight(m.powers, y, a.bits), bin);
-      }
-    }
-  };
-  auto mass_of = [&](uint32_t key) { return whole(weight(m.powers, exponent(r, of_key(key)), a.bits)); };
-  // the k-th token's key, and how many of that key are among the k
-  uint32_t cut = 0, at = 0;
-  uint64_t ties = ~0ull, before = 0, kept = mass;
-  if (by_k) {
-    const uint64_t need = (uint64_t)r.k - k_count;
-    border(m, need, [&](auto f) {
-      each([&](uint32_t key, uint32_t, double, int bin) {
-        if (bin == bin_k) f(~key, 1);
-      });
-    }, &at, &before);
-    cut = ~at;
-    ties = need - before;
-    uint64_t above = 0;
-    each([&](uint32_t key, uint32_t, double w, int bin) {
-      if (bin == bin_k && key > cut) above += whole(w);
-    });
-    block_scan(above, m.part, &kept);
-    kept += k_mass + ties * mass_of(cut);
-  }
-  if (r.by_p) {
-    const uint64_t need = share(r.p, kept);
-    if (need > lo_mass && border(m, need - lo_mass, [&](auto f) {
-          each([&](uint32_t key, uint32_t, double w, int bin) {
-            if (bin >= bin_lo && bin <= bin_hi) f(~key, whole(w));
-          });
-        }, &at, &before)) {
-      const uint32_t key = ~at;
-      const uint64_t each_one = max(mass_of(key), (uint64_t)1), some = (need - lo_mass - before + each_one - 1) / each_one;
-      if (key > cut || (key == cut && some < ties)) {
-        cut = key;
-        ties = some;
-      }
-    }
-  }
-  // the last one of the border's equals that is kept, if not all are
-  uint32_t cut_index = 0xffffffffu;
-  if (border(m, ties, [&](auto f) {
-        each([&](uint32_t key, uint32_t i, double, int) {
-          if (key == cut) f(i, 1);
-        });
-      }, &at, &before))
-    cut_index = at;
-  if (!whole_row) {
-    if (threadIdx.x == 0) {
-      s.cut_key = cut;
-      s.cut_index = cut_index;
-    }
-    return;
-  }
-  auto keeps = [&](uint32_t key, uint32_t i, double w) {
-    return (key > cut || (key == cut && i <= cut_index)) && w >= (double)r.minp * (double)(1ull << a.bits);
-  };
-  uint64_t mine = 0, total = 0;
-  each([&](uint32_t key, uint32_t i, double w, int) { mine += keeps(key, i, w) ? whole(w) : 0; });
-  block_scan(mine, m.part, &total);
-  border(m, drawn(a.u[b], total), [&](auto f) {
-    each([&](uint32_t key, uint32_t i, double w, int) {
-      if (keeps(key, i, w)) f(i, whole(w));
-    });
-  }, &at, &before);
-  if (threadIdx.x == 0) {
-    give(a, s, b, r, (int)at, one<DT>(row, (int)at));
-    s.done = 1;
+  const int count = fits ? (int)(whole_row ? upto : edge) : 0;
+  if (fits && count <= kFew) {
+    if (threadIdx.x < 64) settle<DT, true>(a, m, s, b, r, row, q, count);
+  } else {
+    settle<DT, false>(a, m, s, b, r, row, q, count);
   }
 }
 
@@ -630,7 +752,7 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs 
   if (!r.greedy && cuts && s.done) return;
   row_extremes(a, s, r);
   if (r.greedy || r.arg < 0) {  // the first of the largest, or none
-    if (c == 0 && threadIdx.x == 0) give(a, s, b, r, r.arg, r.max);
+    if (c == 0 && threadIdx.x == 0) give(a, b, r, r.arg, r.max);
     return;
   }
   powers.fill();
@@ -658,15 +780,8 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs 
     for (int j = 0; j < 4; ++j) sum += value(l[j], i + j);
   }
   sum = wave_sum64(sum);
-  if (lane == 0) s.wave_mass[c * kWaves + wave] = sum;
-  __threadfence();
-  __syncthreads();
-  if (a.chunks > 1) {
-    if (threadIdx.x == 0) is_last = atomicAdd(&s.ticket[1], 1u) == (uint32_t)a.chunks - 1;
-    __syncthreads();
-    if (!is_last) return;
-    __threadfence();
-  }
+  if (lane == 0) put_far(&s.wave_mass[c * kWaves + wave], sum);
+  if (!last_of_row(&s.ticket[1], a.chunks, &is_last)) return;
   // the stretch in which the sum passes its mark, then the token: a thread takes some neighbours each
   auto pick = [&](uint64_t v, uint64_t base, uint64_t target, int id) {  // the thread whose values reach it
     uint64_t all;
@@ -678,7 +793,7 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs 
     __syncthreads();
   };
   const int pieces = a.chunks * kWaves;  // 1024 at most
-  const uint64_t mine = (int)threadIdx.x < pieces ? s.wave_mass[threadIdx.x] : 0;
+  const uint64_t mine = (int)threadIdx.x < pieces ? get_far(&s.wave_mass[threadIdx.x]) : 0;
   uint64_t total;
   block_scan(mine, part, &total);
   const uint64_t target = drawn(a.u[b], total);
@@ -696,7 +811,7 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs 
       const float l = one<DT>(row, i);
       at += value(l, i);
       if (at >= target) {
-        give(a, s, b, r, i, l);
+        give(a, b, r, i, l);
         break;
       }
     }
