@@ -61,24 +61,28 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) mx_tile_kernel(const Mx
   // buffers.
   const int su = threadIdx.x % SU, st = threadIdx.x / SU;
   const bool mover = su * 16 < a.D * BITS / 8 && st < KT;
-  const uint8_t *kb = a.k + it.head * a.c_head + su * 16, *vb = a.v + it.head * a.c_head + su * 16;
-  const int block = su * 128 / BITS / kMxBlock;
+  const int unit = mover ? su : 0, block = unit * 128 / BITS / kMxBlock;
+  const uint8_t *kb = a.k + it.head * a.c_head + unit * 16, *vb = a.v + it.head * a.c_head + unit * 16;
   const uint8_t *ksb = m_.ks + it.head * m_.s_head + block, *vsb = m_.vs + it.head * m_.s_head + block;
-  uint4 kr[PASS], vr[PASS];
-  uint32_t kse[PASS], vse[PASS];
-  uint64_t ok = 0, ok_next = 0;  // which keys of the tile are there
-  auto load = [&](int tile) __attribute__((always_inline)) {
-    ok_next = __ballot(lane < KT && tab[(tile * KT + lane) % (2 * kTabHalf)] != kNoRow);
-    if (!mover) return;
+  // SETS tiles are on their way: one, or, where a CU has room for one workgroup only, two (heads of 256 columns, 4 prompts of up to 300
+  // tokens over windows of 1024: 87 us, one 90).  Loads stand in no branch, so that a set waits for its own only; a key that is not
+  // there reads the cache's first row, a thread without a unit the row's first one.
+  constexpr int SETS = DP > 128 ? 2 : 1;
+  uint4 kr[SETS][PASS], vr[SETS][PASS];
+  uint32_t kse[SETS][PASS], vse[SETS][PASS];
+  uint64_t ok = 0, ok_next[SETS];  // which keys of the tile are there
+  auto load = [&](int set, int tile) __attribute__((always_inline)) {
+    tile = min(tile, tiles - 1);
+    ok_next[set] = __ballot(lane < KT && tab[(tile * KT + lane) % (2 * kTabHalf)] != kNoRow);
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
-      uint32_t r = tab[(tile * KT + p * TP + st) % (2 * kTabHalf)];
+      uint32_t r = tab[(tile * KT + min(p * TP + st, KT - 1)) % (2 * kTabHalf)];
       r = r == kNoRow ? 0 : r;
       const uint64_t at = (uint64_t)r * 16, sat = BITS == 4 ? r : r >> 1;
-      kr[p] = *reinterpret_cast<const uint4*>(kb + at);
-      vr[p] = *reinterpret_cast<const uint4*>(vb + at);
-      kse[p] = ksb[sat];
-      vse[p] = vsb[sat];
+      kr[set][p] = *reinterpret_cast<const uint4*>(kb + at);
+      vr[set][p] = *reinterpret_cast<const uint4*>(vb + at);
+      kse[set][p] = ksb[sat];
+      vse[set][p] = vsb[sat];
     }
   };
   auto put = [&](uint8_t* to, int t, const uint4& w, uint32_t byte) __attribute__((always_inline)) {
@@ -90,21 +94,21 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) mx_tile_kernel(const Mx
       *reinterpret_cast<uint4*>(to + (t * U + tile_unit<U>(t, E * su + e)) * 16) = v;
     }
   };
-  auto store = [&](uint8_t* to) __attribute__((always_inline)) {
-    if (ok_next != kAll) {
+  auto store = [&](int set, uint8_t* to) __attribute__((always_inline)) {
+    if (ok_next[set] != kAll) {
       asm volatile("");  // a branch, so that whole tiles skip it
 #pragma unroll
       for (int p = 0; p < PASS; ++p)
-        if (!(ok_next >> ((p * TP + st) & 63) & 1)) {
-          kr[p] = vr[p] = make_uint4(0, 0, 0, 0);
-          kse[p] = vse[p] = 1;
+        if (!(ok_next[set] >> ((p * TP + st) & 63) & 1)) {
+          kr[set][p] = vr[set][p] = make_uint4(0, 0, 0, 0);
+          kse[set][p] = vse[set][p] = 1;
         }
     }
     if (!mover) return;
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
-      put(to, p * TP + st, kr[p], kse[p]);
-      put(to + kBuf, p * TP + st, vr[p], vse[p]);
+      put(to, p * TP + st, kr[set][p], kse[set][p]);
+      put(to + kBuf, p * TP + st, vr[set][p], vse[set][p]);
     }
   };
   if (a.D < DP) {
@@ -112,17 +116,19 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) mx_tile_kernel(const Mx
   }
   __syncthreads();
   if (tiles > 0) {
-    load(0);
-    store(lds);
+    load(0, 0);
+    ok = ok_next[0];
+    if (SETS > 1) load(SETS - 1, 1);
+    store(0, lds);
   }
   // The buffer being read and the one being filled are __restrict__ pointers, so that the reads of the one do not wait for
   // the writes into the other.
-  auto step = [&](int i, uint8_t* __restrict__ cur, uint8_t* __restrict__ nxt) __attribute__((always_inline)) {
+  auto step = [&](int i, int set, uint8_t* __restrict__ cur, uint8_t* __restrict__ nxt) __attribute__((always_inline)) {  // set: of tile i
     const int t0 = i * KT;
     __syncthreads();
     if (t0 % kTabHalf == 0) fill(t0 + kTabHalf);  // read from the half's last tile on, behind other barriers
-    ok = ok_next;
-    if (i + 1 < tiles) load(i + 1);
+    if (SETS == 1) ok = ok_next[0];
+    load(set, i + SETS);
     if (live) {
       f32x16 s[TB];
       s16x8 kf[3][TB];  // read two steps ahead of their products, in this order
@@ -221,11 +227,12 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) mx_tile_kernel(const Mx
         }
       }
     }
-    if (i + 1 < tiles) store(nxt);
+    if (SETS > 1) ok = ok_next[SETS - 1 - set];
+    if (i + 1 < tiles) store(SETS - 1 - set, nxt);
   };
   for (int i = 0; i < tiles; i += 2) {  // the buffers' places are constants of the reads' addresses
-    step(i, lds, lds + 2 * kBuf);
-    if (i + 1 < tiles) step(i + 1, lds + 2 * kBuf, lds);
+    step(i, 0, lds, lds + 2 * kBuf);
+    if (i + 1 < tiles) step(i + 1, SETS - 1, lds + 2 * kBuf, lds);
   }
 
   const float sum = l + __shfl_xor(l, 32, kWave);
