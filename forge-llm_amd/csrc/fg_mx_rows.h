@@ -5,7 +5,7 @@
 // numbered as the runs lie.  Values are converted on the way to LDS and come back through the transposing read.
 #pragma once
 
-#include "fg_attn_rows.h"
+#include "fg_attn.h"
 #include "fg_mx_attn.h"
 
 namespace fg {

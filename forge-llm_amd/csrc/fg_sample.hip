@@ -4,7 +4,7 @@
 // reaches p times the k tokens', and of these the ones with w_i >= min_p; the token is the first, by index, at which the kept
 // weights' sum passes u times their total.
 //
-// Weights are computed in fp64 and summed as whole numbers of 2^-bits (a bits of 44 for 2^17 tokens or so): sums do not hang on their
+// Weights are computed in fp64 and summed as whole numbers of 2^-bits (46 for up to 2^16 tokens, so that 2^62 holds all): sums do not hang on their
 // order, so they go through atomics, and a token of less than half a unit is one that nobody draws.
 //
 // Nothing is sorted.  A histogram of the row over (M - l) log2(e) / T, with the weight and the number of the tokens in each

@@ -119,7 +119,8 @@ def mx_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torc
               q_out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotate ``q [T, heads, dim]`` and ``k [T, kv_heads, dim]`` by ``positions``, write ``k``'s and ``v``'s codes and scales to the
     cache's ``slots [T]`` (``page * page_size + token``; one outside the cache, as -1, is padding) and return the rotated ``q`` (in
-    ``q_out``, which may be ``q``, or a new tensor).
+    ``q_out``, which may be ``q``, or a new tensor).  What a slot given to two tokens then holds is undefined: codes of the one may stand
+    beside scales of the other.
 
     ``cos_sin``, the pairs and ``interleaved`` are those of :func:`ops_decoder.rope_append`.  ``positions`` is ``[T]`` or, with
     ``sections``, ``[axes, T]`` (up to four, as time, height and width of an image's tokens): the first ``sections[0]`` pairs turn

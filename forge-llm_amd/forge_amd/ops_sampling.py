@@ -44,8 +44,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: f
     sum up to more than ``uniform`` times their total.  Temperature 0 gives the first of the largest logits.
 
     Logits of -inf (or NaN) are masked: a row of nothing else gives token -1 (logprob -inf).  Weights are fp64 and summed exactly
-    in units of 2^-46 of the largest (2^-44 from 2^17 tokens on, and so on): the same inputs give the same tokens whatever else
-    runs, and a token of less than half a unit is not drawn.  A row with a logit of +inf draws among such (its logprob is NaN).
+    in units of 2^-46 of the largest (past 2^16 tokens twice that, past 2^17 four times, and so on): the same inputs give the same
+    tokens whatever else runs, and a token of less than half a unit is not drawn.  Up to 65535 rows a call.  A row with a logit of +inf draws among such (its logprob is NaN).
     """
     op = "sample_tokens"
     _on_gpu(logits, op)

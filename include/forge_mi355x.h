@@ -363,7 +363,8 @@ typedef struct fg_mx_cache {
 /* Rotary embedding and cache append of T tokens, as fg_rope_append, with positions of several axes: pair i turns by
  * positions[a * ld_positions + token], where axis a has the sections[a] pairs behind those of the axes before it (host
  * memory; sections[0] + .. = rot / 2, each 0 or more; axes from 1 to 4; with one axis sections may be NULL).  Queries
- * are rotated in fp32; keys with one rounding to fp32, from which their codes are made, as the values' are from them. */
+ * are rotated in fp32; keys with one rounding to fp32, from which their codes are made, as the values' are from them.
+ * What a slot given to two tokens then holds is undefined: codes of the one may stand beside scales of the other. */
 int fg_mx_append(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
                  const void* v, int64_t v_token, int64_t v_head, void* q_out, int64_t qo_token, int64_t qo_head, int dtype,
                  const void* positions, int32_t positions_int64, int64_t ld_positions, int32_t axes, const int32_t* sections,
@@ -398,8 +399,8 @@ int fg_mx_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, c
  * one) and of these the ones that weigh min_p times the largest at least.  token[b] is the first, by index, at which
  * the kept weights' sum passes u[b] times their total (u below 0 or NaN counts as 0, from 1 on gives the last).  A temperature
  * of 0 or less (or NaN) gives the first of the largest logits.
- * Logits of -inf and NaN weigh nothing; a row of nothing else gives -1.  Tokens that weigh less than 2^-47 (2^-31 at the
- * least, for more than 2^16 tokens by as many powers of two less) of the largest are not drawn.
+ * Logits of -inf and NaN weigh nothing; a row of nothing else gives -1.  Tokens that weigh less than 2^-47 of the
+ * largest (past 2^16 tokens 2^-46, past 2^17 2^-45, and so on) are not drawn.
  * logprob (may be NULL): float [B], the logarithm of softmax(l) at the token (temperature 1, all tokens); -inf for token -1, NaN
  * in rows with a logit of +inf.
  * temperature, top_k, top_p, min_p: device arrays of B, or NULL for the value that follows for all rows.
