@@ -169,13 +169,47 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* part, uint6
   if (lane == 0) part[wave] = mine;
   __syncthreads();
   uint64_t before = 0, sum = 0;
-#pragma unroll
+#pragma unroll 4
   for (int w = 0; w < kWaves; ++w) {
     before += w < wave ? part[w] : 0;
     sum += part[w];
   }
   *all = sum;
   return before + in_front;
+}
+
+// Both at once: sums of v and of n in front of this thread, and of all.
+__device__ __forceinline__ void block_scan2(uint64_t v, uint32_t n, uint64_t* part_v, uint32_t* part_n, uint64_t* v0, uint64_t* v_all, uint32_t* n0,
+                                            uint32_t* n_all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t vs = v;
+  uint32_t ns = n;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint64_t vo = shfl_up64(vs, d);
+    const uint32_t no = (uint32_t)__shfl_up((int)ns, d, kWave);
+    if (lane >= d) {
+      vs += vo;
+      ns += no;
+    }
+  }
+  __syncthreads();  // the last call's sums have been read
+  if (lane == 63) {
+    part_v[wave] = vs;
+    part_n[wave] = ns;
+  }
+  __syncthreads();
+  *v0 = vs - v;
+  *n0 = ns - n;
+  *v_all = 0;
+  *n_all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    *v0 += w < wave ? part_v[w] : 0;
+    *n0 += w < wave ? part_n[w] : 0;
+    *v_all += part_v[w];
+    *n_all += part_n[w];
+  }
 }
 
 __device__ __forceinline__ void row_settings(const SampleArgs& a, int b, Row& r) {
@@ -230,10 +264,11 @@ __device__ __forceinline__ void row_extremes(const SampleArgs& a, const RowState
     }
     p.min = fminf(p.min, __shfl_xor(p.min, d, kWave));
   }
-  r.max = __shfl(p.max, 0, kWave);
-  r.min = __shfl(p.min, 0, kWave);
-  r.arg = __shfl(p.arg, 0, kWave);
-  r.sum = __shfl(p.sum, 0, kWave);
+  auto first = [](float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); };
+  r.max = first(p.max);
+  r.min = first(p.min);
+  r.arg = __builtin_amdgcn_readfirstlane(p.arg);
+  r.sum = first(p.sum);
 }
 
 // Token i of logit l for row b.
@@ -375,7 +410,9 @@ struct Shared {
   uint64_t part[kWaves];
   Powers powers;
   uint64_t found[3];
-  uint32_t lo[kWaves], hi[kWaves];
+  uint32_t lo[kWaves], hi[kWaves], tokens[kWaves];
+  uint64_t kept, total;
+  uint32_t edges, cut_key, cut_index;
   int last;
   // the borders' bins, the tokens and the weight in front of them and in them
   int bin_k, bin_lo, bin_hi;
@@ -384,51 +421,35 @@ struct Shared {
   uint32_t listed, place;
 };
 
-// Where a row is settled: by a workgroup, or by one wavefront, which needs no barrier, where its tokens are few.
-template <bool WAVE>
-__device__ __forceinline__ void together() {
-  if constexpr (WAVE) {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  } else {
-    __syncthreads();
-  }
-}
-template <bool WAVE>
-__device__ __forceinline__ uint64_t scan(uint64_t v, uint64_t* part, uint64_t* all) {
-  if constexpr (WAVE) return wave_scan(v, all);
-  else return block_scan(v, part, all);
-}
-
 // The smallest coordinate at which the sum of the values of the elements up to there reaches `target`; the sum in front of it, and what
-// it has itself: by histograms, each over a bin of the one before (2048 bins of a workgroup, 64 of a wavefront).  each(f) calls
-// f(coordinate, value) for the elements; false: the sum of all of them does not reach it.
+// it has itself: by histograms, each over a bin of the one before.  each(f) calls f(coordinate, value) for the elements, whose
+// coordinates are lo .. hi, or where lo > hi looked for first; false: the sum of all of them does not reach it.
 struct Border {
   uint32_t at;
   uint64_t before, here;
 };
-template <bool WAVE, class Each>
-__device__ __forceinline__ bool border(Shared& m, uint64_t target, const Each& each, Border* found) {
-  constexpr int kPer = WAVE ? 1 : kBins / kThreads, kLog = WAVE ? 6 : 11;  // bins of a thread, of all
-  const int me = WAVE ? threadIdx.x & 63 : threadIdx.x;
-  uint32_t lo = 0xffffffffu, hi = 0;
-  each([&](uint32_t c, uint64_t) {
-    lo = min(lo, c);
-    hi = max(hi, c);
-  });
+template <class Each>
+__device__ __forceinline__ bool border(Shared& m, uint64_t target, uint32_t lo, uint32_t hi, const Each& each, Border* found) {
+  constexpr int kPer = kBins / kThreads, kLog = 11;  // bins of a thread, of all
+  static_assert(kBins == 1 << kLog, "");
+  const int me = threadIdx.x;
+  __syncthreads();  // what an earlier call left in m has been read
+  if (lo > hi) {
+    each([&](uint32_t c, uint64_t) {
+      lo = min(lo, c);
+      hi = max(hi, c);
+    });
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    lo = min(lo, (uint32_t)__shfl_xor((int)lo, d, kWave));
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, d, kWave));
-  }
-  if constexpr (!WAVE) {
-    __syncthreads();  // what an earlier call left in m has been read
+    for (int d = 1; d < 64; d *= 2) {
+      lo = min(lo, (uint32_t)__shfl_xor((int)lo, d, kWave));
+      hi = max(hi, (uint32_t)__shfl_xor((int)hi, d, kWave));
+    }
     if ((threadIdx.x & 63) == 0) {
       m.lo[threadIdx.x >> 6] = lo;
       m.hi[threadIdx.x >> 6] = hi;
     }
     __syncthreads();
-#pragma unroll
+#pragma unroll 4  // a sixteenth at once takes the registers of the second workgroup on a CU
     for (int w = 0; w < kWaves; ++w) {
       lo = min(lo, m.lo[w]);
       hi = max(hi, m.hi[w]);
@@ -441,18 +462,18 @@ __device__ __forceinline__ bool border(Shared& m, uint64_t target, const Each& e
 #pragma unroll
     for (int j = 0; j < kPer; ++j) m.mass[me * kPer + j] = 0;
     if (me == 0) m.found[0] = ~0ull;
-    together<WAVE>();
+    __syncthreads();
     each([&](uint32_t c, uint64_t v) {
       if (c >= lo && c <= hi) atomicAdd(reinterpret_cast<unsigned long long*>(&m.mass[(c - lo) >> shift]), (unsigned long long)v);
     });
-    together<WAVE>();
+    __syncthreads();
     uint64_t v[kPer], sum = 0, all;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       v[j] = m.mass[me * kPer + j];
       sum += v[j];
     }
-    sum = base + scan<WAVE>(sum, m.part, &all);
+    sum = base + block_scan(sum, m.part, &all);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       if (sum < target && target <= sum + v[j]) {
@@ -462,7 +483,7 @@ __device__ __forceinline__ bool border(Shared& m, uint64_t target, const Each& e
       }
       sum += v[j];
     }
-    together<WAVE>();
+    __syncthreads();
     const uint64_t bin = m.found[0], here = m.found[2];
     if (bin == ~0ull) return false;
     base = m.found[1];
@@ -472,7 +493,7 @@ __device__ __forceinline__ bool border(Shared& m, uint64_t target, const Each& e
       return true;
     }
     hi = (uint32_t)min((uint64_t)hi, (uint64_t)lo + ((1u << shift) - 1));
-    together<WAVE>();
+    __syncthreads();
   }
 }
 
@@ -491,7 +512,7 @@ __device__ __forceinline__ uint64_t drawn(float u, uint64_t total) {
   return v > 0 ? min((uint64_t)v, total - 1) + 1 : 1;  // NaN counts as 0
 }
 
-constexpr int kFew = 512;  // tokens that a wavefront settles
+constexpr int kFew = 256;  // tokens that are settled by comparing each with all
 
 // What the histogram says of a row: its border bins (bin_lo .. bin_hi of top-p, bin_k of top-k) and what is collected.
 struct Edges {
@@ -502,51 +523,18 @@ struct Edges {
   __device__ __forceinline__ bool border_bin(int bin) const { return (by_k && bin == bin_k) || (bin >= bin_lo && bin <= bin_hi); }
 };
 
-// The row's border from `count` collected tokens and, where these are the whole row that matters, its token.
-template <int DT, bool WAVE>
-__device__ __forceinline__ void settle(const SampleArgs& a, Shared& m, RowState& s, int b, const Row& r, const void* row, const Edges& q, int count) {
-  const double scale = q.scale, top = most(a.bits);
-  // This thread's tokens: key, index, whole weight, bin.
-  constexpr int kEach = WAVE ? kFew / 64 : kList / kThreads, kStep = WAVE ? 64 : kThreads;
-  const int me = WAVE ? threadIdx.x & 63 : threadIdx.x;
-  uint32_t keys[kEach], index[kEach];
-  uint64_t weights[kEach];
-  int bins[kEach];
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = me + e * kStep;
-    bins[e] = -1;
-    if (i >= count) continue;
-    const uint64_t item = a.chunks > 1 ? get_far(&s.list[i]) : m.list[i];
-    keys[e] = (uint32_t)(item >> 32);
-    index[e] = (uint32_t)item;
-    const double y = exponent(r, of_key(keys[e])), w = weight(m.powers, y, a.bits);
-    weights[e] = whole(w);
-    bins[e] = bin_of(y, scale);
-  }
-  // Calls f(key, index, weight, bin) for the collected tokens or, where they are too many for the list, for the border bins'.
-  auto each = [&](auto f) {
-    if (WAVE || q.fits) {
-#pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        if (bins[e] >= 0) f(keys[e], index[e], weights[e], bins[e]);
-    } else {
-      for (int i = threadIdx.x; i < a.V; i += kThreads) {
-        const float l = one<DT>(row, i);
-        const double y = exponent(r, l);
-        if (!(y < top)) continue;
-        const int bin = bin_of(y, scale);
-        if (q.border_bin(bin)) f(key_of(l), (uint32_t)i, whole(weight(m.powers, y, a.bits)), bin);
-      }
-    }
-  };
+// Where the kept tokens end, from the tokens of the border bins: m.cut_key, m.cut_index.  each(f) calls f(key, index, weight, bin) for
+// them (and maybe others).
+template <class Each>
+__device__ __forceinline__ void cut_by_bins(const SampleArgs& a, Shared& m, const Row& r, const Edges& q, const Each& each) {
+  constexpr uint32_t kAny = 0xffffffffu;
   // the k-th token's key, and how many of that key are among the k
   Border at;
   uint32_t cut = 0;
   uint64_t ties = ~0ull, equals = 0, kept = q.mass;
   if (q.by_k) {
     const uint64_t need = (uint64_t)r.k - m.k_count;
-    border<WAVE>(m, need, [&](auto f) {
+    border(m, need, kAny, 0, [&](auto f) {
       each([&](uint32_t key, uint32_t, uint64_t, int bin) {
         if (bin == q.bin_k) f(~key, 1);
       });
@@ -559,13 +547,13 @@ __device__ __forceinline__ void settle(const SampleArgs& a, Shared& m, RowState&
       each([&](uint32_t key, uint32_t, uint64_t w, int bin) {
         if (bin == q.bin_k && key > cut) above += w;
       });
-      scan<WAVE>(above, m.part, &kept);
+      block_scan(above, m.part, &kept);
       kept += m.k_mass + ties * whole(weight(m.powers, exponent(r, of_key(cut)), a.bits));
     }
   }
   if (r.by_p) {
     const uint64_t need = share(r.p, kept), lo_mass = m.lo_mass;
-    if (need > lo_mass && border<WAVE>(m, need - lo_mass, [&](auto f) {
+    if (need > lo_mass && border(m, need - lo_mass, kAny, 0, [&](auto f) {
           each([&](uint32_t key, uint32_t, uint64_t w, int bin) {
             if (bin >= q.bin_lo && bin <= q.bin_hi) f(~key, w);
           });
@@ -581,13 +569,107 @@ __device__ __forceinline__ void settle(const SampleArgs& a, Shared& m, RowState&
     }
   }
   // the last one of the border's equals that is kept, if not all are
-  uint32_t cut_index = 0xffffffffu;
-  if (ties < equals && border<WAVE>(m, ties, [&](auto f) {
+  uint32_t cut_index = kAny;
+  if (ties < equals && border(m, ties, 0, (uint32_t)a.V - 1, [&](auto f) {
         each([&](uint32_t key, uint32_t i, uint64_t, int) {
           if (key == cut) f(i, 1);
         });
       }, &at))
     cut_index = at.at;
+  if (threadIdx.x == 0) {
+    m.cut_key = cut;
+    m.cut_index = cut_index;
+  }
+}
+
+// The same for few tokens: four threads each, which go over a quarter of all of them for what stands in front of their own.  m.mass
+// holds a pair for each token, its place in the order (the key, then the index backwards) and its weight.
+__device__ __forceinline__ void cut_by_places(const SampleArgs& a, Shared& m, const Row& r, const Edges& q, int listed) {
+  ulonglong2* const pairs = reinterpret_cast<ulonglong2*>(m.mass);
+  static_assert(kFew * sizeof(ulonglong2) <= sizeof(m.mass) && kFew * 4 == kThreads, "");
+  for (int i = threadIdx.x; i < listed; i += kThreads) {
+    const uint64_t item = m.list[i];
+    const uint32_t key = (uint32_t)(item >> 32);
+    const double y = exponent(r, of_key(key));
+    if (!q.border_bin(bin_of(y, q.scale))) continue;
+    const uint32_t at = atomicAdd(&m.edges, 1u);
+    if (at < kFew) pairs[at] = make_ulonglong2((uint64_t)key << 32 | (uint32_t)~(uint32_t)item, whole(weight(m.powers, y, a.bits)));
+  }
+  __syncthreads();
+  const int count = min((int)m.edges, kFew), i = threadIdx.x / 4, quarter = threadIdx.x % 4;
+  const bool is = i < count;
+  uint64_t place = 0, w = 0, w_front = 0;
+  uint32_t n_front = 0;
+  if (is) {
+    place = pairs[i].x;
+    w = pairs[i].y;
+#pragma unroll 4
+    for (int j = quarter; j < count; j += 4) {
+      const ulonglong2 p = pairs[j];
+      const bool front = p.x > place;
+      n_front += front;
+      w_front += front ? p.y : 0;
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 4; d *= 2) {
+    n_front += (uint32_t)__shfl_xor((int)n_front, d, kWave);
+    w_front += shfl_xor64(w_front, d);
+  }
+  // The bins of top-p (tokens that weigh up to its mark lie in these alone), then bin_k.
+  bool keep = is;
+  uint64_t mass = q.mass;
+  if (q.by_k) {
+    const uint32_t in_front = !q.by_p ? 0 : (q.bin_k > q.bin_hi ? m.hi_count : m.k_count) - m.lo_count;
+    const bool in_k = is && n_front >= in_front;
+    keep = is && (!in_k || n_front + (m.k_count - in_front) < (uint32_t)r.k);
+    if (q.by_p) {  // what the k tokens weigh
+      if (keep && in_k && quarter == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&m.kept), (unsigned long long)w);
+      __syncthreads();
+      mass = m.k_mass + m.kept;
+    }
+  }
+  if (q.by_p) keep = keep && w_front + m.lo_mass < share(r.p, mass);
+  const int kept = __syncthreads_count(keep && quarter == 0);
+  if (keep && quarter == 0 && (int)n_front == kept - 1) {  // the last one
+    m.cut_key = (uint32_t)(place >> 32);
+    m.cut_index = ~(uint32_t)place;
+  }
+}
+
+// The row's border from its collected tokens and, where these are the whole row that matters, its token.
+template <int DT>
+__device__ __forceinline__ void settle(const SampleArgs& a, Shared& m, RowState& s, int b, const Row& r, const void* row, const Edges& q, int count,
+                                       int edge) {
+  const double scale = q.scale, top = most(a.bits);
+  const int me = threadIdx.x, all = q.fits ? count : a.V;
+  if (q.fits && a.chunks > 1)
+    for (int i = me; i < count; i += kThreads) m.list[i] = get_far(&s.list[i]);
+  if (me == 0) {
+    m.kept = m.total = 0;
+    m.edges = m.cut_key = 0;
+    m.cut_index = 0xffffffffu;
+  }
+  __syncthreads();
+  // Calls f(key, index, weight, bin) for the collected tokens or, where they are too many for the list, for the border bins'.  (Nothing
+  // of them stays in registers: the kernel's 64 let a CU hold two workgroups.)
+  auto each = [&](auto f) {
+#pragma unroll 1
+    for (int i = me; i < all; i += kThreads) {
+      const uint64_t item = q.fits ? m.list[i] : (uint64_t)key_of(one<DT>(row, i)) << 32 | (uint32_t)i;
+      const uint32_t key = (uint32_t)(item >> 32);
+      const double y = exponent(r, of_key(key));
+      if (!(y < top)) continue;
+      const int bin = bin_of(y, scale);
+      if (q.fits || q.border_bin(bin)) f(key, (uint32_t)item, whole(weight(m.powers, y, a.bits)), bin);
+    }
+  };
+  if (q.by_k || q.by_p) {
+    if (q.fits && edge <= kFew) cut_by_places(a, m, r, q, count);
+    else cut_by_bins(a, m, r, q, each);
+    __syncthreads();
+  }
+  const uint32_t cut = m.cut_key, cut_index = m.cut_index;
   if (!q.whole_row) {
     if (me == 0) {
       s.cut_key = cut;
@@ -598,16 +680,49 @@ __device__ __forceinline__ void settle(const SampleArgs& a, Shared& m, RowState&
   auto keeps = [&](uint32_t key, uint32_t i) {
     return (key > cut || (key == cut && i <= cut_index)) && weighs(r, m.powers, exponent(r, of_key(key)), a.bits);
   };
-  uint64_t mine = 0, total = 0;
-  each([&](uint32_t key, uint32_t i, uint64_t w, int) { mine += keeps(key, i) ? w : 0; });
-  scan<WAVE>(mine, m.part, &total);
-  border<WAVE>(m, drawn(a.u[b], total), [&](auto f) {
-    each([&](uint32_t key, uint32_t i, uint64_t w, int) {
-      if (keeps(key, i)) f(i, w);
-    });
-  }, &at);
-  if (me == 0) {
-    give(a, b, r, (int)at.at, one<DT>(row, (int)at.at));
+  int token = -1;  // of the one thread that has it
+  if (count <= kFew) {
+    // four threads a token, for the sum of what is kept in front of it
+    ulonglong2* const pairs = reinterpret_cast<ulonglong2*>(m.mass);  // index, weight
+    const int i = me / 4, quarter = me % 4;
+    uint32_t index = 0;
+    uint64_t w = 0, before = 0;
+    if (i < count) {
+      const uint64_t item = m.list[i];
+      const uint32_t key = (uint32_t)(item >> 32);
+      index = (uint32_t)item;
+      if (keeps(key, index)) w = whole(weight(m.powers, exponent(r, of_key(key)), a.bits));
+    }
+    if (quarter == 0) {
+      pairs[i] = make_ulonglong2(index, w);
+      if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&m.total), (unsigned long long)w);
+    }
+    __syncthreads();
+    if (w) {
+#pragma unroll 4
+      for (int j = quarter; j < count; j += 4) {
+        const ulonglong2 p = pairs[j];
+        before += p.x < index ? p.y : 0;
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d *= 2) before += shfl_xor64(before, d);
+    const uint64_t target = drawn(a.u[b], m.total);
+    if (quarter == 0 && before < target && target <= before + w) token = (int)index;
+  } else {
+    uint64_t mine = 0, total = 0;
+    each([&](uint32_t key, uint32_t i, uint64_t w, int) { mine += keeps(key, i) ? w : 0; });
+    block_scan(mine, m.part, &total);
+    Border at;
+    border(m, drawn(a.u[b], total), 0, (uint32_t)a.V - 1, [&](auto f) {
+      each([&](uint32_t key, uint32_t i, uint64_t w, int) {
+        if (keeps(key, i)) f(i, w);
+      });
+    }, &at);
+    if (me == 0) token = (int)at.at;
+  }
+  if (token >= 0) {
+    give(a, b, r, token, one<DT>(row, token));
     s.done = 1;
   }
 }
@@ -615,14 +730,15 @@ __device__ __forceinline__ void settle(const SampleArgs& a, Shared& m, RowState&
 }  // namespace
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) sample_borders_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) sample_borders_kernel(const SampleArgs a) {
   __shared__ Shared m;
   const int b = blockIdx.x / a.chunks, c = blockIdx.x - b * a.chunks;
   RowState& s = reinterpret_cast<RowState*>(a.ws)[b];
   Row r;
   row_settings(a, b, r);
   if (r.greedy || !(r.by_k || r.by_p)) return;
-  uint64_t v[2], n[2];
+  uint64_t v[2];
+  uint32_t n[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     v[j] = r.by_p ? s.mass[2 * threadIdx.x + j] : 0;
@@ -640,11 +756,12 @@ __global__ void __launch_bounds__(kThreads) sample_borders_kernel(const SampleAr
   }
 
   // Where the borders are: sums in front of each thread's two bins.
-  uint64_t mass = 0, tokens = 0;
-  const uint64_t n0 = block_scan(n[0] + n[1], m.part, &tokens);
-  const uint64_t v0 = r.by_p ? block_scan(v[0] + v[1], m.part, &mass) : 0;
+  uint64_t mass, v0;
+  uint32_t tokens, n0;
+  block_scan2(v[0] + v[1], n[0] + n[1], m.part, m.tokens, &v0, &mass, &n0, &tokens);
   auto find = [&](auto f) {  // calls f(bin, weight in front, tokens in front, weight, tokens)
-    uint64_t vs = v0, ns = n0;
+    uint64_t vs = v0;
+    uint32_t ns = n0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       f(2 * (int)threadIdx.x + j, vs, ns, v[j], n[j]);
@@ -652,15 +769,15 @@ __global__ void __launch_bounds__(kThreads) sample_borders_kernel(const SampleAr
       ns += n[j];
     }
   };
-  const bool by_k = r.by_k && (uint64_t)r.k < tokens;
+  const bool by_k = r.by_k && (uint32_t)r.k < tokens;
   if (by_k)
-    find([&](int bin, uint64_t vs, uint64_t ns, uint64_t vb, uint64_t nb) {
-      if (ns < (uint64_t)r.k && (uint64_t)r.k <= ns + nb) {
+    find([&](int bin, uint64_t vs, uint32_t ns, uint64_t vb, uint32_t nb) {
+      if (ns < (uint32_t)r.k && (uint32_t)r.k <= ns + nb) {
         m.bin_k = bin;
         m.k_mass = vs;
         m.k_full = vs + vb;
-        m.k_count = (uint32_t)ns;
-        m.k_tokens = (uint32_t)nb;
+        m.k_count = ns;
+        m.k_tokens = nb;
       }
     });
   __syncthreads();
@@ -668,23 +785,23 @@ __global__ void __launch_bounds__(kThreads) sample_borders_kernel(const SampleAr
   if (r.by_p) {
     // the k tokens weigh k_mass at least and k_full at most
     const uint64_t t0 = share(r.p, by_k ? m.k_mass : mass), t1 = share(r.p, by_k ? m.k_full : mass);
-    find([&](int bin, uint64_t vs, uint64_t ns, uint64_t vb, uint64_t nb) {
+    find([&](int bin, uint64_t vs, uint32_t ns, uint64_t vb, uint32_t nb) {
       if (bin > bin_k) return;
       if (vs < t0 && t0 <= vs + vb) {
         m.bin_lo = bin;
         m.lo_mass = vs;
-        m.lo_count = (uint32_t)ns;
+        m.lo_count = ns;
       }
       if (vs < t1 && t1 <= vs + vb) {
         m.bin_hi = bin;
-        m.hi_count = (uint32_t)(ns + nb);
+        m.hi_count = ns + nb;
       }
     });
   }
   __syncthreads();
   // All tokens up to the last border, where they are few; else the border bins' own: from bin_lo to bin_hi, and bin_k.
   const int bin_lo = r.by_p ? m.bin_lo : kBins, bin_hi = r.by_p ? m.bin_hi : -1;
-  const uint32_t upto = by_k ? m.k_count + m.k_tokens : (r.by_p ? m.hi_count : (uint32_t)tokens);
+  const uint32_t upto = by_k ? m.k_count + m.k_tokens : (r.by_p ? m.hi_count : tokens);
   const bool whole_row = upto <= kList;
   if (!whole_row && !by_k && !r.by_p) {  // fewer than k tokens weigh anything
     if (c == 0 && threadIdx.x == 0) s.cut_key = s.cut_index = 0;
@@ -729,11 +846,7 @@ __global__ void __launch_bounds__(kThreads) sample_borders_kernel(const SampleAr
   }
 
   const int count = fits ? (int)(whole_row ? upto : edge) : 0;
-  if (fits && count <= kFew) {
-    if (threadIdx.x < 64) settle<DT, true>(a, m, s, b, r, row, q, count);
-  } else {
-    settle<DT, false>(a, m, s, b, r, row, q, count);
-  }
+  settle<DT>(a, m, s, b, r, row, q, count, (int)edge);
 }
 
 // ------------------------------------------------------------------------------------------------ sums in the order of the indexes
