@@ -49,13 +49,32 @@ size_t mx_attn_plan(MxAttnArgs& m) {
   const int64_t span = std::min<int64_t>(a.max_len, (int64_t)m.window + tokens + 30);
   a.tiles_s = (int)((rows + tile - 1) / tile);
   const int64_t sets = (int64_t)a.Hk * a.B, items = std::max<int64_t>(sets * a.tiles_s, 1), unit = m.tile ? 64 : kRowsTile * kRowsWaves;
-  // About two workgroups per CU: us by keys per part, 32 + 2 x 8 heads of 128 in 4 bits, 1 sequence of 5000 128 / 256 / 512: 11.6 / 10.9 /
-  // 12.0, 4 of 16000 512 / 1024: 20.0 / 19.6, 16 of 4000 with 4 queries each 512 / 1024: 21.2 / 20.5.  Where the sequences fill the
-  // CUs by themselves one part does, but for long ones, which would outlast the others: parts of 2048 keys (64 of 2048 to 16384, 64 +
-  // 2 x 8 heads, 16384 / 4096 / 2048: 170 / 148 / 150; 64 of up to 8000 x 64 columns 8000 / 4096 / 2048: 58 / 66 / 56; 64 of up to
-  // 4000 x 256 columns 4000 / 2048: 108 / 129).
-  int64_t parts = std::max<int64_t>(1, 2 * cus / items);
-  if (!m.tile && span > 8192) parts = std::max<int64_t>(parts, (span + 2047) / 2048);
+  int64_t parts = 1;
+  if (m.tile) {
+    // The cheapest number by rounds of the CUs times keys of a part, and 96 keys' worth for each part's begin, end and share of the join.
+    // Row tiles are those that the number of query tokens suggests, as prompts of a batch have other lengths than the longest.  us with 1 /
+    // 2 / 3 / 4 parts: 16 + 2 x 8 heads of 256, one workgroup on a CU, windows of 1024, prompts of 75 to 300 (2) 84 / 63 / 79 / 76, of 300
+    // (3) 86 / 109 / 88 / 108, 512 queries on 4096 keys (4) 251 / 145 / 108 / 87; 32 + 2 x 8 heads of 128, two on a CU, 300 queries
+    // each on 4 x 4000 (3) 156 / 148 / 135 / 137; of 64, 200 on 8 x 2000 (1) 51 / 80 / 79 / 79.
+    const int64_t slots = (a.D > 128 ? 1 : 2) * cus;
+    const int64_t real = std::max<int64_t>(1, std::min(items, a.Hk * ((int64_t)a.T * a.G / tile + (a.B + 1) / 2)));
+    int64_t best = INT64_MAX;
+    for (int p = 1; p <= 16; ++p) {
+      const int64_t cost = (real * p + slots - 1) / slots * ((span + p - 1) / p) + 96 * p;
+      if (cost < best) {
+        best = cost;
+        parts = p;
+      }
+    }
+  } else {
+    // About two workgroups per CU: us by keys per part, 32 + 2 x 8 heads of 128 in 4 bits, 1 sequence of 5000 128 / 256 / 512: 11.6 /
+    // 10.9 / 12.0, 4 of 16000 512 / 1024: 20.0 / 19.6, 16 of 4000 with 4 queries each 512 / 1024: 21.2 / 20.5.  Where the sequences fill
+    // the CUs by themselves one part does, but for long ones, which would outlast the others: parts of 2048 keys (64 of 2048 to 16384,
+    // 64 + 2 x 8 heads, 16384 / 4096 / 2048: 170 / 148 / 150; 64 of up to 8000 x 64 columns 8000 / 4096 / 2048: 58 / 66 / 56; 64 of up
+    // to 4000 x 256 columns 4000 / 2048: 108 / 129).
+    parts = std::max<int64_t>(1, 2 * cus / items);
+    if (span > 8192) parts = std::max<int64_t>(parts, (span + 2047) / 2048);
+  }
   const int64_t part = std::max<int64_t>(m.tile ? 64 : 256, ((span + parts - 1) / parts + unit - 1) / unit * unit);
   a.part_s = (int)part;
   a.parts_s = (int)std::max<int64_t>(1, (span + part - 1) / part);

@@ -10,8 +10,8 @@
 // Nothing is sorted.  A histogram of the row over (M - l) log2(e) / T, with the weight and the number of the tokens in each
 // bin, says in which bin the k-th token and the nucleus's last one lie.  Where all bins up to there hold few tokens (kList), these are
 // collected and settle the row by themselves; else the border bins' tokens settle the border, and one more pass over the row sums
-// up the weights in front of it, in the order of the indexes.  The border within a list is found by histograms again, each over a
-// 2048th of the one before.
+// up the weights in front of it, in the order of the indexes.  The border within a list is found by comparing each of a few
+// tokens (kFew) with all of them, else by histograms again, each over a 2048th of the one before.
 //
 // One launch for each pass (extremes, histogram, collection, sums); a row is cut into chunks of a workgroup each while rows are few,
 // and what follows a pass is done by the workgroup that ends last.  Bound by HBM for the first pass, for the others by
@@ -225,7 +225,7 @@ __device__ __forceinline__ void row_settings(const SampleArgs& a, int b, Row& r)
 }
 
 // What a row's workgroups hand to the one that ends last goes past the XCDs' L2 caches both ways (a fence would write each whole
-// cache back, once for every workgroup: 32 rows of 128000 357 us, now 87), and is in memory when the wavefront's wait is over.
+// cache back, once for every workgroup: 32 rows of 128000 357 us against 87), and is in memory when the wavefront's wait is over.
 template <class T>
 __device__ __forceinline__ void put_far(T* p, T v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
