@@ -65,8 +65,8 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) mx_tile_kernel(const Mx
   const uint8_t *kb = a.k + it.head * a.c_head + unit * 16, *vb = a.v + it.head * a.c_head + unit * 16;
   const uint8_t *ksb = m_.ks + it.head * m_.s_head + block, *vsb = m_.vs + it.head * m_.s_head + block;
   // SETS tiles are on their way: one, or, where a CU has room for one workgroup only, two (heads of 256 columns, 4 prompts of up to 300
-  // tokens over windows of 1024 in three parts: 87 us, one 90).  Loads stand in no branch, so that a set waits for its own only; a key that is not
-  // there reads the cache's first row, a thread without a unit the row's first one.
+  // tokens over windows of 1024 in three parts: 87 us, one 90).  Loads stand in no branch, so that a set waits for its own only; a key
+  // that is not there reads the cache's first row, a thread without a unit the row's first one.
   constexpr int SETS = DP > 128 ? 2 : 1;
   uint4 kr[SETS][PASS], vr[SETS][PASS];
   uint32_t kse[SETS][PASS], vse[SETS][PASS];

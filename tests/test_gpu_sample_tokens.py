@@ -226,3 +226,15 @@ def test_no_rows_and_refusals():
         sample_tokens(x.cpu(), u.cpu())
     with pytest.raises(_lib.KernelLaunchError, match="sizes"):
         sample_tokens(x[:1].expand(1 << 16, 100), torch.zeros(1 << 16, device=DEV))
+
+
+@pytest.mark.parametrize("dt", [FP, BF])
+@pytest.mark.parametrize("spread", [0.01, 0.7, 2.5, 9.0])
+def test_borders_of_both_kinds_near_and_far(spread, dt):
+    """Top-k's border in front of top-p's, behind it and in the same bin, in rows of few and of many tokens up to there."""
+    k = torch.tensor([1, 2, 40, 255, 256, 257, 300, 1000, 4095, 4097, 5000, 12000, 20010, 0], dtype=torch.int32)
+    for p in (1e-6, 0.2, 0.7, 0.95, 0.9999):
+        logits, uniform = _logits(len(k), 20011, dt, seed=int(1000 * p), spread=spread)
+        _check(logits, uniform, top_k=k, top_p=p)
+    _check(logits, uniform, top_k=k, min_p=0.02)
+    _check(logits[:2], uniform[:2], top_k=5000, top_p=0.8, temperature=0.5)  # a row in more chunks
