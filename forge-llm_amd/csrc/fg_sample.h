@@ -19,6 +19,7 @@ struct SampleArgs {
   float* logprob;  // or null
   int bits;           // a weight of one is 2^bits
   int chunks, chunk;  // workgroups per row, and their columns
+  int sum_chunks, sum_chunk;  // of the sums
   bool cuts;          // some row may have top-k or top-p
   uint8_t* ws;
 };

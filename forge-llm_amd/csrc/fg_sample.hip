@@ -16,7 +16,7 @@
 // One launch for each pass (extremes, histogram, collection, sums); a row is cut into chunks of a workgroup each while rows are few,
 // and what follows a pass is done by the workgroup that ends last.  Bound by HBM for the first pass, for the others by
 // the L2 and Infinity caches and the arithmetic of the weights; for one row by the launches (256 rows of 150001 in fp32, mixed settings
-// 197 us: 32 + 50 + 51 + 64; one row of 32000 in bf16, top-k 50 and top-p 0.9 25 us).
+// 169 us: 32 + 47 + 50 + 41; one row of 32000 in bf16, top-k 50 and top-p 0.9 25 us).
 #include <algorithm>
 
 #include "fg_sample.h"
@@ -71,27 +71,47 @@ __device__ __forceinline__ float one(const void* row, int i) {
 typedef uint32_t u32x4_by4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_by2 __attribute__((ext_vector_type(2), aligned(2)));
 
-// Four neighbouring logits, as many as there are up to `end`; the others are -inf.
+// Four neighbouring logits.
 template <int DT>
-__device__ __forceinline__ void four(const void* row, int i, int end, float (&l)[4]) {
-  if (i + 4 <= end) {
-    if constexpr (DT == FG_F32) {
-      const u32x4_by4 w = *reinterpret_cast<const u32x4_by4*>(static_cast<const float*>(row) + i);
+__device__ __forceinline__ void four(const void* row, int i, float (&l)[4]) {
+  if constexpr (DT == FG_F32) {
+    const u32x4_by4 w = *reinterpret_cast<const u32x4_by4*>(static_cast<const float*>(row) + i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) l[j] = __uint_as_float(w[j]);
-    } else {
-      const u32x2_by2 w = *reinterpret_cast<const u32x2_by2*>(static_cast<const uint16_t*>(row) + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint16_t b = (uint16_t)(w[j / 2] >> (16 * (j % 2)));
-        l[j] = DT == FG_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) l[j] = __builtin_isnan(l[j]) ? -__builtin_inff() : l[j];
+    for (int j = 0; j < 4; ++j) l[j] = __uint_as_float(w[j]);
   } else {
+    const u32x2_by2 w = *reinterpret_cast<const u32x2_by2*>(static_cast<const uint16_t*>(row) + i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) l[j] = i + j < end ? one<DT>(row, i + j) : -__builtin_inff();
+    for (int j = 0; j < 4; ++j) {
+      const uint16_t b = (uint16_t)(w[j / 2] >> (16 * (j % 2)));
+      l[j] = DT == FG_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) l[j] = __builtin_isnan(l[j]) ? -__builtin_inff() : l[j];
+}
+
+// Calls f(i, l) for each four logits l from token i on, i = first, first + step, .. in front of end; those from end on are -inf.  U whole
+// fours are loaded at a time, with no branch between the loads, which would wait for each.
+template <int DT, int U, class F>
+__device__ __forceinline__ void sweep(const void* row, int first, int step, int end, F f) {
+  int i = first;
+  for (; i + (U - 1) * step + 4 <= end; i += U * step) {
+    float l[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) four<DT>(row, i + u * step, l[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) f(i + u * step, l[u]);
+  }
+#pragma unroll 1
+  for (; i < end; i += step) {
+    float l[4];
+    if (i + 4 <= end) {
+      four<DT>(row, i, l);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l[j] = i + j < end ? one<DT>(row, i + j) : -__builtin_inff();
+    }
+    f(i, l);
   }
 }
 
@@ -105,7 +125,7 @@ struct Powers {
 };
 __device__ __forceinline__ double weight(const Powers& t, double y, int bits) {
   // k to the nearest by adding 3 2^51, whose last bits it then is; the power of two goes into the exponent's bits.  (Conversions and
-  // ldexp run at a part of the additions' rate: 256 rows of 150001 with mixed settings 201 us, now 197.)
+  // ldexp run at a part of the additions' rate: 256 rows of 150001 with mixed settings 201 us against 197.)
   const double at = __builtin_fma(y, 64.0, 0x1.8p52);
   const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, at);
   const double x = __builtin_fma(at - 0x1.8p52, 0.015625, -y) * 0.6931471805599453;
@@ -315,10 +335,7 @@ __global__ void __launch_bounds__(kThreads) sample_extremes_kernel(const SampleA
   const float inf = __builtin_inff(), log2e = 1.4426950408889634f;
   float mx = -inf, mn = inf, sum = 0.f;
   int arg = -1;
-#pragma unroll 2
-  for (int i = c * a.chunk + 4 * threadIdx.x; i < end; i += 4 * kThreads) {
-    float l[4];
-    four<DT>(row, i, end, l);
+  sweep<DT, 2>(row, c * a.chunk + 4 * threadIdx.x, 4 * kThreads, end, [&](int i, const float (&l)[4]) {
     const float was = mx;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -333,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) sample_extremes_kernel(const SampleA
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum += __builtin_amdgcn_exp2f((l[j] - mx) * log2e);
     }
-  }
+  });
   auto join = [&](float m2, float n2, int a2, float s2) {
     if (a2 < 0) return;
     if (arg < 0 || m2 > mx || (m2 == mx && a2 < arg)) {
@@ -380,10 +397,7 @@ __global__ void __launch_bounds__(kThreads) sample_histogram_kernel(const Sample
   const void* row = row_of(a, b, DT);
   const int end = min(a.V, (c + 1) * a.chunk);
   const double scale = bin_scale(r, a.bits), top = most(a.bits);
-#pragma unroll 2
-  for (int i = c * a.chunk + 4 * threadIdx.x; i < end; i += 4 * kThreads) {
-    float l[4];
-    four<DT>(row, i, end, l);
+  sweep<DT, 2>(row, c * a.chunk + 4 * threadIdx.x, 4 * kThreads, end, [&](int, const float (&l)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double y = exponent(r, l[j]);
@@ -393,7 +407,7 @@ __global__ void __launch_bounds__(kThreads) sample_histogram_kernel(const Sample
       if (r.by_p) atomicAdd(reinterpret_cast<unsigned long long*>(&mass[bin]), (unsigned long long)whole(weight(powers, y, a.bits)));
       atomicAdd(&count[bin], 1u);
     }
-  }
+  });
   __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
     if (a.chunks == 1) {
@@ -819,24 +833,19 @@ __global__ void __launch_bounds__(kThreads, 8) sample_borders_kernel(const Sampl
   if (fits) {
     const int end = min(a.V, (c + 1) * a.chunk);
     const float least = floor_of(r, (last + 1.0) / scale);
-    for (int i = c * a.chunk + 4 * threadIdx.x; i < end; i += 8 * kThreads) {
-      float l[2][4];
-      four<DT>(row, i, end, l[0]);
-      four<DT>(row, min(i + 4 * kThreads, end), end, l[1]);
+    sweep<DT, 2>(row, c * a.chunk + 4 * threadIdx.x, 4 * kThreads, end, [&](int i, const float (&l)[4]) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (!(l[u][j] >= least)) continue;
-          const double y = exponent(r, l[u][j]);
-          if (!(y < top)) continue;
-          const int bin = bin_of(y, scale);
-          if (whole_row ? bin <= last : q.border_bin(bin)) {
-            const uint32_t at = atomicAdd(&m.listed, 1u);  // the histogram has counted them: below kList
-            if (at < kList) m.list[at] = (uint64_t)key_of(l[u][j]) << 32 | (uint32_t)(i + 4 * kThreads * u + j);
-          }
+      for (int j = 0; j < 4; ++j) {
+        if (!(l[j] >= least)) continue;
+        const double y = exponent(r, l[j]);
+        if (!(y < top)) continue;
+        const int bin = bin_of(y, scale);
+        if (whole_row ? bin <= last : q.border_bin(bin)) {
+          const uint32_t at = atomicAdd(&m.listed, 1u);  // the histogram has counted them: below kList
+          if (at < kList) m.list[at] = (uint64_t)key_of(l[j]) << 32 | (uint32_t)(i + j);
         }
-    }
+      }
+    });
   }
   if (a.chunks > 1) {
     __syncthreads();
@@ -856,12 +865,12 @@ __global__ void __launch_bounds__(kThreads, 8) sample_borders_kernel(const Sampl
 
 // ------------------------------------------------------------------------------------------------ sums in the order of the indexes
 template <int DT>
-__global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) sample_sums_kernel(const SampleArgs a) {
   __shared__ Powers powers;
   __shared__ uint64_t part[kWaves];
   __shared__ int is_last, found;
   __shared__ uint64_t found_before;
-  const int b = blockIdx.x / a.chunks, c = blockIdx.x - b * a.chunks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.x / a.sum_chunks, c = blockIdx.x - b * a.sum_chunks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   RowState& s = reinterpret_cast<RowState*>(a.ws)[b];
   Row r;
   row_settings(a, b, r);
@@ -886,20 +895,17 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs 
     return w >= least ? whole(w) : 0;
   };
   // a wavefront sums up a stretch of its own
-  const int stretch = a.chunk / kWaves;
+  const int stretch = a.sum_chunk / kWaves;
   auto first_of = [&](int piece) { return piece * stretch; };
   const int begin = first_of(c * kWaves + wave), end = min(a.V, begin + stretch);
   uint64_t sum = 0;
-#pragma unroll 2
-  for (int i = begin + 4 * lane; i < end; i += 256) {
-    float l[4];
-    four<DT>(row, i, end, l);
+  sweep<DT, 4>(row, begin + 4 * lane, 256, end, [&](int i, const float (&l)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum += value(l[j], i + j);
-  }
+  });
   sum = wave_sum64(sum);
   if (lane == 0) put_far(&s.wave_mass[c * kWaves + wave], sum);
-  if (!last_of_row(&s.ticket[1], a.chunks, &is_last)) return;
+  if (!last_of_row(&s.ticket[1], a.sum_chunks, &is_last)) return;
   // the stretch in which the sum passes its mark, then the token: a thread takes some neighbours each
   auto pick = [&](uint64_t v, uint64_t base, uint64_t target, int id) {  // the thread whose values reach it
     uint64_t all;
@@ -910,7 +916,7 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(const SampleArgs 
     }
     __syncthreads();
   };
-  const int pieces = a.chunks * kWaves;  // 1024 at most
+  const int pieces = a.sum_chunks * kWaves;  // 1024 at most
   const uint64_t mine = (int)threadIdx.x < pieces ? get_far(&s.wave_mass[threadIdx.x]) : 0;
   uint64_t total;
   block_scan(mine, part, &total);
@@ -942,6 +948,10 @@ size_t sample_plan(SampleArgs& a) {
   const int64_t chunks = std::min<int64_t>(most_chunks, std::max<int64_t>(1, 2 * (int64_t)device_cus() / std::max(a.B, 1)));
   a.chunk = (int)(((a.V + chunks - 1) / chunks + unit - 1) / unit * unit);
   a.chunks = (a.V + a.chunk - 1) / a.chunk;
+  // The sums in pieces of half that, where it is 32768 columns or more (and a row's stretches stay as many as a workgroup's threads): rows that are settled before leave their CUs to the others (256 rows of 150001: mixed settings 192 us, now 169,
+  // top-p 0.95 for all 185, now 192).
+  a.sum_chunk = a.chunk >= 8 * unit && a.chunks <= kMaxChunks / 2 ? (int)((a.chunk / 2 + unit - 1) / unit * unit) : a.chunk;
+  a.sum_chunks = (a.V + a.sum_chunk - 1) / a.sum_chunk;
   int log = 0;
   while ((1LL << log) < a.V) ++log;
   a.bits = std::min(46, 62 - log);  // the sum of all weights stays below 2^63
@@ -957,7 +967,7 @@ hipError_t launch_sample(const SampleArgs& a, int dt, hipStream_t st) {
       hipLaunchKernelGGL((sample_histogram_kernel<DT>), grid, block, 0, st, a);
       hipLaunchKernelGGL((sample_borders_kernel<DT>), grid, block, 0, st, a);
     }
-    hipLaunchKernelGGL((sample_sums_kernel<DT>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((sample_sums_kernel<DT>), dim3((unsigned)((int64_t)a.B * a.sum_chunks)), block, 0, st, a);
     note_kernel("sample_extremes_kernel%s + sample_sums_kernel chunks=%d",
                 a.cuts ? " + sample_histogram_kernel + sample_borders_kernel" : "", a.chunks);
     return hipGetLastError();

@@ -238,3 +238,13 @@ def test_borders_of_both_kinds_near_and_far(spread, dt):
         _check(logits, uniform, top_k=k, top_p=p)
     _check(logits, uniform, top_k=k, min_p=0.02)
     _check(logits[:2], uniform[:2], top_k=5000, top_p=0.8, temperature=0.5)  # a row in more chunks
+
+
+@pytest.mark.parametrize("b,v", [(270, 40001), (1, 3000000), (9, 1200000)])
+def test_rows_that_are_cut_up_more_finely_for_the_sums(b, v):
+    """Many rows of long vocabularies, of which some are settled by few tokens and others need every sum; rows of most chunks."""
+    logits, uniform = _logits(b, v, FP)
+    k = torch.tensor([0, 5, 0, 0], dtype=torch.int32).repeat(b)[:b]
+    p = torch.tensor([1.0, 0.9, 0.97, 0.3]).repeat(b)[:b]
+    _check(logits, uniform, top_k=k, top_p=p)
+    _check(logits[:9], uniform[:9])
